@@ -41,7 +41,27 @@ class _Page(ctypes.Structure):
     _fields_ = [("k", ctypes.c_void_p), ("v", ctypes.c_void_p), ("hk", ctypes.c_void_p), ("hv", ctypes.c_void_p)]
 
 
+class _Cache(ctypes.Structure):
+    _fields_ = [("k", ctypes.c_void_p), ("v", ctypes.c_void_p), ("n_layers", ctypes.c_uint32),
+                ("n_pages", ctypes.c_uint32), ("page_keys", ctypes.c_uint32)]
+
+
+class _Mask(ctypes.Structure):
+    _fields_ = [("n_tok", ctypes.c_uint32), ("window", ctypes.c_uint32), ("sinks", ctypes.c_uint32),
+                ("tree", ctypes.c_uint32)]
+
+
+class _Append(ctypes.Structure):
+    _fields_ = [("q", ctypes.c_void_p), ("k", ctypes.c_void_p), ("v", ctypes.c_void_p),
+                ("q_set", ctypes.c_int64), ("q_tok", ctypes.c_int64), ("k_set", ctypes.c_int64),
+                ("k_tok", ctypes.c_int64), ("v_set", ctypes.c_int64), ("v_tok", ctypes.c_int64),
+                ("wq", ctypes.c_void_p), ("wk", ctypes.c_void_p), ("freqs", ctypes.c_void_p), ("pos", ctypes.c_void_p),
+                ("dtype", ctypes.c_uint32), ("w_dtype", ctypes.c_uint32), ("rot", ctypes.c_uint32),
+                ("interleaved", ctypes.c_uint32), ("eps", ctypes.c_float), ("scale", ctypes.c_float)]
+
+
 _P = ctypes.c_void_p
+_U = ctypes.c_uint32
 _SIGS = {
     "pa_cuda_available": (ctypes.c_int, []),
     "pa_cuda_abi_version": (ctypes.c_int, []),
@@ -96,6 +116,19 @@ _SIGS = {
     "pa_cuda_graph_calls": (ctypes.c_uint64, [_P]),
     "pa_cuda_attn_noalloc": (ctypes.c_int, [ctypes.POINTER(_Shape), _P, _P, _P, ctypes.c_uint32, _P, _P, _P, _P,
                                             ctypes.POINTER(ctypes.c_char_p)]),
+    "pa_cuda_cache_plan_create": (ctypes.c_int, [_P, ctypes.POINTER(_Shape), ctypes.POINTER(_Cache), _U, _U,
+                                                 ctypes.POINTER(_Mask), ctypes.POINTER(_P)]),
+    "pa_cuda_cache_plan_kernel": (ctypes.c_char_p, [_P]),
+    "pa_cuda_cache_plan_destroy": (None, [_P]),
+    "pa_cuda_cache_attn": (ctypes.c_int, [_P, _U, _P, _P, _P, _P, _P, _P, _P, _P, _P]),
+    "pa_cuda_cache_attn_reply": (ctypes.c_int, [_P, _U, _P, _P, _P, _P, _P, _P, _P, _P]),
+    "pa_cuda_cache_append": (ctypes.c_int, [_P, ctypes.POINTER(_Shape), ctypes.POINTER(_Cache), _U,
+                                            ctypes.POINTER(_Append), _U, _U, _P, _U, _P, _P, _P]),
+    "pa_cuda_cache_rows": (ctypes.c_int, [_P, ctypes.POINTER(_Shape), ctypes.POINTER(_Cache), _U, _U, _U, _P, _U, _P,
+                                          _P, _P, _P]),
+    "pa_cuda_cache_copy_pages": (ctypes.c_int, [_P, ctypes.POINTER(_Shape), ctypes.POINTER(_Cache), _P, _P, _U, _P]),
+    "pa_cuda_cache_compact": (ctypes.c_int, [_P, ctypes.POINTER(_Shape), ctypes.POINTER(_Cache), _U, _U, _P, _U, _P, _P,
+                                             _P, _P, _P]),
 }
 
 _lib = None
@@ -506,3 +539,227 @@ class Engine:
     @property
     def exec_ms(self) -> float:
         return float(lib().pa_cuda_exec_ms(self.ctx.handle))
+
+
+# ---------------------------------------------------------------- paged cache
+def _want(ctx: Context, t, name: str, dtype, shape):
+    """Pointer of a contiguous tensor of this type and shape on the context's device; anything else is an error."""
+    if t.dtype is not dtype or tuple(t.shape) != shape or not t.is_contiguous() or t.get_device() != ctx.device:
+        raise PaCudaError(EINVAL, f"{name}: needs a contiguous {dtype} tensor {shape} on cuda:{ctx.device}, got "
+                                  f"{t.dtype} {tuple(t.shape)} on {t.device}")
+    return t.data_ptr()
+
+
+def _stream_on(ctx: Context, stream) -> int:
+    """_stream_ptr for the context's device, whatever the current one is."""
+    if stream is None:
+        import torch
+        stream = torch.cuda.current_stream(ctx.device)
+    return _stream_ptr(stream)
+
+
+class Cache:
+    """A paged device cache (pa_cuda_cache): K and V uint8 [n_layers][n_pages][page_keys][row bytes] on one device, rows of
+    nkv heads in the F16, Q8_0 or Q4_0 format. Tables, lengths and positions stay with the caller."""
+
+    def __init__(self, hd: int, nkv: int, quant: int = Q8_0, n_layers: int = 1, n_pages: int = 1, page_keys: int = 256,
+                 device: int = 0, rs: int | None = None):
+        import torch
+        hb = head_bytes(quant, hd)
+        rs = rs if rs is not None else (nkv * hb + 15) // 16 * 16
+        K = torch.zeros((n_layers, n_pages, page_keys, rs), dtype=torch.uint8, device=f"cuda:{device}")
+        self._set(K, torch.zeros_like(K), hd, nkv, quant)
+
+    @classmethod
+    def of(cls, K, V, hd: int, nkv: int, quant: int) -> "Cache":
+        """The same over tensors the caller holds."""
+        c = cls.__new__(cls)
+        c._set(K, V, hd, nkv, quant)
+        return c
+
+    def _set(self, K, V, hd, nkv, quant):
+        import torch
+        for name, t in (("K", K), ("V", V)):
+            if t.dtype is not torch.uint8 or t.dim() != 4 or not t.is_contiguous() or not t.is_cuda:
+                raise PaCudaError(EINVAL, f"cache {name}: needs a contiguous CUDA uint8 tensor [layers][pages][page_keys]"
+                                          f"[row bytes], got {t.dtype} {tuple(t.shape)}")
+        if K.shape != V.shape or K.device != V.device:
+            raise PaCudaError(EINVAL, "cache K and V differ in shape or device")
+        self.K, self.V, self.hd, self.nkv, self.quant = K, V, hd, nkv, quant
+        self.n_layers, self.n_pages, self.page_keys, self.rs = K.shape
+        self.hb = head_bytes(quant, hd)
+        self.device = K.get_device()
+        self._c = _Cache(K.data_ptr(), V.data_ptr(), self.n_layers, self.n_pages, self.page_keys)
+
+    def shape(self, rows: int) -> _Shape:
+        return _Shape(self.hd, self.nkv, rows, self.quant, self.rs, self.hb)
+
+    def on(self, ctx: Context):
+        if self.device != ctx.device:
+            raise PaCudaError(EINVAL, f"the cache is on cuda:{self.device}, the context on cuda:{ctx.device}")
+        return ctypes.byref(self._c)
+
+
+class CachePlan:
+    """Attention of n_sets sequences x n_tok query tokens over a paged cache (pa_cuda_cache_plan_create): causal, with a
+    sliding window and sinks (window > 0), or for drafted tokens that form a tree (tree=True). One call at a time."""
+
+    def __init__(self, ctx: Context, cache: Cache, n_sets: int, n_tok: int, gqa: int, max_pages: int, window: int = 0,
+                 sinks: int = 0, tree: bool = False):
+        self.ctx, self.cache, self.n_sets, self.n_tok, self.gqa = ctx, cache, n_sets, n_tok, gqa
+        self.max_pages, self.tree = max_pages, bool(tree)
+        self._h = _P()
+        sh, mask = cache.shape(gqa * n_tok), _Mask(n_tok, window, sinks, 1 if tree else 0)
+        ctx.check(lib().pa_cuda_cache_plan_create(ctx.handle, ctypes.byref(sh), cache.on(ctx), n_sets, max_pages,
+                                                  ctypes.byref(mask), ctypes.byref(self._h)), "cache_plan_create")
+        self._rows = (n_sets, cache.nkv, gqa * n_tok)
+
+    @property
+    def kernel(self) -> str:
+        """Name of the attention kernel the plan launches."""
+        return lib().pa_cuda_cache_plan_kernel(self._h).decode()
+
+    def _args(self, layer, Qs, table, n_keys, q_pos, tree):
+        import torch
+        ctx, i32, per = self.ctx, torch.int32, (self.n_sets,)
+        if (tree is not None) != self.tree:
+            raise PaCudaError(EINVAL, "a tree plan takes the tree's masks, another plan none")
+        return (self._h, layer, _want(ctx, Qs, "Qs", torch.float16, self._rows + (self.cache.hd,)),
+                _want(ctx, table, "table", i32, (self.n_sets, self.max_pages)), _want(ctx, n_keys, "n_keys", i32, per),
+                None if q_pos is None else _want(ctx, q_pos, "q_pos", i32, per),
+                None if tree is None else _want(ctx, tree, "tree", torch.int64, (self.n_sets, self.n_tok)))
+
+    def run(self, layer: int, Qs, table, n_keys, q_pos=None, tree=None, out=None, stream=None):
+        """The unnormalised partial (O, m, l) (pa_cuda_cache_attn). Qs: f16(q * scale) [n_sets][nkv][gqa * n_tok][hd],
+        row g * n_tok + t; table int32 [n_sets][max_pages]; n_keys, q_pos int32 [n_sets]; tree int64 [n_sets][n_tok]."""
+        import torch
+        args, f32 = self._args(layer, Qs, table, n_keys, q_pos, tree), torch.float32
+        if out is None:
+            O = torch.empty(Qs.shape, dtype=f32, device=Qs.device)
+            m = torch.empty(self._rows, dtype=f32, device=Qs.device)
+            out = (O, m, torch.empty_like(m))
+        O, m, l = out
+        self.ctx.check(lib().pa_cuda_cache_attn(*args, _want(self.ctx, O, "O", f32, tuple(Qs.shape)),
+                                                _want(self.ctx, m, "m", f32, self._rows),
+                                                _want(self.ctx, l, "l", f32, self._rows), _stream_on(self.ctx, stream)),
+                       "cache_attn")
+        return O, m, l
+
+    def reply(self, layer: int, Qs, table, n_keys, q_pos=None, tree=None, out=None, stream=None):
+        """The same, normalised: (f16 O / l, lse) (pa_cuda_cache_attn_reply)."""
+        import torch
+        args = self._args(layer, Qs, table, n_keys, q_pos, tree)
+        if out is None:
+            out = (torch.empty(Qs.shape, dtype=torch.float16, device=Qs.device),
+                   torch.empty(self._rows, dtype=torch.float32, device=Qs.device))
+        Oh, lse = out
+        self.ctx.check(lib().pa_cuda_cache_attn_reply(*args, _want(self.ctx, Oh, "Oh", torch.float16, tuple(Qs.shape)),
+                                                      _want(self.ctx, lse, "lse", torch.float32, self._rows),
+                                                      _stream_on(self.ctx, stream)), "cache_attn_reply")
+        return Oh, lse
+
+    def close(self):
+        if self._h:
+            lib().pa_cuda_cache_plan_destroy(self._h)
+            self._h = _P()
+
+    def __del__(self):  # pragma: no cover
+        try:
+            self.close()
+        except Exception:
+            pass
+
+
+def cache_append(ctx: Context, cache: Cache, layer: int, q, k, v, table, start, pos=None, wq=None, wk=None, freqs=None,
+                 eps: float = 1e-6, scale: float = 1.0, interleaved: bool = False, out=None, stream=None):
+    """Head norm and rotation of new queries and keys, and the append of their rows (pa_cuda_cache_append). q
+    [n_sets][n_tok][nkv * gqa][hd], k, v [n_sets][n_tok][nkv][hd]: f16, bf16 or f32, any strides over sets and tokens; wq, wk
+    [hd]; freqs float64 [rot / 2]; table int32 [n_sets][max_pages]; start int32 [n_sets]: key index of token 0; pos int32
+    [n_sets][n_tok] (< 0: padding). Returns Qs f16 [n_sets][nkv][gqa * n_tok][hd], what CachePlan takes."""
+    import torch
+    S, T, nq, hd = q.shape
+    kv = (S, T, cache.nkv, cache.hd)
+    kinds = {torch.float16: 0, torch.bfloat16: 1, torch.float32: 2}
+    if hd != cache.hd or nq == 0 or nq % cache.nkv or tuple(k.shape) != kv or tuple(v.shape) != kv or q.dtype not in kinds:
+        raise PaCudaError(EINVAL, f"cache_append: q {tuple(q.shape)} {q.dtype}, k {tuple(k.shape)}, v {tuple(v.shape)} do "
+                                  f"not fit nkv {cache.nkv}, hd {cache.hd} (f16, bf16 or f32)")
+    st = []
+    for name, t in (("q", q), ("k", k), ("v", v)):
+        s = t.stride()
+        if t.dtype is not q.dtype or t.get_device() != ctx.device or (s[3] != 1 and hd > 1) or (s[2] != hd and t.shape[2] > 1):
+            raise PaCudaError(EINVAL, f"cache_append: {name} needs heads of hd consecutive elements, hd apart, of q's type, "
+                                      f"on cuda:{ctx.device}")
+        st += [s[0], s[1]]
+    w_dtype = kinds[q.dtype]
+    for name, w in (("wq", wq), ("wk", wk)):
+        if w is not None:
+            w_dtype = kinds.get(w.dtype, 3)
+            _want(ctx, w, name, w.dtype, (hd,))
+    if wq is not None and wk is not None and wq.dtype is not wk.dtype:
+        raise PaCudaError(EINVAL, "cache_append: wq and wk differ in type")
+    rot = 0 if freqs is None else 2 * freqs.numel()
+    a = _Append(q.data_ptr(), k.data_ptr(), v.data_ptr(), *st, _ptr(wq) or None, _ptr(wk) or None,
+                None if freqs is None else _want(ctx, freqs, "freqs", torch.float64, (rot // 2,)),
+                None if pos is None else _want(ctx, pos, "pos", torch.int32, (S, T)),
+                kinds[q.dtype], w_dtype, rot, 1 if interleaved else 0, eps, scale)
+    rows = (S, cache.nkv, nq // cache.nkv * T, hd)
+    if out is None:
+        out = torch.empty(rows, dtype=torch.float16, device=q.device)
+    if table.dim() != 2:
+        raise PaCudaError(EINVAL, "table: needs int32 [n_sets][max_pages]")
+    sh = cache.shape(max(1, nq // cache.nkv * T))
+    ctx.check(lib().pa_cuda_cache_append(ctx.handle, ctypes.byref(sh), cache.on(ctx), layer, ctypes.byref(a), S, T,
+                                         _want(ctx, table, "table", torch.int32, (S, table.shape[1])), table.shape[1],
+                                         _want(ctx, start, "start", torch.int32, (S,)),
+                                         _want(ctx, out, "out", torch.float16, rows), _stream_on(ctx, stream)),
+              "cache_append")
+    return out
+
+
+def cache_rows(ctx: Context, cache: Cache, layer: int, table, first, n: int, out=None, stream=None):
+    """Keys first[s] .. first[s] + n - 1 of every sequence as the f16 values their rows stand for: (K, V)
+    [n_sets][n][nkv][hd] (pa_cuda_cache_rows)."""
+    import torch
+    S = table.shape[0]
+    shape = (S, n, cache.nkv, cache.hd)
+    if out is None:
+        K = torch.empty(shape, dtype=torch.float16, device=table.device)
+        out = (K, torch.empty_like(K))
+    sh = cache.shape(1)
+    ctx.check(lib().pa_cuda_cache_rows(ctx.handle, ctypes.byref(sh), cache.on(ctx), layer, S, n,
+                                       _want(ctx, table, "table", torch.int32, (S, table.shape[1])), table.shape[1],
+                                       _want(ctx, first, "first", torch.int32, (S,)),
+                                       _want(ctx, out[0], "K", torch.float16, shape),
+                                       _want(ctx, out[1], "V", torch.float16, shape), _stream_on(ctx, stream)), "cache_rows")
+    return out
+
+
+def cache_copy_pages(ctx: Context, cache: Cache, src, dst, stream=None):
+    """Pages src[i] -> dst[i] (int32 [n]) of every layer, K and V (pa_cuda_cache_copy_pages): a sequence forked off a shared
+    prefix copies the page it will write to. No page is both read and written in one call."""
+    import torch
+    n = src.numel()
+    sh = cache.shape(1)
+    ctx.check(lib().pa_cuda_cache_copy_pages(ctx.handle, ctypes.byref(sh), cache.on(ctx),
+                                             _want(ctx, src, "src", torch.int32, (n,)),
+                                             _want(ctx, dst, "dst", torch.int32, (n,)), n, _stream_on(ctx, stream)),
+              "cache_copy_pages")
+
+
+def cache_compact(ctx: Context, cache: Cache, table, start, path, count, out=None, stream=None):
+    """Keeps the accepted rows of a verified draft (pa_cuda_cache_compact): rows start[s] + path[s][i] move to start[s] + i,
+    i < count[s], in every layer. start, count int32 [n_sets], path int32 [n_sets][n_tok], rising. Returns the new n_keys,
+    start + count."""
+    import torch
+    S, T = path.shape
+    if out is None:
+        out = torch.empty((S,), dtype=torch.int32, device=path.device)
+    sh = cache.shape(1)
+    ctx.check(lib().pa_cuda_cache_compact(ctx.handle, ctypes.byref(sh), cache.on(ctx), S, T,
+                                          _want(ctx, table, "table", torch.int32, (S, table.shape[1])), table.shape[1],
+                                          _want(ctx, start, "start", torch.int32, (S,)),
+                                          _want(ctx, path, "path", torch.int32, (S, T)),
+                                          _want(ctx, count, "count", torch.int32, (S,)),
+                                          _want(ctx, out, "out", torch.int32, (S,)), _stream_on(ctx, stream)),
+              "cache_compact")
+    return out

@@ -1,0 +1,351 @@
+// pa_cache_host.h - the host side of the paged-cache entry points of include/pa_cuda.h: argument checks, plans and
+// launches. Part of pa_cuda.cu, whose contexts and checks it uses.
+#pragma once
+
+namespace {
+
+// the context's device for the length of a call; the caller's current device afterwards
+struct DeviceScope {
+    int before = -1;
+    bool ok;
+    explicit DeviceScope(int device) {
+        ok = cudaGetDevice(&before) == cudaSuccess && (before == device || cudaSetDevice(device) == cudaSuccess);
+        if (before == device) before = -1;
+    }
+    ~DeviceScope() {
+        if (before >= 0) cudaSetDevice(before);
+    }
+    DeviceScope(const DeviceScope &) = delete;
+    DeviceScope &operator=(const DeviceScope &) = delete;
+};
+
+constexpr uint64_t kCacheMaxKeys = 1ull << 30;   // keys a page table reaches: key indexes and sums of them stay in 32 bits
+
+int check_cache(pa_cuda_ctx *ctx, const pa_cuda_shape *sh, const pa_cuda_cache *c) {
+    int rc = check_shape(ctx, sh);
+    if (rc) return rc;
+    if (!c || !c->k || !c->v) return fail(ctx, PA_CUDA_EINVAL, "cache is null");
+    if (((uintptr_t) c->k | (uintptr_t) c->v) & 15) return fail(ctx, PA_CUDA_EINVAL, "cache K/V must be 16-byte aligned");
+    if (c->page_keys == 0 || c->page_keys % 64) return fail(ctx, PA_CUDA_EUNSUPPORTED, "page_keys must be a multiple of 64");
+    if (c->n_layers == 0 || c->n_pages == 0) return fail(ctx, PA_CUDA_EINVAL, "a cache needs a layer and a page");
+    if (c->n_layers > 32767) return fail(ctx, PA_CUDA_EUNSUPPORTED, "more than 32,767 layers");
+    // rows of the whole cache are numbered in 31 bits (tensor-map coordinates)
+    if ((uint64_t) c->n_pages * c->page_keys > 0x7FFFFFFFull / c->n_layers)
+        return fail(ctx, PA_CUDA_EUNSUPPORTED, "more than 2^31 - 1 rows in the cache");
+    return PA_CUDA_OK;
+}
+int check_table(pa_cuda_ctx *ctx, const pa_cuda_cache *c, uint32_t n_sets, uint32_t max_pages) {
+    if (max_pages == 0 || (uint64_t) max_pages * c->page_keys > kCacheMaxKeys)
+        return fail(ctx, PA_CUDA_EINVAL, "max_pages must be >= 1 and reach at most 2^30 keys");
+    if (n_sets > 65535) return fail(ctx, PA_CUDA_EUNSUPPORTED, "more than 65,535 sequences");
+    return PA_CUDA_OK;
+}
+uint64_t layer_bytes(const pa_cuda_shape &sh, const pa_cuda_cache &c) { return (uint64_t) c.n_pages * c.page_keys * sh.rs; }
+
+}  // namespace
+
+struct pa_cuda_cache_plan {
+    pa_cuda_ctx *ctx = nullptr;
+    pa_cuda_shape sh{};
+    pa_cuda_cache cache{};
+    pa_cuda_mask mask{};
+    uint32_t n_sets = 0, max_pages = 0;
+    const char *kernel = "";
+};
+
+namespace {
+
+pa::pg::View view_of(const pa_cuda_cache_plan *p, const int32_t *table, const int32_t *n_keys, const int32_t *q_pos,
+                     const uint64_t *tree) {
+    pa::pg::View v{};
+    v.table = table;
+    v.n_keys = n_keys;
+    v.q_pos = q_pos;
+    v.tree = p->mask.tree ? tree : nullptr;
+    v.n_sets = p->n_sets;
+    v.max_pages = p->max_pages;
+    v.n_pages = p->cache.n_pages;
+    v.page_keys = p->cache.page_keys;
+    v.n_tok = p->mask.n_tok;
+    v.window = p->mask.window;
+    v.sinks = p->mask.sinks;
+    v.status = p->ctx->d_status;
+    return v;
+}
+
+template <int HD>
+void launch_row_attn(const pa_cuda_cache_plan *p, const pa::pg::AttnParams &a, cudaStream_t st) {
+    const dim3 grid(p->sh.rows, p->sh.nkv, p->n_sets);
+    if (p->sh.quant == PA_CUDA_Q8_0) pa::pg::row_attn_kernel<HD, 1><<<grid, 32, 0, st>>>(a);
+    else if (p->sh.quant == PA_CUDA_Q4_0) pa::pg::row_attn_kernel<HD, 2><<<grid, 32, 0, st>>>(a);
+    else pa::pg::row_attn_kernel<HD, 0><<<grid, 32, 0, st>>>(a);
+}
+
+// O, m, l or Oh, lse: one of the two forms
+int cache_attn(pa_cuda_cache_plan *p, uint32_t layer, const uint16_t *Qs, const int32_t *table, const int32_t *n_keys,
+               const int32_t *q_pos, const uint64_t *tree, float *O, float *m, float *l, uint16_t *Oh, float *lse, void *stream) {
+    if (!p) return PA_CUDA_EINVAL;
+    pa_cuda_ctx *ctx = p->ctx;
+    if (layer >= p->cache.n_layers) return fail(ctx, PA_CUDA_EINVAL, "layer out of range");
+    if (!Qs || !table || !n_keys) return fail(ctx, PA_CUDA_EINVAL, "null argument");
+    if ((p->mask.tree != 0) != (tree != nullptr)) return fail(ctx, PA_CUDA_EINVAL, "a tree plan takes the tree's masks, another plan none");
+    if (((uintptr_t) Qs | (uintptr_t) O | (uintptr_t) Oh) & 15) return fail(ctx, PA_CUDA_EINVAL, "Q and O must be 16-byte aligned");
+    DeviceScope dev(ctx->device);
+    if (!dev.ok) return fail(ctx, PA_CUDA_ECUDA, "cudaSetDevice");
+    cudaStream_t st = pick(ctx, stream);
+    pa::pg::AttnParams a{};
+    a.v = view_of(p, table, n_keys, q_pos, tree);
+    a.k = p->cache.k + layer * layer_bytes(p->sh, p->cache);
+    a.v_rows = p->cache.v + layer * layer_bytes(p->sh, p->cache);
+    a.Qs = Qs;
+    a.rs = p->sh.rs;
+    a.hb = p->sh.hb;
+    a.nkv = p->sh.nkv;
+    a.rows = p->sh.rows;
+    a.O = O;
+    a.M = m;
+    a.L = l;
+    a.Oh = Oh;
+    a.lse = lse;
+    if (p->sh.hd == 128) launch_row_attn<128>(p, a, st);
+    else launch_row_attn<256>(p, a, st);
+    PA_CK(cudaGetLastError(), "cache attention launch");
+    ctx->launches++;
+    return PA_CUDA_OK;
+}
+
+template <int HD, int DT>
+void launch_append_q(const pa::pg::AppendParams &a, uint32_t quant, dim3 grid, uint32_t hpb, cudaStream_t st) {
+    constexpr int threads = 32 * pa::pg::APPEND_WARPS;
+    if (quant == PA_CUDA_Q8_0) pa::pg::append_kernel<HD, DT, 1><<<grid, threads, 0, st>>>(a, hpb);
+    else if (quant == PA_CUDA_Q4_0) pa::pg::append_kernel<HD, DT, 2><<<grid, threads, 0, st>>>(a, hpb);
+    else pa::pg::append_kernel<HD, DT, 0><<<grid, threads, 0, st>>>(a, hpb);
+}
+template <int HD>
+void launch_append(const pa::pg::AppendParams &a, uint32_t dtype, uint32_t quant, dim3 grid, uint32_t hpb, cudaStream_t st) {
+    if (dtype == PA_CUDA_T_F16) launch_append_q<HD, pa::pg::DT_F16>(a, quant, grid, hpb, st);
+    else if (dtype == PA_CUDA_T_BF16) launch_append_q<HD, pa::pg::DT_BF16>(a, quant, grid, hpb, st);
+    else launch_append_q<HD, pa::pg::DT_F32>(a, quant, grid, hpb, st);
+}
+template <int HD>
+void launch_rows(const pa::pg::RowsParams &a, uint32_t quant, unsigned blocks, cudaStream_t st) {
+    if (quant == PA_CUDA_Q8_0) pa::pg::rows_kernel<HD, 1><<<blocks, 256, 0, st>>>(a);
+    else if (quant == PA_CUDA_Q4_0) pa::pg::rows_kernel<HD, 2><<<blocks, 256, 0, st>>>(a);
+    else pa::pg::rows_kernel<HD, 0><<<blocks, 256, 0, st>>>(a);
+}
+
+}  // namespace
+
+extern "C" {
+
+int pa_cuda_cache_plan_create(pa_cuda_ctx *ctx, const pa_cuda_shape *shape, const pa_cuda_cache *cache, uint32_t n_sets,
+                              uint32_t max_pages, const pa_cuda_mask *mask, pa_cuda_cache_plan **out) {
+    if (!ctx || !out) return PA_CUDA_EINVAL;
+    *out = nullptr;
+    int rc = check_cache(ctx, shape, cache);
+    if (rc || (rc = check_table(ctx, cache, n_sets, max_pages))) return rc;
+    if (n_sets == 0) return fail(ctx, PA_CUDA_EINVAL, "n_sets must be >= 1");
+    if (!mask || mask->n_tok == 0 || shape->rows % mask->n_tok) return fail(ctx, PA_CUDA_EINVAL, "rows must be a multiple of n_tok >= 1");
+    if (mask->window > kCacheMaxKeys) return fail(ctx, PA_CUDA_EINVAL, "window above 2^30 keys (0: none)");
+    if (mask->sinks && !mask->window) return fail(ctx, PA_CUDA_EINVAL, "sinks without a window");
+    if (mask->tree && mask->n_tok > 64) return fail(ctx, PA_CUDA_EUNSUPPORTED, "a tree has at most 64 tokens");
+    if (mask->tree && mask->window && mask->window < mask->n_tok)
+        return fail(ctx, PA_CUDA_EUNSUPPORTED, "a tree needs a window of at least n_tok keys");
+    if (ctx->qk_domain == PA_CUDA_QK_INT8)
+        return fail(ctx, PA_CUDA_EUNSUPPORTED, "the int8-domain QK does not cover the paged cache");
+    auto *p = new pa_cuda_cache_plan();
+    p->ctx = ctx;
+    p->sh = *shape;
+    p->cache = *cache;
+    p->mask = *mask;
+    p->n_sets = n_sets;
+    p->max_pages = max_pages;
+    p->kernel = "pa::pg::row_attn_kernel";
+    *out = p;
+    return PA_CUDA_OK;
+}
+const char *pa_cuda_cache_plan_kernel(const pa_cuda_cache_plan *plan) { return plan ? plan->kernel : ""; }
+void pa_cuda_cache_plan_destroy(pa_cuda_cache_plan *plan) { delete plan; }
+
+int pa_cuda_cache_attn(pa_cuda_cache_plan *plan, uint32_t layer, const uint16_t *Qs, const int32_t *table, const int32_t *n_keys,
+                       const int32_t *q_pos, const uint64_t *tree, float *O, float *m, float *l, void *stream) {
+    if (plan && (!O || !m || !l)) return fail(plan->ctx, PA_CUDA_EINVAL, "null argument");
+    return cache_attn(plan, layer, Qs, table, n_keys, q_pos, tree, O, m, l, nullptr, nullptr, stream);
+}
+int pa_cuda_cache_attn_reply(pa_cuda_cache_plan *plan, uint32_t layer, const uint16_t *Qs, const int32_t *table,
+                             const int32_t *n_keys, const int32_t *q_pos, const uint64_t *tree, uint16_t *Oh, float *lse,
+                             void *stream) {
+    if (plan && (!Oh || !lse)) return fail(plan->ctx, PA_CUDA_EINVAL, "null argument");
+    return cache_attn(plan, layer, Qs, table, n_keys, q_pos, tree, nullptr, nullptr, nullptr, Oh, lse, stream);
+}
+
+int pa_cuda_cache_append(pa_cuda_ctx *ctx, const pa_cuda_shape *shape, const pa_cuda_cache *cache, uint32_t layer,
+                         const pa_cuda_append *in, uint32_t n_sets, uint32_t n_tok, const int32_t *table, uint32_t max_pages,
+                         const int32_t *start, uint16_t *Qs, void *stream) {
+    if (!ctx) return PA_CUDA_EINVAL;
+    int rc = check_cache(ctx, shape, cache);
+    if (rc || (rc = check_table(ctx, cache, n_sets, max_pages))) return rc;
+    if (layer >= cache->n_layers) return fail(ctx, PA_CUDA_EINVAL, "layer out of range");
+    if (n_sets == 0 || n_tok == 0) return PA_CUDA_OK;
+    if (!in || !in->q || !in->k || !in->v || !table || !start || !Qs) return fail(ctx, PA_CUDA_EINVAL, "null argument");
+    if (shape->rows % n_tok) return fail(ctx, PA_CUDA_EINVAL, "rows must be a multiple of n_tok");
+    if ((uint64_t) n_sets * n_tok > 0x7FFFFFFFull) return fail(ctx, PA_CUDA_EUNSUPPORTED, "more than 2^31 - 1 tokens");
+    if (in->dtype > PA_CUDA_T_F32 || in->w_dtype > PA_CUDA_T_F32 || (in->w_dtype != in->dtype && in->w_dtype != PA_CUDA_T_F32))
+        return fail(ctx, PA_CUDA_EUNSUPPORTED, "inputs are f16, bf16 or f32; weights of the inputs' type or f32");
+    if (in->rot % 2 || in->rot > shape->hd || (in->rot && !in->freqs))
+        return fail(ctx, PA_CUDA_EINVAL, "rot must be even, at most hd, with rot / 2 frequencies");
+    if ((uintptr_t) Qs & 15) return fail(ctx, PA_CUDA_EINVAL, "Q must be 16-byte aligned");
+    DeviceScope dev(ctx->device);
+    if (!dev.ok) return fail(ctx, PA_CUDA_ECUDA, "cudaSetDevice");
+    pa::pg::AppendParams a{};
+    a.q = in->q;
+    a.k = in->k;
+    a.v = in->v;
+    a.q_set = in->q_set;
+    a.q_tok = in->q_tok;
+    a.k_set = in->k_set;
+    a.k_tok = in->k_tok;
+    a.v_set = in->v_set;
+    a.v_tok = in->v_tok;
+    a.wq = in->wq;
+    a.wk = in->wk;
+    a.freqs = in->freqs;
+    a.start = start;
+    a.pos = in->pos;
+    a.view.table = table;
+    a.view.n_sets = n_sets;
+    a.view.max_pages = max_pages;
+    a.view.n_pages = cache->n_pages;
+    a.view.page_keys = cache->page_keys;
+    a.view.n_tok = n_tok;
+    a.view.status = ctx->d_status;
+    a.K = cache->k + layer * layer_bytes(*shape, *cache);
+    a.V = cache->v + layer * layer_bytes(*shape, *cache);
+    a.Qs = Qs;
+    a.rs = shape->rs;
+    a.hb = shape->hb;
+    a.nkv = shape->nkv;
+    a.gqa = shape->rows / n_tok;
+    a.rot = in->rot;
+    a.eps = in->eps;
+    a.scale = in->scale;
+    a.inter = in->interleaved != 0;
+    a.w32 = in->w_dtype == PA_CUDA_T_F32;
+    // a lane's hd / 32 elements in one load where every head starts on such a boundary
+    const uint64_t size = in->dtype == PA_CUDA_T_F32 ? 4 : 2, vec = std::min<uint64_t>(16, shape->hd / 32 * size);
+    uint64_t odd = (uintptr_t) in->q | (uintptr_t) in->k | (uintptr_t) in->v;
+    for (int64_t s : {in->q_set, in->q_tok, in->k_set, in->k_tok, in->v_set, in->v_tok}) odd |= (uint64_t) s * size;
+    a.vec = odd % vec == 0;
+    const uint32_t heads = shape->nkv * (a.gqa + 2), hpb = std::min<uint32_t>(heads, 8);
+    const dim3 grid(n_sets * n_tok, (heads + hpb - 1) / hpb);
+    if (grid.y > 65535) return fail(ctx, PA_CUDA_EUNSUPPORTED, "too many heads");
+    if (shape->hd == 128) launch_append<128>(a, in->dtype, shape->quant, grid, hpb, pick(ctx, stream));
+    else launch_append<256>(a, in->dtype, shape->quant, grid, hpb, pick(ctx, stream));
+    PA_CK(cudaGetLastError(), "append launch");
+    ctx->launches++;
+    return PA_CUDA_OK;
+}
+
+int pa_cuda_cache_rows(pa_cuda_ctx *ctx, const pa_cuda_shape *shape, const pa_cuda_cache *cache, uint32_t layer, uint32_t n_sets,
+                       uint32_t n_tok, const int32_t *table, uint32_t max_pages, const int32_t *first, uint16_t *K, uint16_t *V,
+                       void *stream) {
+    if (!ctx) return PA_CUDA_EINVAL;
+    int rc = check_cache(ctx, shape, cache);
+    if (rc || (rc = check_table(ctx, cache, n_sets, max_pages))) return rc;
+    if (layer >= cache->n_layers) return fail(ctx, PA_CUDA_EINVAL, "layer out of range");
+    if (n_sets == 0 || n_tok == 0) return PA_CUDA_OK;
+    if (!table || !first || !K || !V) return fail(ctx, PA_CUDA_EINVAL, "null argument");
+    if (((uintptr_t) K | (uintptr_t) V) & 15) return fail(ctx, PA_CUDA_EINVAL, "K and V must be 16-byte aligned");
+    const uint64_t warps = 2ull * n_sets * n_tok * shape->nkv;
+    if ((warps + 7) / 8 > 0x7FFFFFFFull) return fail(ctx, PA_CUDA_EUNSUPPORTED, "too many rows in one call");
+    DeviceScope dev(ctx->device);
+    if (!dev.ok) return fail(ctx, PA_CUDA_ECUDA, "cudaSetDevice");
+    pa::pg::RowsParams a{};
+    a.v.table = table;
+    a.v.n_sets = n_sets;
+    a.v.max_pages = max_pages;
+    a.v.n_pages = cache->n_pages;
+    a.v.page_keys = cache->page_keys;
+    a.v.n_tok = n_tok;
+    a.v.status = ctx->d_status;
+    a.first = first;
+    a.K = cache->k + layer * layer_bytes(*shape, *cache);
+    a.V = cache->v + layer * layer_bytes(*shape, *cache);
+    a.Ko = K;
+    a.Vo = V;
+    a.rs = shape->rs;
+    a.hb = shape->hb;
+    a.nkv = shape->nkv;
+    const unsigned blocks = (unsigned) ((warps + 7) / 8);
+    if (shape->hd == 128) launch_rows<128>(a, shape->quant, blocks, pick(ctx, stream));
+    else launch_rows<256>(a, shape->quant, blocks, pick(ctx, stream));
+    PA_CK(cudaGetLastError(), "cache rows launch");
+    ctx->launches++;
+    return PA_CUDA_OK;
+}
+
+int pa_cuda_cache_copy_pages(pa_cuda_ctx *ctx, const pa_cuda_shape *shape, const pa_cuda_cache *cache, const int32_t *src,
+                             const int32_t *dst, uint32_t n, void *stream) {
+    if (!ctx) return PA_CUDA_EINVAL;
+    int rc = check_cache(ctx, shape, cache);
+    if (rc) return rc;
+    if (n == 0) return PA_CUDA_OK;
+    if (!src || !dst) return fail(ctx, PA_CUDA_EINVAL, "null argument");
+    DeviceScope dev(ctx->device);
+    if (!dev.ok) return fail(ctx, PA_CUDA_ECUDA, "cudaSetDevice");
+    pa::pg::CopyParams a{};
+    a.K = cache->k;
+    a.V = cache->v;
+    a.page_bytes = cache->page_keys * shape->rs;
+    a.n_pages = cache->n_pages;
+    a.n_layers = cache->n_layers;
+    a.status = ctx->d_status;
+    const uint64_t per = 256ull * 16 * pa::pg::COPY_UNROLL, x = (a.page_bytes + per - 1) / per;
+    if (x > 0x7FFFFFFFull) return fail(ctx, PA_CUDA_EUNSUPPORTED, "pages too large");
+    for (uint32_t i = 0; i < n; i += 65535) {
+        a.src = src + i;
+        a.dst = dst + i;
+        const dim3 grid((unsigned) x, std::min<uint32_t>(65535, n - i), 2 * cache->n_layers);
+        pa::pg::copy_pages_kernel<<<grid, 256, 0, pick(ctx, stream)>>>(a);
+        PA_CK(cudaGetLastError(), "copy pages launch");
+        ctx->launches++;
+    }
+    return PA_CUDA_OK;
+}
+
+int pa_cuda_cache_compact(pa_cuda_ctx *ctx, const pa_cuda_shape *shape, const pa_cuda_cache *cache, uint32_t n_sets,
+                          uint32_t n_tok, const int32_t *table, uint32_t max_pages, const int32_t *start, const int32_t *path,
+                          const int32_t *count, int32_t *n_keys_out, void *stream) {
+    if (!ctx) return PA_CUDA_EINVAL;
+    int rc = check_cache(ctx, shape, cache);
+    if (rc || (rc = check_table(ctx, cache, n_sets, max_pages))) return rc;
+    if (n_sets == 0) return PA_CUDA_OK;
+    if (n_tok == 0 || n_tok > pa::pg::COMPACT_MAX) return fail(ctx, PA_CUDA_EUNSUPPORTED, "a path has 1 to 1,024 tokens");
+    if (!table || !start || !path || !count) return fail(ctx, PA_CUDA_EINVAL, "null argument");
+    DeviceScope dev(ctx->device);
+    if (!dev.ok) return fail(ctx, PA_CUDA_ECUDA, "cudaSetDevice");
+    pa::pg::CompactParams a{};
+    a.v.table = table;
+    a.v.n_sets = n_sets;
+    a.v.max_pages = max_pages;
+    a.v.n_pages = cache->n_pages;
+    a.v.page_keys = cache->page_keys;
+    a.v.n_tok = n_tok;
+    a.v.status = ctx->d_status;
+    a.K = cache->k;
+    a.V = cache->v;
+    a.start = start;
+    a.path = path;
+    a.count = count;
+    a.n_keys_out = n_keys_out;
+    a.rs = shape->rs;
+    a.n_layers = cache->n_layers;
+    const uint64_t threads = shape->rs / 16 * 2 * cache->n_layers;
+    const dim3 grid((unsigned) ((threads + 127) / 128), n_sets);
+    pa::pg::compact_kernel<<<grid, 128, 0, pick(ctx, stream)>>>(a);
+    PA_CK(cudaGetLastError(), "compact launch");
+    ctx->launches++;
+    return PA_CUDA_OK;
+}
+
+}  // extern "C"

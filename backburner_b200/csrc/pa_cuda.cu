@@ -20,6 +20,7 @@
 #include <unordered_map>
 #include <vector>
 
+#include "pa_cache.cuh"
 #include "pa_decode.cuh"
 #include "pa_merge.cuh"
 #include "pa_prefill.cuh"
@@ -793,6 +794,8 @@ int pa_cuda_status(pa_cuda_ctx *ctx, void *stream) {
     if (h != pa::ST_OK) {
         PA_CK(cudaMemsetAsync(ctx->d_status, 0, sizeof h, st), "status clear");
         PA_CK(cudaStreamSynchronize(st), "stream synchronize");
+        if (h == pa::ST_BAD_ARGS)
+            return fail(ctx, PA_CUDA_EINVAL, "a cache call met a page id, length or path out of range on the device");
         return fail(ctx, PA_CUDA_ETIMEOUT, "a kernel gave up a bounded wait (code " + std::to_string(h) + ")");
     }
     return PA_CUDA_OK;
@@ -1831,3 +1834,6 @@ extern "C" int pa_cuda_attn_noalloc(const pa_cuda_shape *shape, const uint16_t *
     if (h != pa::ST_OK) return na_fail(why, PA_CUDA_ETIMEOUT, "a kernel gave up a bounded wait");
     return PA_CUDA_OK;
 }
+
+// ====================================================================================================== paged cache
+#include "pa_cache_host.h"

@@ -88,7 +88,8 @@ int pa_cuda_create(int device, pa_cuda_ctx **out);
 void pa_cuda_destroy(pa_cuda_ctx *ctx);
 const char *pa_cuda_last_error(const pa_cuda_ctx *ctx);
 /* Synchronise `stream` (a cudaStream_t; NULL = the context's stream), then return and clear the device status word:
- * PA_CUDA_OK, or PA_CUDA_ETIMEOUT if a kernel gave up a bounded wait since the last call. */
+ * PA_CUDA_OK, PA_CUDA_ETIMEOUT if a kernel gave up a bounded wait since the last call, or PA_CUDA_EINVAL if a paged-cache
+ * kernel met an argument out of range. */
 int pa_cuda_status(pa_cuda_ctx *ctx, void *stream);
 /* Bound on every in-kernel wait (default 2 s). */
 void pa_cuda_set_timeout_ns(pa_cuda_ctx *ctx, uint64_t ns);
@@ -246,6 +247,96 @@ int pa_cuda_arm(pa_cuda_ctx *ctx, const pa_cuda_page *pages, const uint32_t *nke
                 int ntok);
 /* number of begin calls served by an armed graph */
 uint64_t pa_cuda_graph_calls(const pa_cuda_ctx *ctx);
+
+/* ---- paged cache (no counterpart in the reference's engines, whose pages are host-managed: an addition of this library)
+ * A device cache whose sequences grow and branch: rows in pages, a page table per sequence, and everything that changes
+ * from step to step (tables, lengths, positions, masks) read on the device, so that one captured call serves a whole
+ * generation. The rows have the layout above. A step appends the new tokens' rows (pa_cuda_cache_append), attends
+ * (pa_cuda_cache_attn), and after a verify keeps the accepted rows (pa_cuda_cache_compact); pa_cuda_cache_copy_pages forks.
+ *
+ * Row of layer i, page p, position j: k + (((uint64_t) i * n_pages + p) * page_keys + j) * rs, v alike (rs, hb of the
+ * shape; device pointers, 16-byte aligned). page_keys: a multiple of 64. At most 2^31 - 1 rows in all layers.
+ * Sequences ("sets") number their keys 0, 1, ...: key j of set s lies in page table[s][j / page_keys] (int32, device,
+ * [n_sets][max_pages]; entries no key needs are not read and may hold anything). Rows past a sequence's keys, and rows no
+ * token of the call sees, may hold anything, NaN included; a row that some tokens of a call see has to be finite.
+ * Arguments that only the device can check (a page id outside the pool, a length past the table's reach, a bad path) do
+ * no harm: the rest of the call runs, what they touch is undefined, and pa_cuda_status reports PA_CUDA_EINVAL. */
+typedef struct pa_cuda_cache {
+    uint8_t *k, *v;
+    uint32_t n_layers, n_pages, page_keys;
+} pa_cuda_cache;
+
+/* Which keys a query token sees. n_tok tokens per set; token t's own key has index q0 + t, q0 = q_pos[s] (any value: a
+ * cache that holds an older position range than the queries' has q0 >= n_keys[s]) or, without q_pos, n_keys[s] - n_tok.
+ *   tree = 0: token t sees the keys j <= q0 + t that are held; with window > 0 only those with j > q0 + t - window or
+ *     j < sinks (window 0: all, and sinks must be 0).
+ *   tree = 1: the tokens are drafted and n_tok <= 64; token t sees the keys before q0 (with window > 0 those with
+ *     j > q0 + depth - window or j < sinks, depth = the bits set in its mask less one; window >= n_tok) and the drafted
+ *     keys q0 + u for which bit u of tree[s][t] is set (its ancestors and itself). A mask of 0 marks padding: it sees nothing.
+ * A token that sees nothing has m = -inf, l = 0 (lse = -inf) and O = 0. */
+typedef struct pa_cuda_mask {
+    uint32_t n_tok, window, sinks, tree;
+} pa_cuda_mask;
+
+typedef struct pa_cuda_cache_plan pa_cuda_cache_plan;
+/* A plan fixes the geometry (shape->rows = GQA group x n_tok rows per KV head, row g * n_tok + t) and owns the workspace
+ * of its calls: calls of one plan must not overlap (two streams, two captured graphs replayed at once: two plans).
+ * Reads pa_cuda_set_kernel (0, 1 or 2) as pa_cuda_plan_create does; the int8-domain QK is refused. */
+int pa_cuda_cache_plan_create(pa_cuda_ctx *ctx, const pa_cuda_shape *shape, const pa_cuda_cache *cache, uint32_t n_sets,
+                              uint32_t max_pages, const pa_cuda_mask *mask, pa_cuda_cache_plan **out);
+/* name of the plan's attention kernel (static storage) */
+const char *pa_cuda_cache_plan_kernel(const pa_cuda_cache_plan *plan);
+void pa_cuda_cache_plan_destroy(pa_cuda_cache_plan *plan);
+/* Attention of every set over one layer. Qs: f16(q * scale) [n_sets][nkv][rows][hd]; table, n_keys [n_sets], q_pos [n_sets]
+ * or NULL, tree [n_sets][n_tok] (tree plans) or NULL: device. Gives the unnormalised partial O [n_sets][nkv][rows][hd],
+ * m, l [n_sets][nkv][rows], which pa_cuda_merge folds with other partials of the same queries; the _reply form gives
+ * f16(O / l) and lse = m + log l, as pa_cuda_normalize. Asynchronous, capturable. */
+int pa_cuda_cache_attn(pa_cuda_cache_plan *plan, uint32_t layer, const uint16_t *Qs, const int32_t *table, const int32_t *n_keys,
+                       const int32_t *q_pos, const uint64_t *tree, float *O, float *m, float *l, void *stream);
+int pa_cuda_cache_attn_reply(pa_cuda_cache_plan *plan, uint32_t layer, const uint16_t *Qs, const int32_t *table,
+                             const int32_t *n_keys, const int32_t *q_pos, const uint64_t *tree, uint16_t *Oh, float *lse,
+                             void *stream);
+
+/* types of pa_cuda_cache_append's inputs */
+enum { PA_CUDA_T_F16 = 0, PA_CUDA_T_BF16 = 1, PA_CUDA_T_F32 = 2 };
+/* New tokens: q [n_sets][n_tok][nkv * gqa][hd] (head h * gqa + g is query head g of KV head h), k, v [n_sets][n_tok][nkv][hd],
+ * each with strides of its own over sets and tokens (elements; heads hd apart, as in a slice of one projection's output).
+ * wq, wk: [hd] norm weights or NULL (no norm); freqs: rot / 2 angles per position (radians, double, device); pos:
+ * [n_sets][n_tok] rotary positions or NULL (start[s] + t); a token with pos < 0 is padding. */
+typedef struct pa_cuda_append {
+    const void *q, *k, *v;
+    int64_t q_set, q_tok, k_set, k_tok, v_set, v_tok;
+    const void *wq, *wk;
+    const double *freqs;
+    const int32_t *pos;
+    uint32_t dtype, w_dtype;   /* PA_CUDA_T_*; weights: the inputs' type or f32 */
+    uint32_t rot;              /* leading dims that turn (0: none) */
+    uint32_t interleaved;      /* pairs (2i, 2i + 1), else (i, i + rot / 2) */
+    float eps, scale;
+} pa_cuda_append;
+/* For every token: y = x * rsqrt(mean(x^2) + eps) * w for its query and key heads, the first rot dims of y turned by
+ * pos * freqs; Qs [n_sets][nkv][gqa * n_tok][hd] = f16(y * scale) (rows g * n_tok + t, what the attention calls take), the
+ * key heads and the value heads as they are stored as the cache row of key start[s] + t, quantised as the format says
+ * (d = f16(max|x| / 127 or 7), q = rint(x / d)). fp32 arithmetic, angles in fp64. Padding: Qs = 0, nothing stored.
+ * shape->rows = gqa * n_tok. Bytes of a row past nkv * hb are left as they are. */
+int pa_cuda_cache_append(pa_cuda_ctx *ctx, const pa_cuda_shape *shape, const pa_cuda_cache *cache, uint32_t layer,
+                         const pa_cuda_append *in, uint32_t n_sets, uint32_t n_tok, const int32_t *table, uint32_t max_pages,
+                         const int32_t *start, uint16_t *Qs, void *stream);
+/* Keys first[s] + t, t < n_tok, as the f16 values the rows stand for: K, V [n_sets][n_tok][nkv][hd] */
+int pa_cuda_cache_rows(pa_cuda_ctx *ctx, const pa_cuda_shape *shape, const pa_cuda_cache *cache, uint32_t layer, uint32_t n_sets,
+                       uint32_t n_tok, const int32_t *table, uint32_t max_pages, const int32_t *first, uint16_t *K, uint16_t *V,
+                       void *stream);
+/* Pages src[i] -> dst[i], i < n (int32, device), of every layer, K and V. A page written by the call is not read by it and
+ * is written once (src[i] == dst[i] does nothing). */
+int pa_cuda_cache_copy_pages(pa_cuda_ctx *ctx, const pa_cuda_shape *shape, const pa_cuda_cache *cache, const int32_t *src,
+                             const int32_t *dst, uint32_t n, void *stream);
+/* After a verify: the rows of keys start[s] + path[s][i], i < count[s], move to start[s] + i in place, in every layer, K and
+ * V; path [n_sets][n_tok] rises strictly (an accepted path of a tree whose tokens follow their parents). n_keys_out[s] =
+ * start[s] + count[s] (may be NULL). n_tok <= 1,024, start[s] + n_tok within the table's reach; a set with a bad path, count
+ * or page keeps its rows, and n_keys_out[s] = start[s]. Rows behind the kept ones stay as they are. */
+int pa_cuda_cache_compact(pa_cuda_ctx *ctx, const pa_cuda_shape *shape, const pa_cuda_cache *cache, uint32_t n_sets,
+                          uint32_t n_tok, const int32_t *table, uint32_t max_pages, const int32_t *start, const int32_t *path,
+                          const int32_t *count, int32_t *n_keys_out, void *stream);
 
 /* ---- allocation-free call (no counterpart in the reference: an addition of this library)
  * For callers that cannot allocate device memory: a host runtime that owns every device allocation itself (a fixed
