@@ -9,103 +9,10 @@
 #pragma once
 #include "pa_common.cuh"
 #include "pa_decode.cuh"
+#include "pa_mask.cuh"
 
 namespace pa {
 namespace pg {
-
-// ---------------------------------------------------------------- which keys a token sees
-// Token t of set s has its own key at q0 + t (q0 = q_pos[s], or n_keys[s] - n_tok). Without a tree it sees keys j <= q0 + t,
-// with a window w only j > q0 + t - w or j < sinks. With a tree it sees the keys before q0 (the window measured from
-// q0 + depth, depth = its ancestors) and the drafted keys q0 + u whose bit u is set in its mask; a token with no bit set
-// is padding and sees nothing.
-struct View {
-    const int32_t *table, *n_keys, *q_pos;   // [n_sets][max_pages], [n_sets], [n_sets] or null
-    const uint64_t *tree;                    // [n_sets][n_tok] or null
-    uint32_t n_sets, max_pages, n_pages, page_keys, n_tok, window, sinks;
-    int *status;
-};
-struct Set {
-    int nk, q0;   // keys held, clamped to the table's reach; key of token 0 (may be negative or past nk)
-};
-// the keys a row sees: [lo, hi), [0, sink) and q0 + u for each bit u
-struct Row {
-    int lo, hi, sink, q0;
-    uint64_t bits;
-};
-
-#define PA_HD __host__ __device__ __forceinline__
-PA_HD int capacity(const View &v) { return (int) (v.max_pages * v.page_keys); }   // <= 2^30
-PA_HD int clampi(int64_t x, int lo, int hi) { return x < lo ? lo : x > hi ? hi : (int) x; }
-// the low n bits
-PA_HD uint64_t low_bits(int64_t n) { return n <= 0 ? 0ull : n >= 64 ? ~0ull : (1ull << n) - 1; }
-
-__device__ __forceinline__ Set set_of(const View &v, uint32_t s) {
-    const int n = v.n_keys[s];
-    if (n < 0 || n > capacity(v)) atomicCAS(v.status, ST_OK, ST_BAD_ARGS);
-    return Set{clampi(n, 0, capacity(v)), v.q_pos ? v.q_pos[s] : clampi((int64_t) n - (int) v.n_tok, INT32_MIN, INT32_MAX)};
-}
-PA_HD int bit_count(uint64_t b) {
-#ifdef __CUDA_ARCH__
-    return __popcll(b);
-#else
-    return __builtin_popcountll(b);
-#endif
-}
-// the first `sinks` keys, of at most hi
-PA_HD int sink_end(const View &v, int hi) { return !v.window ? 0 : v.sinks < (uint32_t) hi ? (int) v.sinks : hi; }
-PA_HD Row row_from(const View &v, Set st, int64_t at, int hi, uint64_t bits) {
-    Row r;
-    r.hi = hi;
-    r.lo = v.window ? clampi(at - (int64_t) v.window + 1, 0, hi) : 0;
-    r.sink = sink_end(v, hi);
-    r.q0 = st.q0;
-    r.bits = bits & low_bits((int64_t) st.nk - st.q0) & ~low_bits(-(int64_t) st.q0);   // drafted keys that exist
-    return r;
-}
-PA_HD Row row_of(const View &v, Set st, uint32_t s, uint32_t t) {
-    if (!v.tree) return row_from(v, st, (int64_t) st.q0 + t, clampi((int64_t) st.q0 + t + 1, 0, st.nk), 0);
-    const uint64_t b = v.tree[(uint64_t) s * v.n_tok + t] & low_bits(v.n_tok);
-    if (!b) return Row{0, 0, 0, st.q0, 0};
-    return row_from(v, st, (int64_t) st.q0 + bit_count(b) - 1, clampi(st.q0, 0, st.nk), b);
-}
-// bit i: the row sees key k0 + i
-PA_HD uint64_t vis64(const Row &r, int k0) {
-    uint64_t m = (low_bits((int64_t) r.hi - k0) & ~low_bits((int64_t) r.lo - k0)) | low_bits((int64_t) r.sink - k0);
-    const int64_t d = (int64_t) r.q0 - k0;
-    if (d >= 0) m |= d < 64 ? r.bits << d : 0;
-    else m |= d > -64 ? r.bits >> -d : 0;
-    return m;
-}
-
-// The groups of G keys that tokens [t0, t1] of a set see together: the sinks' groups 0 .. a-1, then groups b, b+1, ...
-struct Span {
-    int a, b, n;   // n groups in all
-    PA_HD int group(int i) const { return i < a ? i : b + (i - a); }
-};
-template <int G>
-PA_HD Span span_of(const View &v, Set st, uint32_t t0, uint32_t t1) {
-    // a tree's tokens: depth 0 starts the window earliest, the drafted keys end at q0 + n_tok
-    const int hi = clampi((int64_t) st.q0 + (v.tree ? (int64_t) v.n_tok : (int64_t) t1 + 1), 0, st.nk);
-    const int lo = v.window ? clampi((int64_t) st.q0 + (v.tree ? 0 : t0) - (int64_t) v.window + 1, 0, hi) : 0;
-    const int end = lo < hi ? (hi + G - 1) / G : 0;
-    Span p;
-    p.a = (sink_end(v, hi) + G - 1) / G;
-    p.b = lo / G > p.a ? lo / G : p.a;
-    p.n = p.a + (end > p.b ? end - p.b : 0);
-    return p;
-}
-
-// the page of the 64-key group that holds key `key` (a page id outside the pool is reported and replaced by page 0)
-__device__ __forceinline__ uint32_t page_of(const View &v, uint32_t s, uint32_t key) {
-    const int32_t p = __ldg(v.table + (uint64_t) s * v.max_pages + key / v.page_keys);
-    if ((uint32_t) p < v.n_pages) return (uint32_t) p;
-    atomicCAS(v.status, ST_OK, ST_BAD_ARGS);
-    return 0;
-}
-// row of the pool (within a layer) that holds key `key`
-__device__ __forceinline__ uint32_t row_at(const View &v, uint32_t s, uint32_t key) {
-    return page_of(v, s, key) * v.page_keys + key % v.page_keys;
-}
 
 // ---------------------------------------------------------------- elements of a head
 // value i of a head row: f16(d * q), or the f16 itself
@@ -118,66 +25,6 @@ __device__ __forceinline__ float head_value(const uint8_t *head, int i) {
     if (QUANT == 1) q = (int8_t) blk[2 + i % 32];
     else q = (int) ((blk[2 + i % 16] >> (i % 32 < 16 ? 0 : 4)) & 15) - 8;
     return __half2float(__hmul(d, __int2half_rn(q)));
-}
-
-// ---------------------------------------------------------------- attention, one warp per query row
-// The plain kernel: a lane holds hd / 32 dims; every key the row sees in turn, with the running maximum and sum.
-struct AttnParams {
-    View v;
-    const uint8_t *k, *v_rows;   // the layer's rows
-    const uint16_t *Qs;
-    uint64_t rs, hb;
-    uint32_t nkv, rows;
-    float *O, *M, *L;            // unnormalised partial, or (Oh, lse)
-    uint16_t *Oh;
-    float *lse;
-};
-template <int HD, int QUANT>
-__global__ void __launch_bounds__(32) row_attn_kernel(const AttnParams p) {
-    constexpr int E = HD / 32;
-    const uint32_t r = blockIdx.x, h = blockIdx.y, s = blockIdx.z, lane = threadIdx.x;
-    const Set st = set_of(p.v, s);
-    const uint32_t t = r % p.v.n_tok;
-    const Row row = row_of(p.v, st, s, t);
-    const Span sp = span_of<64>(p.v, st, t, t);
-    const uint64_t ro = ((uint64_t) s * p.nkv + h) * p.rows + r;
-    float q[E], o[E], m = -INFINITY, l = 0.f;
-#pragma unroll
-    for (int e = 0; e < E; e++) {
-        q[e] = h2f_bits(p.Qs[ro * HD + 32 * e + lane]);
-        o[e] = 0.f;
-    }
-    for (int i = 0; i < sp.n; i++) {
-        const int k0 = sp.group(i) * 64;
-        uint64_t see = vis64(row, k0);
-        if (!see) continue;
-        const uint64_t base = (uint64_t) row_at(p.v, s, (uint32_t) k0) * p.rs + h * p.hb;
-        while (see) {
-            const int b = __ffsll((long long) see) - 1;
-            see &= see - 1;
-            const uint8_t *kr = p.k + base + (uint64_t) b * p.rs, *vr = p.v_rows + base + (uint64_t) b * p.rs;
-            float x = 0.f;
-#pragma unroll
-            for (int e = 0; e < E; e++) x = fmaf(q[e], head_value<QUANT>(kr, 32 * e + lane), x);
-#pragma unroll
-            for (int w = 16; w > 0; w >>= 1) x += __shfl_xor_sync(0xffffffffu, x, w);
-            const float m2 = fmaxf(m, x), al = ex2((m - m2) * LOG2E), pr = ex2((x - m2) * LOG2E);
-            l = fmaf(l, al, pr);
-#pragma unroll
-            for (int e = 0; e < E; e++) o[e] = fmaf(o[e], al, pr * head_value<QUANT>(vr, 32 * e + lane));
-            m = m2;
-        }
-    }
-    if (p.Oh) {
-        const float inv = l > 0.f ? 1.f / l : 0.f;
-#pragma unroll
-        for (int e = 0; e < E; e++) p.Oh[ro * HD + 32 * e + lane] = __half_as_ushort(__float2half_rn(o[e] * inv));
-        if (lane == 0) p.lse[ro] = l > 0.f ? m + logf(l) : -INFINITY;
-    } else {
-#pragma unroll
-        for (int e = 0; e < E; e++) p.O[ro * HD + 32 * e + lane] = o[e];
-        if (lane == 0) { p.M[ro] = l > 0.f ? m : -INFINITY; p.L[ro] = l; }
-    }
 }
 
 // ---------------------------------------------------------------- append: head norm, rotation, scale, quantised store

@@ -50,35 +50,69 @@ struct pa_cuda_cache_plan {
     pa_cuda_cache cache{};
     pa_cuda_mask mask{};
     uint32_t n_sets = 0, max_pages = 0;
+    pa_cuda_plan d;                  // launch shape of the split-K kernel
+    bool tc = false;                 // the tcgen05 kernel
+    int nt = 1;                      // ... with nt tiles of 128 rows per CTA, n_rt groups of them per head
+    uint32_t n_rt = 1;
+    uint32_t n_parts = 1;            // CTAs along the keys = slots of partials (pa_mask.cuh)
+    CUtensorMap *d_maps = nullptr;   // K and V rows of the whole cache
+    float *d_part = nullptr;         // O [slot][nkv][rows][hd], then m, then l
+    uint32_t *d_crange = nullptr;    // [n_sets + 1]: slots of each set, written by every call
     const char *kernel = "";
 };
 
 namespace {
 
-pa::pg::View view_of(const pa_cuda_cache_plan *p, const int32_t *table, const int32_t *n_keys, const int32_t *q_pos,
-                     const uint64_t *tree) {
-    pa::pg::View v{};
-    v.table = table;
-    v.n_keys = n_keys;
-    v.q_pos = q_pos;
-    v.tree = p->mask.tree ? tree : nullptr;
-    v.n_sets = p->n_sets;
-    v.max_pages = p->max_pages;
-    v.n_pages = p->cache.n_pages;
-    v.page_keys = p->cache.page_keys;
-    v.n_tok = p->mask.n_tok;
-    v.window = p->mask.window;
-    v.sinks = p->mask.sinks;
-    v.status = p->ctx->d_status;
-    return v;
+// Least groups of keys a part takes (16-key groups in the split-K kernel, 64-key groups in the tcgen05 kernel).
+constexpr uint32_t kMinGroups16 = 4, kMinGroups64 = 2;
+constexpr uint32_t kGroups64Overhead = 8;   // what a CTA of the tcgen05 kernel costs besides its groups, in groups
+
+template <int HD, int Q, int W>
+cudaError_t launch_decode_paged(const pa_cuda_cache_plan *p, const pa::dec::PagedParams &prm, cudaStream_t st) {
+    pa::dec::decode_kernel<HD, Q, W, true><<<dim3(p->n_parts, p->d.grid_y), 32 * p->d.n_consumers, p->d.smem, st>>>(prm);
+    return cudaGetLastError();
+}
+template <int Q, int NT, int D>
+cudaError_t launch_prefill_paged(const pa_cuda_cache_plan *p, const CUtensorMap &tq, const pa::pre::PagedParams &prm, cudaStream_t st) {
+    constexpr int smem = pa::pre::Smem<Q, NT, D>::TOTAL + 1024;
+    pa::pre::prefill_kernel<Q, NT, D, true>
+        <<<p->n_parts * p->sh.nkv * p->n_rt, 32 * pa::pre::cta_warps(NT), smem, st>>>(tq, prm);
+    return cudaGetLastError();
+}
+// f(kernel instance's constants) for the plan's kernel; f is a generic lambda
+template <int HD, int W, class F>
+auto with_quant(uint32_t quant, F &&f) {
+    using std::integral_constant;
+    if (quant == PA_CUDA_Q8_0) return f(integral_constant<int, HD>{}, integral_constant<int, 1>{}, integral_constant<int, W>{});
+    if (quant == PA_CUDA_Q4_0) return f(integral_constant<int, HD>{}, integral_constant<int, 2>{}, integral_constant<int, W>{});
+    return f(integral_constant<int, HD>{}, integral_constant<int, 0>{}, integral_constant<int, W>{});
+}
+template <class F>
+auto with_decode(const pa_cuda_cache_plan *p, F &&f) {
+    if (p->sh.hd == 128) return with_quant<128, 8>(p->sh.quant, f);
+    return p->d.w == 4 ? with_quant<256, 4>(p->sh.quant, f) : with_quant<256, 8>(p->sh.quant, f);
+}
+template <class F>
+auto with_prefill(const pa_cuda_cache_plan *p, F &&f) {
+    using std::integral_constant;
+    using I1 = integral_constant<int, 1>;
+    using I2 = integral_constant<int, 2>;
+    using D128 = integral_constant<int, 128>;
+    using D256 = integral_constant<int, 256>;
+    if (p->sh.hd == 256) return p->sh.quant == PA_CUDA_Q8_0 ? f(I1{}, I1{}, D256{}) : f(I2{}, I1{}, D256{});
+    if (p->nt == 2) return p->sh.quant == PA_CUDA_Q8_0 ? f(I1{}, I2{}, D128{}) : f(I2{}, I2{}, D128{});
+    return p->sh.quant == PA_CUDA_Q8_0 ? f(I1{}, I1{}, D128{}) : f(I2{}, I1{}, D128{});
 }
 
-template <int HD>
-void launch_row_attn(const pa_cuda_cache_plan *p, const pa::pg::AttnParams &a, cudaStream_t st) {
-    const dim3 grid(p->sh.rows, p->sh.nkv, p->n_sets);
-    if (p->sh.quant == PA_CUDA_Q8_0) pa::pg::row_attn_kernel<HD, 1><<<grid, 32, 0, st>>>(a);
-    else if (p->sh.quant == PA_CUDA_Q4_0) pa::pg::row_attn_kernel<HD, 2><<<grid, 32, 0, st>>>(a);
-    else pa::pg::row_attn_kernel<HD, 0><<<grid, 32, 0, st>>>(a);
+template <int HD, bool REPLY>
+cudaError_t launch_cache_merge(const pa_cuda_cache_plan *p, const pa::mrg::Params &mp, cudaStream_t st) {
+    const uint64_t rows = (uint64_t) mp.n_sets * mp.rows_per_set;
+    // 8 warps a row where the rows alone leave SMs idle and a set can have many parts (as launch_merge)
+    if (rows * 8 <= (uint64_t) p->ctx->n_sm * 128 && p->n_parts >= 8 * p->n_sets)
+        pa::mrg::merge_kernel<HD, 8, REPLY><<<(unsigned) rows, 256, 0, st>>>(mp);
+    else
+        pa::mrg::merge_kernel<HD, 1, REPLY><<<(unsigned) ((rows + 7) / 8), 256, 0, st>>>(mp);
+    return cudaGetLastError();
 }
 
 // O, m, l or Oh, lse: one of the two forms
@@ -93,24 +127,142 @@ int cache_attn(pa_cuda_cache_plan *p, uint32_t layer, const uint16_t *Qs, const 
     DeviceScope dev(ctx->device);
     if (!dev.ok) return fail(ctx, PA_CUDA_ECUDA, "cudaSetDevice");
     cudaStream_t st = pick(ctx, stream);
-    pa::pg::AttnParams a{};
-    a.v = view_of(p, table, n_keys, q_pos, tree);
-    a.k = p->cache.k + layer * layer_bytes(p->sh, p->cache);
-    a.v_rows = p->cache.v + layer * layer_bytes(p->sh, p->cache);
-    a.Qs = Qs;
-    a.rs = p->sh.rs;
-    a.hb = p->sh.hb;
-    a.nkv = p->sh.nkv;
-    a.rows = p->sh.rows;
-    a.O = O;
-    a.M = m;
-    a.L = l;
-    a.Oh = Oh;
-    a.lse = lse;
-    if (p->sh.hd == 128) launch_row_attn<128>(p, a, st);
-    else launch_row_attn<256>(p, a, st);
-    PA_CK(cudaGetLastError(), "cache attention launch");
-    ctx->launches++;
+    const pa_cuda_shape &sh = p->sh;
+    const uint64_t rows_all = (uint64_t) sh.nkv * sh.rows;
+    float *Op = p->d_part, *Mp = Op + p->n_parts * rows_all * sh.hd, *Lp = Mp + p->n_parts * rows_all;
+    pa::pg::Paged pg{};
+    pg.v.table = table;
+    pg.v.n_keys = n_keys;
+    pg.v.q_pos = q_pos;
+    pg.v.tree = tree;
+    pg.v.n_sets = p->n_sets;
+    pg.v.max_pages = p->max_pages;
+    pg.v.n_pages = p->cache.n_pages;
+    pg.v.page_keys = p->cache.page_keys;
+    pg.v.n_tok = p->mask.n_tok;
+    pg.v.window = p->mask.window;
+    pg.v.sinks = p->mask.sinks;
+    pg.v.status = ctx->d_status;
+    pg.k = p->cache.k + layer * layer_bytes(sh, p->cache);
+    pg.vr = p->cache.v + layer * layer_bytes(sh, p->cache);
+    pg.row0 = layer * p->cache.n_pages * p->cache.page_keys;
+    pg.n_parts = p->n_parts;
+    pg.min_groups = p->tc ? kMinGroups64 : kMinGroups16;
+    pg.crange = p->d_crange;
+    cudaError_t e;
+    if (p->tc) {
+        CUtensorMap tq;
+        if (!map_q(&tq, Qs, p->n_sets * rows_all, sh.hd)) return fail(ctx, PA_CUDA_ECUDA, "cuTensorMapEncodeTiled (Q) failed");
+        pa::pre::PagedParams prm{};
+        prm.pg = pg;
+        prm.Qs = Qs;
+        prm.kv_maps = p->d_maps;
+        prm.Op = Op;
+        prm.Mp = Mp;
+        prm.Lp = Lp;
+        prm.status = ctx->d_status;
+        prm.rs = sh.rs;
+        prm.hb = sh.hb;
+        prm.nkv = sh.nkv;
+        prm.rows = sh.rows;
+        prm.n_rt = p->n_rt;
+        prm.timeout_ns = ctx->timeout_ns;
+        prm.stall = ctx->stall_test;
+        e = with_prefill(p, [&](auto q, auto nt, auto d) { return launch_prefill_paged<q.value, nt.value, d.value>(p, tq, prm, st); });
+    } else {
+        pa::dec::PagedParams prm{};
+        prm.pg = pg;
+        prm.Qs = Qs;
+        prm.Op = Op;
+        prm.Mp = Mp;
+        prm.Lp = Lp;
+        prm.status = ctx->d_status;
+        prm.rs = sh.rs;
+        prm.hb = sh.hb;
+        prm.nkv = sh.nkv;
+        prm.rows = sh.rows;
+        prm.hg = p->d.hg;
+        prm.rgc = p->d.rgc;
+        prm.n_rg = p->d.n_rg;
+        prm.row = p->d.row;
+        prm.gs = p->d.gs;
+        prm.n_jobs = p->n_parts;
+        prm.n_consumers = p->d.n_consumers;
+        prm.timeout_ns = ctx->timeout_ns;
+        prm.stall = ctx->stall_test;
+        e = with_decode(p, [&](auto hd, auto q, auto w) { return launch_decode_paged<hd.value, q.value, w.value>(p, prm, st); });
+    }
+    if (e != cudaSuccess) return cuda_fail(ctx, e, "cache attention launch");
+    pa::mrg::Params mp{};
+    mp.Op = Op;
+    mp.Mp = Mp;
+    mp.Lp = Lp;
+    mp.c_range = p->d_crange;
+    mp.n_parts = p->n_parts;
+    mp.op_stride = rows_all * sh.hd;
+    mp.ml_stride = rows_all;
+    mp.O = O;
+    mp.M = m;
+    mp.L = l;
+    mp.rows_per_set = rows_all;
+    mp.n_sets = p->n_sets;
+    mp.Oh = Oh;
+    mp.lse = lse;
+    if (sh.hd == 128) e = Oh ? launch_cache_merge<128, true>(p, mp, st) : launch_cache_merge<128, false>(p, mp, st);
+    else e = Oh ? launch_cache_merge<256, true>(p, mp, st) : launch_cache_merge<256, false>(p, mp, st);
+    if (e != cudaSuccess) return cuda_fail(ctx, e, "cache merge launch");
+    ctx->launches += 2;
+    return PA_CUDA_OK;
+}
+
+// the launch shape of a plan: kernel, row tiles, parts
+int shape_cache_plan(pa_cuda_cache_plan *p) {
+    pa_cuda_ctx *ctx = p->ctx;
+    const pa_cuda_shape &sh = p->sh;
+    p->d.ctx = ctx;
+    p->d.sh = sh;
+    int rc = plan_decode_shape(ctx, &p->d);
+    if (rc) return rc;
+    const bool tc_ok = sh.quant != PA_CUDA_F16 && encode_fn() != nullptr;
+    if (ctx->kernel_choice > 2 || (ctx->kernel_choice == 2 && !tc_ok))
+        return fail(ctx, PA_CUDA_EUNSUPPORTED, "the paged cache takes the split-K kernel or, over quantised rows, the single-CTA tcgen05 kernel");
+    p->tc = tc_ok && (ctx->kernel_choice == 2 || (ctx->kernel_choice == 0 && sh.rows >= (sh.hd == 128 ? kPrefillMinRows128 : kPrefillMinRows256)));
+    // groups of keys that one set can have to read
+    const uint32_t G = p->tc ? 64 : 16;
+    const uint64_t cap = (uint64_t) p->max_pages * p->cache.page_keys;
+    uint64_t groups = cap / G;
+    if (p->mask.window)
+        groups = std::min(groups, ((uint64_t) p->mask.window + p->mask.n_tok + G - 1) / G + 1 + std::min<uint64_t>((p->mask.sinks + (uint64_t) G - 1) / G, groups));
+    const uint64_t spare = p->n_sets > 1 ? p->n_sets : 0;   // find_part: parts lost to the sets' remainders
+    uint64_t parts;
+    if (p->tc) {
+        p->nt = sh.hd == 128 && sh.rows > (uint32_t) pa::pre::BM ? 2 : 1;
+        p->n_rt = (sh.rows + pa::pre::BM * p->nt - 1) / (pa::pre::BM * p->nt);
+        p->kernel = p->nt == 2 ? "pa::pre::prefill_kernel<2 tiles, paged>" : "pa::pre::prefill_kernel<1 tile, paged>";
+        // the count that minimises waves x (groups of a part + a CTA's overhead), the sets as long as they can be
+        const uint64_t y = (uint64_t) sh.nkv * p->n_rt;
+        uint64_t best = ~0ull;
+        parts = spare + 1;
+        for (uint64_t c = spare + 1; c <= spare + std::max<uint64_t>(1, 8ull * ctx->n_sm / y); c++) {
+            const uint64_t per = (groups * p->n_sets + (c - spare) - 1) / (c - spare);
+            const uint64_t cost = ((c * y + ctx->n_sm - 1) / ctx->n_sm) * (per + kGroups64Overhead);
+            if (cost < best) { best = cost; parts = c; }
+        }
+        if (parts * y > 0x7FFFFFFFull) return fail(ctx, PA_CUDA_EUNSUPPORTED, "too many rows and sets in one call");
+    } else {
+        if (p->d.grid_y > 65535) return fail(ctx, PA_CUDA_EUNSUPPORTED, "too many head/row groups");
+        p->kernel = "pa::dec::decode_kernel<paged>";
+        int per_sm = 1;
+        with_decode(p, [&](auto hd, auto q, auto w) {
+            auto *k = pa::dec::decode_kernel<hd.value, q.value, w.value, true>;
+            cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, (int) p->d.smem);
+            return cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, k, 32 * (int) p->d.n_consumers, p->d.smem);
+        });
+        // as many CTAs as run at once
+        parts = std::max<uint64_t>(spare + 1, (uint64_t) ctx->n_sm * std::max(1, per_sm) / p->d.grid_y);
+    }
+    parts = std::min(parts, spare + p->n_sets * std::max<uint64_t>(1, groups));
+    p->n_parts = (uint32_t) std::max<uint64_t>(parts, 2 * spare);
     return PA_CUDA_OK;
 }
 
@@ -160,12 +312,49 @@ int pa_cuda_cache_plan_create(pa_cuda_ctx *ctx, const pa_cuda_shape *shape, cons
     p->mask = *mask;
     p->n_sets = n_sets;
     p->max_pages = max_pages;
-    p->kernel = "pa::pg::row_attn_kernel";
+    DeviceScope dev(ctx->device);
+    if (!dev.ok) rc = fail(ctx, PA_CUDA_ECUDA, "cudaSetDevice");
+    if (rc || (rc = shape_cache_plan(p))) {
+        delete p;
+        return rc;
+    }
+    const uint64_t rows_all = (uint64_t) shape->nkv * shape->rows;
+    cudaError_t e = cudaMalloc((void **) &p->d_part, p->n_parts * rows_all * (shape->hd + 2) * sizeof(float));
+    if (e == cudaSuccess) e = cudaMalloc((void **) &p->d_crange, (n_sets + 1) * sizeof(uint32_t));
+    if (e == cudaSuccess && p->tc) {
+        const uint32_t rows = cache->n_layers * cache->n_pages * cache->page_keys;
+        const uint32_t raw = (uint32_t) pa::pre::raw_row_bytes((int) shape->quant, (int) shape->hd);
+        CUtensorMap maps[2];
+        if (!map_rows(&maps[0], cache->k, shape->rs, rows, raw, pa::pre::BN) || !map_rows(&maps[1], cache->v, shape->rs, rows, raw, pa::pre::BN)) {
+            pa_cuda_cache_plan_destroy(p);
+            return fail(ctx, PA_CUDA_ECUDA, "cuTensorMapEncodeTiled (K/V rows) failed");
+        }
+        if ((e = cudaMalloc((void **) &p->d_maps, sizeof maps)) == cudaSuccess)
+            e = cudaMemcpy(p->d_maps, maps, sizeof maps, cudaMemcpyHostToDevice);
+        if (e == cudaSuccess)
+            e = with_prefill(p, [&](auto q, auto nt, auto d) {
+                constexpr int smem = pa::pre::Smem<q.value, nt.value, d.value>::TOTAL + 1024;
+                return cudaFuncSetAttribute(pa::pre::prefill_kernel<q.value, nt.value, d.value, true>,
+                                            cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+            });
+    }
+    if (e != cudaSuccess) {
+        pa_cuda_cache_plan_destroy(p);
+        cudaGetLastError();
+        return fail(ctx, e == cudaErrorMemoryAllocation ? PA_CUDA_ENOMEM : PA_CUDA_ECUDA, std::string("cache plan: ") + cudaGetErrorString(e));
+    }
     *out = p;
     return PA_CUDA_OK;
 }
 const char *pa_cuda_cache_plan_kernel(const pa_cuda_cache_plan *plan) { return plan ? plan->kernel : ""; }
-void pa_cuda_cache_plan_destroy(pa_cuda_cache_plan *plan) { delete plan; }
+void pa_cuda_cache_plan_destroy(pa_cuda_cache_plan *plan) {
+    if (!plan) return;
+    DeviceScope dev(plan->ctx->device);
+    if (plan->d_part) cudaFree(plan->d_part);
+    if (plan->d_crange) cudaFree(plan->d_crange);
+    if (plan->d_maps) cudaFree(plan->d_maps);
+    delete plan;
+}
 
 int pa_cuda_cache_attn(pa_cuda_cache_plan *plan, uint32_t layer, const uint16_t *Qs, const int32_t *table, const int32_t *n_keys,
                        const int32_t *q_pos, const uint64_t *tree, float *O, float *m, float *l, void *stream) {

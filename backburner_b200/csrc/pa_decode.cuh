@@ -30,8 +30,13 @@
 //     quantised per 32-block by the Q8_0 rule (d = f16(max|x| / 127), q = rint(x / d)) when a job starts, one
 //     mma.m16n8k32 s8 per quant block gives the block's exact int32 dot products T for 16 keys x 8 rows, and
 //     s = sum_b float(T_b) * (dq_b * dk_b) in block order (fma). Softmax and P.V are those of QUANT 1.
+//   * PAGED: the keys come from a paged cache and the rows see them through a mask (pa_mask.cuh). A CTA finds its part of
+//     its set's visible 16-key groups on the device; pages hold whole stages, so a stage is copied whole. Only stages at the
+//     edge of what the rows see compute the mask (one 64-bit word per row, from its range and its tree bits); keys no row of
+//     the warp sees get a zero V scale, since their rows may hold NaN.
 #pragma once
 #include "pa_common.cuh"
+#include "pa_mask.cuh"
 
 namespace pa {
 namespace dec {
@@ -77,6 +82,12 @@ struct Params {
     uint64_t timeout_ns;
     int stall;            // test hook: consumers first wait on a barrier that nothing completes (bounded)
 };
+// the paged kernel's: jobs, n_jobs unused
+struct PagedParams : Params {
+    pg::Paged pg;
+};
+template <bool PAGED> struct ParamsOf { using type = Params; };
+template <> struct ParamsOf<true> { using type = PagedParams; };
 
 __host__ __device__ constexpr int q_group_bytes(int quant) { return quant == 1 ? 34 : quant == 2 ? 18 : 64; }
 
@@ -158,8 +169,8 @@ __device__ __forceinline__ void q4_word(uint32_t w, uint32_t s2, uint32_t &l02, 
 // stages of a CTA's jobs, in order, are one stream g = 0, 1, 2, ... through the ring: stage g lands in buffer
 // g % NSTAGE, so the copies of a next job's first stages are in flight while the previous job's last stages are
 // computed and its partial written.
-template <int HD, int QUANT, int W>
-__global__ void __launch_bounds__(32 * W, min_ctas(HD, W)) decode_kernel(const Params p) {
+template <int HD, int QUANT, int W, bool PAGED = false>
+__global__ void __launch_bounds__(32 * W, min_ctas(HD, W)) decode_kernel(const typename ParamsOf<PAGED>::type p) {
     constexpr int NMT = HD / 16;   // k-steps of QK^T = m-tiles of P.V
     constexpr int STAGE_KEYS = stage_keys(HD);
     constexpr int NSTAGE = nstage(HD);
@@ -199,16 +210,50 @@ __global__ void __launch_bounds__(32 * W, min_ctas(HD, W)) decode_kernel(const P
         *abort_flag = *(volatile int *) p.status != ST_OK;
         fence_mbar_init();
     }
+    __shared__ pg::Part s_part;   // PAGED: what this CTA works on, and what its tokens see together
+    __shared__ pg::Tile s_tile;
+    if constexpr (PAGED) {
+        if (warp == 0) {
+            const pg::Part f = pg::find_part<STAGE_KEYS>(p.pg, blockIdx.x, blockIdx.x == 0 && blockIdx.y == 0, lane);
+            const pg::Tile tl = pg::tile_of(p.pg.v, f.st, f.set, 0, p.pg.v.n_tok - 1, lane);
+            if (lane == 0) {
+                s_part = f;
+                s_tile = tl;
+            }
+        }
+    }
     __syncthreads();
     if (*abort_flag || warp >= n_active || blockIdx.x >= p.n_jobs) return;
+    // PAGED: groups [pg0, pg0 + pgn) of the set's span, a stage each
+    pg::Span span{};
+    uint32_t pg0 = 0, pgn = 0;
+    if constexpr (PAGED) {
+        if (s_part.of == 0) return;
+        span = pg::span_of<STAGE_KEYS>(p.pg.v, s_part.st, 0, p.pg.v.n_tok - 1);
+        const uint32_t per = ((uint32_t) span.n + s_part.of - 1) / s_part.of;
+        pg0 = min(s_part.index * per, (uint32_t) span.n);
+        pgn = min(per, (uint32_t) span.n - pg0);
+    }
 
-    auto stages_of = [&](uint32_t jn) -> uint32_t { return (p.jobs[jn].nk + STAGE_KEYS - 1) / STAGE_KEYS; };
+    auto stages_of = [&](uint32_t jn) -> uint32_t {
+        if constexpr (PAGED) return pgn;
+        else return (p.jobs[jn].nk + STAGE_KEYS - 1) / STAGE_KEYS;
+    };
     // stage `it` of job `jn` as stream stage g, into buffer g % NSTAGE: K rows then V rows, one bulk copy per pair of
     // key rows (warp-collective)
     auto issue = [&](uint32_t jn, uint32_t it, uint32_t g) {
-        const Job jb = p.jobs[jn];
         const uint32_t s = g % NSTAGE;
-        const uint32_t valid = min((uint32_t) STAGE_KEYS, jb.nk - it * STAGE_KEYS);
+        Job jb;
+        uint32_t valid;
+        if constexpr (PAGED) {
+            jb.k = p.pg.k;
+            jb.v = p.pg.vr;
+            jb.key0 = pg::row_at(p.pg.v, s_part.set, (uint32_t) span.group((int) (pg0 + it)) * STAGE_KEYS) - it * STAGE_KEYS;
+            valid = STAGE_KEYS;
+        } else {
+            jb = p.jobs[jn];
+            valid = min((uint32_t) STAGE_KEYS, jb.nk - it * STAGE_KEYS);
+        }
         if (lane == 0) {
             issued[s] = g;
             mbar_arrive_expect_tx(&full[s], 2u * valid * copy_bytes);
@@ -239,6 +284,7 @@ __global__ void __launch_bounds__(32 * W, min_ctas(HD, W)) decode_kernel(const P
         uint32_t target = g + NSTAGE - g0, jn = jc, n = nc;
         while (target >= n) {
             target -= n;
+            if constexpr (PAGED) return;
             jn += gridDim.x;
             if (jn >= p.n_jobs) return;
             n = stages_of(jn);
@@ -263,9 +309,10 @@ __global__ void __launch_bounds__(32 * W, min_ctas(HD, W)) decode_kernel(const P
     };
     if (warp == 0) {   // the first NSTAGE stream stages
         uint32_t jn = blockIdx.x, it = 0, n = stages_of(jn);
-        for (uint32_t g = 0; g < NSTAGE; g++) {
+        for (uint32_t g = 0; g < NSTAGE && n > 0; g++) {
             issue(jn, it, g);
             if (++it == n) {
+                if constexpr (PAGED) break;
                 it = 0;
                 jn += gridDim.x;
                 if (jn >= p.n_jobs) break;
@@ -284,8 +331,14 @@ __global__ void __launch_bounds__(32 * W, min_ctas(HD, W)) decode_kernel(const P
 
     uint32_t gst = 0;   // stream stage
     for (uint32_t jc = blockIdx.x; ok && jc < p.n_jobs; jc += gridDim.x) {
-    const Job job = p.jobs[jc];
-    const uint32_t n_stages = (job.nk + STAGE_KEYS - 1) / STAGE_KEYS;
+    Job job;
+    if constexpr (PAGED) {
+        job.set = s_part.set;
+        job.slot = blockIdx.x;
+    } else {
+        job = p.jobs[jc];
+    }
+    const uint32_t n_stages = stages_of(jc);
     const uint32_t g0 = gst;
 
     // Q fragments (B operand of S^T = K.Q^T): row n = g of this row group, k values permuted as dK
@@ -351,7 +404,23 @@ __global__ void __launch_bounds__(32 * W, min_ctas(HD, W)) decode_kernel(const P
     for (uint32_t it = 0; it < n_stages; it++, gst++) {
         const uint32_t s = gst % NSTAGE;
         if (!mbar_wait_bounded(&full[s], (gst / NSTAGE) & 1, p.timeout_ns, abort_flag)) { ok = false; break; }
-        const uint32_t valid = min((uint32_t) STAGE_KEYS, job.nk - it * STAGE_KEYS);
+        uint32_t valid = STAGE_KEYS;
+        if constexpr (!PAGED) valid = min((uint32_t) STAGE_KEYS, job.nk - it * STAGE_KEYS);
+        // PAGED: bit k of see0 / see1: rows 2t / 2t+1 of the group see key k of the stage; of live: any row of the group
+        bool edge = false;
+        uint32_t see0 = 0xFFFFu, see1 = 0xFFFFu, live = 0xFFFFu;
+        if constexpr (PAGED) {
+            const int k0 = span.group((int) (pg0 + it)) * STAGE_KEYS;
+            edge = !s_tile.full(k0, STAGE_KEYS);
+            if (edge) {
+                const uint32_t r = rg * 8 + 2 * t, T = p.pg.v.n_tok;
+                see0 = (uint32_t) (pg::vis64(pg::row_of(p.pg.v, s_part.st, s_part.set, r % T), k0 & ~63) >> (k0 & 63)) & 0xFFFFu;
+                see1 = (uint32_t) (pg::vis64(pg::row_of(p.pg.v, s_part.st, s_part.set, (r + 1) % T), k0 & ~63) >> (k0 & 63)) & 0xFFFFu;
+                live = see0 | see1;
+                live |= __shfl_xor_sync(0xffffffffu, live, 1);
+                live |= __shfl_xor_sync(0xffffffffu, live, 2);
+            }
+        }
         const uint32_t kbase = smem_u32(smem + s * stage_bytes) + hoff;
         const uint32_t vbase = kbase + half_stage;
         for (uint32_t tt = 0; tt < STAGE_KEYS / TILE_KEYS; tt++) {
@@ -501,6 +570,11 @@ __global__ void __launch_bounds__(32 * W, min_ctas(HD, W)) decode_kernel(const P
                 for (int kk = 0; kk < 4; kk++)
                     if ((int) key[kk] >= tvalid) sc[kk] = 0u;
             }
+            if (PAGED && edge) {
+#pragma unroll
+                for (int kk = 0; kk < 4; kk++)
+                    if (!(live >> key[kk] & 1u)) sc[kk] = 0u;
+            }
             // key pairs: (key0,key1) -> a0/a1, (key2,key3) -> a2/a3
             s01 = sc[0] | (sc[1] << 16);
             s23 = sc[2] | (sc[3] << 16);
@@ -510,6 +584,12 @@ __global__ void __launch_bounds__(32 * W, min_ctas(HD, W)) decode_kernel(const P
             if (tvalid < TILE_KEYS) {
                 if ((int) (2 * g) >= tvalid) c[0] = c[1] = -INFINITY;       // row g = key 2g
                 if ((int) (2 * g + 1) >= tvalid) c[2] = c[3] = -INFINITY;   // row g+8 = key 2g+1
+            }
+            if (PAGED && edge) {
+                if (!(see0 >> (2 * g) & 1u)) c[0] = -INFINITY;
+                if (!(see1 >> (2 * g) & 1u)) c[1] = -INFINITY;
+                if (!(see0 >> (2 * g + 1) & 1u)) c[2] = -INFINITY;
+                if (!(see1 >> (2 * g + 1) & 1u)) c[3] = -INFINITY;
             }
             float mx0 = fmaxf(c[0], c[2]), mx1 = fmaxf(c[1], c[3]);
             ml0 = fmaxf(ml0, mx0);
@@ -550,6 +630,10 @@ __global__ void __launch_bounds__(32 * W, min_ctas(HD, W)) decode_kernel(const P
                     if (tvalid < TILE_KEYS) {
                         m01 = ((int) key[0] < tvalid ? 0x0000FFFFu : 0u) | ((int) key[1] < tvalid ? 0xFFFF0000u : 0u);
                         m23 = ((int) key[2] < tvalid ? 0x0000FFFFu : 0u) | ((int) key[3] < tvalid ? 0xFFFF0000u : 0u);
+                    }
+                    if (PAGED && edge) {
+                        m01 = (live >> key[0] & 1u ? 0x0000FFFFu : 0u) | (live >> key[1] & 1u ? 0xFFFF0000u : 0u);
+                        m23 = (live >> key[2] & 1u ? 0x0000FFFFu : 0u) | (live >> key[3] & 1u ? 0xFFFF0000u : 0u);
                     }
 #pragma unroll
                     for (int mt = 0; mt < NMT; mt++) {
@@ -623,6 +707,11 @@ __global__ void __launch_bounds__(32 * W, min_ctas(HD, W)) decode_kernel(const P
         l1 += __shfl_xor_sync(0xffffffffu, l1, x);
     }
 
+    if constexpr (PAGED) {   // a padding token's row is empty, whatever its scores were
+        const uint32_t r = rg * 8 + 2 * t, T = p.pg.v.n_tok;
+        if (pg::is_padding(p.pg.v, s_part.set, r % T)) l0 = 0.f;
+        if (pg::is_padding(p.pg.v, s_part.set, (r + 1) % T)) l1 = 0.f;
+    }
     // ---- write the job's slot partial
     const uint64_t rbase = ((uint64_t) job.slot * p.nkv + h) * p.rows;
     const uint32_t r0 = rg * 8 + 2 * t, r1 = r0 + 1;

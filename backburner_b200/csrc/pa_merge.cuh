@@ -24,6 +24,8 @@ struct Params {
     uint64_t rows_per_set;       // nkv * rows
     uint32_t n_sets;
     int fold;                    // 1: (O, M, L) already hold a partial to fold in
+    uint16_t *Oh;                // REPLY: f16(O / l) and lse = m + log l instead of O, M, L (normalize_kernel's)
+    float *lse;
 };
 
 // SPLIT warps per output row (1: 8 rows per 256-thread block; 8: one row per block, for calls with few rows and many
@@ -32,7 +34,7 @@ struct Params {
 // memory, and every warp accumulates sum_c w_c O_c, sum_c w_c l_c against that same M, so the warps' sums simply add.
 // Weights are computed 32 parts at a time (one per lane) and broadcast; the O loads of a batch do not depend on one
 // another, and a part with l <= 0 (no keys) gets weight 0 and its O is not used.
-template <int HD, int SPLIT>
+template <int HD, int SPLIT, bool REPLY = false>
 __global__ void __launch_bounds__(256) merge_kernel(const Params p) {
     constexpr int V = HD / 32;          // floats per lane
     constexpr int RPB = 8 / SPLIT;      // rows per block
@@ -136,6 +138,14 @@ __global__ void __launch_bounds__(256) merge_kernel(const Params p) {
         }
     }
     if (!active) return;
+    if constexpr (REPLY) {
+        const float inv = Ls > 0.f ? 1.f / Ls : 0.f;
+#pragma unroll
+        for (int i = 0; i < V; i += 2)
+            *reinterpret_cast<uint32_t *>(p.Oh + orow * HD + lane * V + i) = pack_h2(acc[i] * inv, acc[i + 1] * inv);
+        if (lane == 0) p.lse[orow] = Ls > 0.f ? M + logf(Ls) : -INFINITY;
+        return;
+    }
     float4 *dst = reinterpret_cast<float4 *>(p.O + orow * HD + lane * V);
 #pragma unroll
     for (int i = 0; i < V / 4; i++) dst[i] = make_float4(acc[4 * i], acc[4 * i + 1], acc[4 * i + 2], acc[4 * i + 3]);

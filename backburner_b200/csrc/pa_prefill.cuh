@@ -57,6 +57,12 @@ struct Params {
     uint64_t timeout_ns;
     int stall;                    // test hook: the softmax warps first wait on a barrier that nothing completes (bounded)
 };
+// the paged kernel's: jobs unused; kv_maps: K and V rows of the whole cache
+struct PagedParams : Params {
+    pg::Paged pg;
+};
+template <bool PAGED> struct ParamsOf { using type = Params; };
+template <> struct ParamsOf<true> { using type = PagedParams; };
 
 // ---------------------------------------------------------------- tcgen05 / TMA helpers
 __device__ __forceinline__ void tma_2d(void *dst, const void *tmap, int x, int y, uint64_t *bar) {
@@ -237,9 +243,13 @@ struct Smem {
     static constexpr int TOTAL = BAR + N_BAR * 8 + 32;
 };
 
-template <int QUANT, int NT, int D = 128>
+// PAGED: the keys come from a paged cache and the rows see them through a mask (pa_mask.cuh). A block is B / 64 groups of 64
+// keys, each copied from its own page; the CTA walks its share of the groups its own row tile sees. Only groups at the edge of
+// what the tile's rows see are masked (a thread has its row's 64-bit word for the group); keys no row of the tile sees get a
+// zero V scale in the dequantisers, since their rows may hold NaN (a masked K row only reaches its own masked scores).
+template <int QUANT, int NT, int D = 128, bool PAGED = false>
 __global__ void __launch_bounds__(32 * cta_warps(NT), 1) prefill_kernel(const __grid_constant__ CUtensorMap tq,
-                                                                       const Params p) {
+                                                                       const typename ParamsOf<PAGED>::type p) {
     using L = Smem<QUANT, NT, D>;
     constexpr int KVB = L::KVB;
     constexpr int B = L::B;   // keys per block
@@ -287,9 +297,15 @@ __global__ void __launch_bounds__(32 * cta_warps(NT), 1) prefill_kernel(const __
     // blocks (all row groups and heads of one chunk of keys) run at the same time and share them through L2
     const uint32_t cid = blockIdx.x;
     const uint32_t rt = cid % p.n_rt, h = (cid / p.n_rt) % p.nkv;
-    const dec::Job job = p.jobs[cid / (p.n_rt * p.nkv)];
     const uint32_t warp = threadIdx.x / 32, lane = threadIdx.x % 32;
-    const uint32_t nblk = (job.nk + B - 1) / B;
+    dec::Job job;
+    uint32_t nblk = 0;
+    if constexpr (PAGED) {
+        job.slot = cid / (p.n_rt * p.nkv);
+    } else {
+        job = p.jobs[cid / (p.n_rt * p.nkv)];
+        nblk = (job.nk + B - 1) / B;
+    }
     const uint32_t hbyte = h * (uint32_t) p.hb;
     const int hx = (int) (hbyte & ~15u);          // window start (16-byte aligned) of this head in a key row
     const uint32_t hoff = hbyte & 15u;            // head start inside the window
@@ -325,8 +341,34 @@ __global__ void __launch_bounds__(32 * cta_warps(NT), 1) prefill_kernel(const __
         *abort_flag = *(volatile int *) p.status != ST_OK;
         fence_mbar_init();
     }
+    __shared__ pg::Part s_part;
+    __shared__ pg::Tile s_tile;
+    pg::Span span{};
+    uint32_t pg0 = 0, pgn = 0;   // PAGED: this CTA's groups [pg0, pg0 + pgn) of its row tile's span
+    if constexpr (PAGED) {
+        // the tokens of the tile's rows (row r: token r % n_tok): all of them when the rows pass the last token
+        const uint32_t T = p.pg.v.n_tok, n = min((uint32_t) (NT * BM), p.rows - row0), a = row0 % T;
+        const uint32_t t0 = a + n > T ? 0u : a, t1 = a + n > T ? T - 1 : a + n - 1;
+        if (warp == 2) {
+            const pg::Part f = pg::find_part<64>(p.pg, job.slot, cid == 0, lane);
+            const pg::Tile tl = pg::tile_of(p.pg.v, f.st, f.set, t0, t1, lane);
+            if (lane == 0) {
+                s_part = f;
+                s_tile = tl;
+            }
+        }
+        __syncthreads();
+        job.set = s_part.set;
+        span = pg::span_of<64>(p.pg.v, s_part.st, t0, t1);
+        if (s_part.of) {
+            const uint32_t per = ((uint32_t) span.n + s_part.of - 1) / s_part.of;
+            pg0 = min(s_part.index * per, (uint32_t) span.n);
+            pgn = min(per, (uint32_t) span.n - pg0);
+        }
+        nblk = (pgn + B / 64 - 1) / (B / 64);
+    }
     __syncthreads();
-    if (*abort_flag) return;   // uniform: before TMEM is allocated
+    if (*abort_flag || (PAGED && s_part.of == 0)) return;   // uniform: before TMEM is allocated
     if (warp == 1) {   // TMEM: per tile S, two P buffers and O; one tile: a second S
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)),
                      "r"(TCOLS)
@@ -371,11 +413,20 @@ __global__ void __launch_bounds__(32 * cta_warps(NT), 1) prefill_kernel(const __
             for (uint32_t j = 0; j < nblk; j++) {
                 const uint32_t st = j % NRS;
                 if (j >= NRS && !wait(&raw_empty[st], ((j / NRS) - 1) & 1)) break;
-                mbar_arrive_expect_tx(&raw_full[st], 2 * B * RAWB);
+                // PAGED: the last block may hold one group fewer
+                const uint32_t copies = PAGED ? min((uint32_t) (B / BN), pgn - j * (B / BN)) : (uint32_t) (B / BN);
+                mbar_arrive_expect_tx(&raw_full[st], 2 * copies * BN * RAWB);
                 uint8_t *dst = smem + L::RAW + st * L::RAW_STAGE;
 #pragma unroll
                 for (int c = 0; c < B / BN; c++) {   // the tensor maps' boxes hold 64 keys
-                    const int key = (int) (job.key0 + j * B) + c * BN;
+                    int key;
+                    if constexpr (PAGED) {
+                        if (c >= (int) copies) break;
+                        key = (int) (p.pg.row0 + pg::row_at(p.pg.v, job.set,
+                                                            (uint32_t) span.group((int) (pg0 + j * (B / BN)) + c) * BN));
+                    } else {
+                        key = (int) (job.key0 + j * B) + c * BN;
+                    }
                     tma_2d(dst + c * BN * RAWB, km, hx / 2, key, &raw_full[st]);
                     tma_2d(dst + (B + c * BN) * RAWB, vm, hx / 2, key, &raw_full[st]);
                 }
@@ -498,6 +549,8 @@ __global__ void __launch_bounds__(32 * cta_warps(NT), 1) prefill_kernel(const __
         }
         float m_used = -INFINITY, l = 0.f;
         float m_row = -INFINITY;   // the row's exact maximum (log2 units); O and l are reported against it
+        pg::Row mine{};
+        if constexpr (PAGED) mine = pg::row_of(p.pg.v, s_part.st, job.set, (row0 + t * BM + r) % p.pg.v.n_tok);
         for (uint32_t j = 0; j < nblk && !pad; j++) {
             const uint32_t b = j % NPB;                    // the block's P buffer
             const uint32_t sb = t * NSB + j % NSB;         // the block's S buffer
@@ -518,11 +571,28 @@ __global__ void __launch_bounds__(32 * cta_warps(NT), 1) prefill_kernel(const __
             tc_fence_before();
             __syncwarp();
             if (lane == 0) mbar_arrive(&s_empty[sb]);
+            if constexpr (PAGED) {
+#pragma unroll
+                for (int c = 0; c < B / 64; c++) {
+                    const uint32_t gi = j * (B / 64) + c;   // the group within the CTA's
+                    const int k0 = span.group((int) (pg0 + gi)) * 64;
+                    if (gi >= pgn || !s_tile.full(k0, 64)) {
+                        const uint64_t see = gi < pgn ? pg::vis64(mine, k0) : 0ull;
+                        const uint32_t lo = (uint32_t) see, hi = (uint32_t) (see >> 32);
+#pragma unroll
+                        for (int i = 0; i < 32; i++) {
+                            if (!(lo >> i & 1u)) s[64 * c + i] = -INFINITY;
+                            if (!(hi >> i & 1u)) s[64 * c + 32 + i] = -INFINITY;
+                        }
+                    }
+                }
+            } else {
             const int nvalid = (int) (job.nk - j * B);
             if (nvalid < B) {
 #pragma unroll
                 for (int i = 0; i < B; i++)
                     if (i >= nvalid) s[i] = -INFINITY;
+            }
             }
             float mx = s[0];
 #pragma unroll
@@ -532,7 +602,7 @@ __global__ void __launch_bounds__(32 * cta_warps(NT), 1) prefill_kernel(const __
             m_row = fmaxf(m_row, mx);
             float alpha = 1.f;
             bool rescale = false;
-            if (j == 0) m_used = mx;
+            if (j == 0) m_used = PAGED ? fmaxf(mx, M_EMPTY) : mx;   // PAGED: the row may see nothing of the block
             else if (mx > m_used + 8.f) {
                 alpha = ex2(m_used - mx);
                 m_used = mx;
@@ -586,6 +656,9 @@ __global__ void __launch_bounds__(32 * cta_warps(NT), 1) prefill_kernel(const __
             tc_fence_after();
             const uint32_t row = row0 + t * BM + r;
             const uint64_t orow = ((uint64_t) job.slot * p.nkv + h) * p.rows + row;
+            if constexpr (PAGED) {   // a padding token's row is empty, whatever its scores were
+                if (pg::is_padding(p.pg.v, job.set, row % p.pg.v.n_tok)) l = 0.f;
+            }
             const float fix = m_row > -INFINITY ? ex2(m_used - m_row) : 1.f;
 #pragma unroll
             for (int q = 0; q < D / 32; q++) {
@@ -604,6 +677,14 @@ __global__ void __launch_bounds__(32 * cta_warps(NT), 1) prefill_kernel(const __
                 p.Lp[orow] = l * fix;
             }
         }
+        if constexpr (PAGED) {   // a part of the set that holds nothing for this row tile
+            const uint32_t row = row0 + t * BM + r;
+            if (nblk == 0 && row < p.rows) {
+                const uint64_t orow = ((uint64_t) job.slot * p.nkv + h) * p.rows + row;
+                p.Mp[orow] = -INFINITY;
+                p.Lp[orow] = 0.f;
+            }
+        }
     } else {
         // ------------------------------------------------ dequantisers: warp dw owns quant blocks dw % 4 (+ 4 at
         // D = 256) of every key (4 warps: both 32-key halves of each 64 keys; 8 warps, NT = 1: key half dw / 4 of each
@@ -615,6 +696,15 @@ __global__ void __launch_bounds__(32 * cta_warps(NT), 1) prefill_kernel(const __
             const uint32_t st = j % NRS, b = j % KVB;
             if (!wait(&raw_full[st], (j / NRS) & 1)) break;
             const uint32_t raw = sbase + L::RAW + st * L::RAW_STAGE;
+            uint64_t live[B / 64];   // PAGED: keys of each group that some row of the tile sees
+            if constexpr (PAGED) {
+#pragma unroll
+                for (int c = 0; c < B / 64; c++) {
+                    const uint32_t gi = j * (B / 64) + c;
+                    const int k0 = span.group((int) (pg0 + gi)) * 64;
+                    live[c] = gi >= pgn ? 0ull : s_tile.full(k0, 64) ? ~0ull : pg::vis64(s_tile.any, k0);
+                }
+            }
 #pragma unroll
             for (int kv = 0; kv < 2; kv++) {
                 if (j >= KVB && !wait(kv == 0 ? &k_free[b] : &v_free[b], ((j / KVB) - 1) & 1)) break;
@@ -632,7 +722,10 @@ __global__ void __launch_bounds__(32 * cta_warps(NT), 1) prefill_kernel(const __
                     const uint32_t dst = sbase + (kv == 0 ? L::K : L::V) + b * B * D * 2 + (qblk / 2) * B * 128;
                     const uint32_t key = 64 * (uint32_t) kc + (NDQ == 8 ? dw / 4 : (uint32_t) pass) * 32 + lane;
                     const uint32_t rb = src + key * RAWB;
-                    const uint32_t s2 = lds16(rb + bo);
+                    uint32_t s2 = lds16(rb + bo);
+                    if constexpr (PAGED) {
+                        if (kv == 1 && !(live[kc] >> (key % 64) & 1ull)) s2 = 0u;
+                    }
                     const uint32_t sc2 = s2 | (s2 << 16);
                     uint32_t W[12];
                     // q8_0: the block's 34 bytes lie within 3 aligned 16-byte chunks; q4_0: 18 bytes within 2
