@@ -544,7 +544,7 @@ class Engine:
 # ---------------------------------------------------------------- paged cache
 def _want(ctx: Context, t, name: str, dtype, shape):
     """Pointer of a contiguous tensor of this type and shape on the context's device; anything else is an error."""
-    if t.dtype is not dtype or tuple(t.shape) != shape or not t.is_contiguous() or t.get_device() != ctx.device:
+    if t.dtype is not dtype or t.shape != shape or not t.is_contiguous() or t.get_device() != ctx.device:
         raise PaCudaError(EINVAL, f"{name}: needs a contiguous {dtype} tensor {shape} on cuda:{ctx.device}, got "
                                   f"{t.dtype} {tuple(t.shape)} on {t.device}")
     return t.data_ptr()
@@ -554,7 +554,7 @@ def _stream_on(ctx: Context, stream) -> int:
     """_stream_ptr for the context's device, whatever the current one is."""
     if stream is None:
         import torch
-        stream = torch.cuda.current_stream(ctx.device)
+        return torch._C._cuda_getCurrentRawStream(ctx.device) or 1   # (current_stream's handle, without its Stream object)
     return _stream_ptr(stream)
 
 
@@ -589,15 +589,16 @@ class Cache:
         self.n_layers, self.n_pages, self.page_keys, self.rs = K.shape
         self.hb = head_bytes(quant, hd)
         self.device = K.get_device()
-        self._c = _Cache(K.data_ptr(), V.data_ptr(), self.n_layers, self.n_pages, self.page_keys)
+        self._c = ctypes.byref(_Cache(K.data_ptr(), V.data_ptr(), self.n_layers, self.n_pages, self.page_keys))
 
-    def shape(self, rows: int) -> _Shape:
-        return _Shape(self.hd, self.nkv, rows, self.quant, self.rs, self.hb)
+    def shape(self, rows: int):
+        """A reference to the C geometry with this many query rows per KV head."""
+        return ctypes.byref(_Shape(self.hd, self.nkv, rows, self.quant, self.rs, self.hb))
 
     def on(self, ctx: Context):
         if self.device != ctx.device:
             raise PaCudaError(EINVAL, f"the cache is on cuda:{self.device}, the context on cuda:{ctx.device}")
-        return ctypes.byref(self._c)
+        return self._c
 
 
 class CachePlan:
@@ -609,10 +610,11 @@ class CachePlan:
         self.ctx, self.cache, self.n_sets, self.n_tok, self.gqa = ctx, cache, n_sets, n_tok, gqa
         self.max_pages, self.tree = max_pages, bool(tree)
         self._h = _P()
-        sh, mask = cache.shape(gqa * n_tok), _Mask(n_tok, window, sinks, 1 if tree else 0)
-        ctx.check(lib().pa_cuda_cache_plan_create(ctx.handle, ctypes.byref(sh), cache.on(ctx), n_sets, max_pages,
+        mask = _Mask(n_tok, window, sinks, 1 if tree else 0)
+        ctx.check(lib().pa_cuda_cache_plan_create(ctx.handle, cache.shape(gqa * n_tok), cache.on(ctx), n_sets, max_pages,
                                                   ctypes.byref(mask), ctypes.byref(self._h)), "cache_plan_create")
         self._rows = (n_sets, cache.nkv, gqa * n_tok)
+        self._full = self._rows + (cache.hd,)
 
     @property
     def kernel(self) -> str:
@@ -624,7 +626,7 @@ class CachePlan:
         ctx, i32, per = self.ctx, torch.int32, (self.n_sets,)
         if (tree is not None) != self.tree:
             raise PaCudaError(EINVAL, "a tree plan takes the tree's masks, another plan none")
-        return (self._h, layer, _want(ctx, Qs, "Qs", torch.float16, self._rows + (self.cache.hd,)),
+        return (self._h, layer, _want(ctx, Qs, "Qs", torch.float16, self._full),
                 _want(ctx, table, "table", i32, (self.n_sets, self.max_pages)), _want(ctx, n_keys, "n_keys", i32, per),
                 None if q_pos is None else _want(ctx, q_pos, "q_pos", i32, per),
                 None if tree is None else _want(ctx, tree, "tree", torch.int64, (self.n_sets, self.n_tok)))
@@ -639,7 +641,7 @@ class CachePlan:
             m = torch.empty(self._rows, dtype=f32, device=Qs.device)
             out = (O, m, torch.empty_like(m))
         O, m, l = out
-        self.ctx.check(lib().pa_cuda_cache_attn(*args, _want(self.ctx, O, "O", f32, tuple(Qs.shape)),
+        self.ctx.check(lib().pa_cuda_cache_attn(*args, _want(self.ctx, O, "O", f32, self._full),
                                                 _want(self.ctx, m, "m", f32, self._rows),
                                                 _want(self.ctx, l, "l", f32, self._rows), _stream_on(self.ctx, stream)),
                        "cache_attn")
@@ -650,10 +652,9 @@ class CachePlan:
         import torch
         args = self._args(layer, Qs, table, n_keys, q_pos, tree)
         if out is None:
-            out = (torch.empty(Qs.shape, dtype=torch.float16, device=Qs.device),
-                   torch.empty(self._rows, dtype=torch.float32, device=Qs.device))
+            out = torch.empty_like(Qs), Qs.new_empty(self._rows, dtype=torch.float32)
         Oh, lse = out
-        self.ctx.check(lib().pa_cuda_cache_attn_reply(*args, _want(self.ctx, Oh, "Oh", torch.float16, tuple(Qs.shape)),
+        self.ctx.check(lib().pa_cuda_cache_attn_reply(*args, _want(self.ctx, Oh, "Oh", torch.float16, self._full),
                                                       _want(self.ctx, lse, "lse", torch.float32, self._rows),
                                                       _stream_on(self.ctx, stream)), "cache_attn_reply")
         return Oh, lse
@@ -670,6 +671,15 @@ class CachePlan:
             pass
 
 
+_kinds = {}
+
+
+def _kinds_of(torch):
+    """PA_CUDA_T_* of the types cache_append takes."""
+    _kinds.update({torch.float16: 0, torch.bfloat16: 1, torch.float32: 2})
+    return _kinds
+
+
 def cache_append(ctx: Context, cache: Cache, layer: int, q, k, v, table, start, pos=None, wq=None, wk=None, freqs=None,
                  eps: float = 1e-6, scale: float = 1.0, interleaved: bool = False, out=None, stream=None):
     """Head norm and rotation of new queries and keys, and the append of their rows (pa_cuda_cache_append). q
@@ -677,39 +687,38 @@ def cache_append(ctx: Context, cache: Cache, layer: int, q, k, v, table, start, 
     [hd]; freqs float64 [rot / 2]; table int32 [n_sets][max_pages]; start int32 [n_sets]: key index of token 0; pos int32
     [n_sets][n_tok] (< 0: padding). Returns Qs f16 [n_sets][nkv][gqa * n_tok][hd], what CachePlan takes."""
     import torch
+    kinds = _kinds or _kinds_of(torch)
     S, T, nq, hd = q.shape
-    kv = (S, T, cache.nkv, cache.hd)
-    kinds = {torch.float16: 0, torch.bfloat16: 1, torch.float32: 2}
-    if hd != cache.hd or nq == 0 or nq % cache.nkv or tuple(k.shape) != kv or tuple(v.shape) != kv or q.dtype not in kinds:
-        raise PaCudaError(EINVAL, f"cache_append: q {tuple(q.shape)} {q.dtype}, k {tuple(k.shape)}, v {tuple(v.shape)} do "
-                                  f"not fit nkv {cache.nkv}, hd {cache.hd} (f16, bf16 or f32)")
-    st = []
-    for name, t in (("q", q), ("k", k), ("v", v)):
-        s = t.stride()
-        if t.dtype is not q.dtype or t.get_device() != ctx.device or (s[3] != 1 and hd > 1) or (s[2] != hd and t.shape[2] > 1):
-            raise PaCudaError(EINVAL, f"cache_append: {name} needs heads of hd consecutive elements, hd apart, of q's type, "
-                                      f"on cuda:{ctx.device}")
-        st += [s[0], s[1]]
-    w_dtype = kinds[q.dtype]
-    for name, w in (("wq", wq), ("wk", wk)):
-        if w is not None:
-            w_dtype = kinds.get(w.dtype, 3)
-            _want(ctx, w, name, w.dtype, (hd,))
-    if wq is not None and wk is not None and wq.dtype is not wk.dtype:
-        raise PaCudaError(EINVAL, "cache_append: wq and wk differ in type")
-    rot = 0 if freqs is None else 2 * freqs.numel()
-    a = _Append(q.data_ptr(), k.data_ptr(), v.data_ptr(), *st, _ptr(wq) or None, _ptr(wk) or None,
+    kv, dt, dev = (S, T, cache.nkv, cache.hd), q.dtype, ctx.device
+    if hd != cache.hd or nq == 0 or nq % cache.nkv or k.shape != kv or v.shape != kv or dt not in kinds:
+        raise PaCudaError(EINVAL, f"cache_append: q {tuple(q.shape)} {dt}, k {tuple(k.shape)}, v {tuple(v.shape)} do not fit "
+                                  f"nkv {cache.nkv}, hd {cache.hd} (f16, bf16 or f32)")
+    qs, ks, vs = q.stride(), k.stride(), v.stride()
+    if (qs[3] != 1 or ks[3] != 1 or vs[3] != 1 or (qs[2] != hd and nq > 1) or ((ks[2] != hd or vs[2] != hd) and kv[2] > 1) or
+            k.dtype is not dt or v.dtype is not dt or q.get_device() != dev or k.get_device() != dev or v.get_device() != dev):
+        raise PaCudaError(EINVAL, f"cache_append: q, k and v need one type and heads of hd consecutive elements, hd apart, on "
+                                  f"cuda:{dev}")
+    w_dtype = kinds[dt]
+    if wq is not None or wk is not None:
+        w = wk if wq is None else wq
+        w_dtype = kinds.get(w.dtype, 3)
+        if wq is not None:
+            _want(ctx, wq, "wq", w.dtype, (hd,))
+        if wk is not None:
+            _want(ctx, wk, "wk", w.dtype, (hd,))
+    rot = 0 if freqs is None else 2 * freqs.shape[0]
+    a = _Append(q.data_ptr(), k.data_ptr(), v.data_ptr(), qs[0], qs[1], ks[0], ks[1], vs[0], vs[1],
+                None if wq is None else wq.data_ptr(), None if wk is None else wk.data_ptr(),
                 None if freqs is None else _want(ctx, freqs, "freqs", torch.float64, (rot // 2,)),
                 None if pos is None else _want(ctx, pos, "pos", torch.int32, (S, T)),
-                kinds[q.dtype], w_dtype, rot, 1 if interleaved else 0, eps, scale)
-    rows = (S, cache.nkv, nq // cache.nkv * T, hd)
+                kinds[dt], w_dtype, rot, 1 if interleaved else 0, eps, scale)
+    n_rows = nq // cache.nkv * T
+    rows = (S, cache.nkv, n_rows, hd)
     if out is None:
-        out = torch.empty(rows, dtype=torch.float16, device=q.device)
-    if table.dim() != 2:
-        raise PaCudaError(EINVAL, "table: needs int32 [n_sets][max_pages]")
-    sh = cache.shape(max(1, nq // cache.nkv * T))
-    ctx.check(lib().pa_cuda_cache_append(ctx.handle, ctypes.byref(sh), cache.on(ctx), layer, ctypes.byref(a), S, T,
-                                         _want(ctx, table, "table", torch.int32, (S, table.shape[1])), table.shape[1],
+        out = q.new_empty(rows, dtype=torch.float16)
+    pages = table.shape[-1]
+    ctx.check(lib().pa_cuda_cache_append(ctx.handle, cache.shape(n_rows or 1), cache.on(ctx), layer, ctypes.byref(a), S, T,
+                                         _want(ctx, table, "table", torch.int32, (S, pages)), pages,
                                          _want(ctx, start, "start", torch.int32, (S,)),
                                          _want(ctx, out, "out", torch.float16, rows), _stream_on(ctx, stream)),
               "cache_append")
@@ -723,10 +732,9 @@ def cache_rows(ctx: Context, cache: Cache, layer: int, table, first, n: int, out
     S = table.shape[0]
     shape = (S, n, cache.nkv, cache.hd)
     if out is None:
-        K = torch.empty(shape, dtype=torch.float16, device=table.device)
+        K = table.new_empty(shape, dtype=torch.float16)
         out = (K, torch.empty_like(K))
-    sh = cache.shape(1)
-    ctx.check(lib().pa_cuda_cache_rows(ctx.handle, ctypes.byref(sh), cache.on(ctx), layer, S, n,
+    ctx.check(lib().pa_cuda_cache_rows(ctx.handle, cache.shape(1), cache.on(ctx), layer, S, n,
                                        _want(ctx, table, "table", torch.int32, (S, table.shape[1])), table.shape[1],
                                        _want(ctx, first, "first", torch.int32, (S,)),
                                        _want(ctx, out[0], "K", torch.float16, shape),
@@ -739,8 +747,7 @@ def cache_copy_pages(ctx: Context, cache: Cache, src, dst, stream=None):
     prefix copies the page it will write to. No page is both read and written in one call."""
     import torch
     n = src.numel()
-    sh = cache.shape(1)
-    ctx.check(lib().pa_cuda_cache_copy_pages(ctx.handle, ctypes.byref(sh), cache.on(ctx),
+    ctx.check(lib().pa_cuda_cache_copy_pages(ctx.handle, cache.shape(1), cache.on(ctx),
                                              _want(ctx, src, "src", torch.int32, (n,)),
                                              _want(ctx, dst, "dst", torch.int32, (n,)), n, _stream_on(ctx, stream)),
               "cache_copy_pages")
@@ -754,8 +761,7 @@ def cache_compact(ctx: Context, cache: Cache, table, start, path, count, out=Non
     S, T = path.shape
     if out is None:
         out = torch.empty((S,), dtype=torch.int32, device=path.device)
-    sh = cache.shape(1)
-    ctx.check(lib().pa_cuda_cache_compact(ctx.handle, ctypes.byref(sh), cache.on(ctx), S, T,
+    ctx.check(lib().pa_cuda_cache_compact(ctx.handle, cache.shape(1), cache.on(ctx), S, T,
                                           _want(ctx, table, "table", torch.int32, (S, table.shape[1])), table.shape[1],
                                           _want(ctx, start, "start", torch.int32, (S,)),
                                           _want(ctx, path, "path", torch.int32, (S, T)),

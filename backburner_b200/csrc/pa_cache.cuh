@@ -14,19 +14,6 @@
 namespace pa {
 namespace pg {
 
-// ---------------------------------------------------------------- elements of a head
-// value i of a head row: f16(d * q), or the f16 itself
-template <int QUANT>
-__device__ __forceinline__ float head_value(const uint8_t *head, int i) {
-    if (QUANT == 0) return __half2float(reinterpret_cast<const __half *>(head)[i]);
-    const uint8_t *blk = head + (i / 32) * dec::q_group_bytes(QUANT);
-    const __half d = *reinterpret_cast<const __half *>(blk);
-    int q;
-    if (QUANT == 1) q = (int8_t) blk[2 + i % 32];
-    else q = (int) ((blk[2 + i % 16] >> (i % 32 < 16 ? 0 : 4)) & 15) - 8;
-    return __half2float(__hmul(d, __int2half_rn(q)));
-}
-
 // ---------------------------------------------------------------- append: head norm, rotation, scale, quantised store
 // q, k: y = x * rsqrt(mean(x^2) + eps) * w (no weight: y = x); the first `rot` dims turned in pairs by angle pos * freq;
 // queries leave as f16(y * scale) in the attention calls' layout [set][nkv][gqa * n_tok][hd] (row g * n_tok + t), keys and the
@@ -44,207 +31,328 @@ struct AppendParams {
     uint64_t rs, hb;
     uint32_t nkv, gqa, rot;
     float eps, scale;
-    int inter, w32, vec;                                // vec: E-element loads are aligned
+    int inter, w32;
 };
 enum { DT_F16 = 0, DT_BF16 = 1, DT_F32 = 2 };
+// 8 consecutive elements as loaded: 8 fp32 or 4 words of 16-bit pairs
 template <int DT>
-__device__ __forceinline__ float load1(const void *p, int64_t i) {
+__device__ __forceinline__ float load1(const void *p, uint32_t i) {
     if (DT == DT_F32) return reinterpret_cast<const float *>(p)[i];
     const uint32_t x = reinterpret_cast<const uint16_t *>(p)[i];
     return DT == DT_F16 ? h2f_bits(x) : __uint_as_float(x << 16);
 }
-// E consecutive elements from element i
-template <int DT, int E>
-__device__ __forceinline__ void load_e(const void *p, int64_t i, int vec, float (&x)[E]) {
-    if (!vec) {
+template <int DT> constexpr int RAW8 = DT == DT_F32 ? 8 : 4;
+template <int DT, bool VEC>
+__device__ __forceinline__ void load_raw(const uint8_t *p, uint32_t (&w)[RAW8<DT>]) {
+    if constexpr (VEC) {
 #pragma unroll
-        for (int e = 0; e < E; e++) x[e] = load1<DT>(p, i + e);
-    } else if (DT == DT_F32) {
-#pragma unroll
-        for (int e = 0; e < E; e += 4) {
-            const float4 f = *reinterpret_cast<const float4 *>(reinterpret_cast<const float *>(p) + i + e);
-            x[e] = f.x; x[e + 1] = f.y; x[e + 2] = f.z; x[e + 3] = f.w;
+        for (int i = 0; i < RAW8<DT>; i += 4) {
+            const uint4 x = *reinterpret_cast<const uint4 *>(p + 4 * i);
+            w[i] = x.x; w[i + 1] = x.y; w[i + 2] = x.z; w[i + 3] = x.w;
         }
     } else {
-        uint32_t w[E / 2];
-        const uint16_t *src = reinterpret_cast<const uint16_t *>(p) + i;
-        if (E == 8) *reinterpret_cast<uint4 *>(w) = *reinterpret_cast<const uint4 *>(src);
-        else *reinterpret_cast<uint2 *>(w) = *reinterpret_cast<const uint2 *>(src);
 #pragma unroll
-        for (int e = 0; e < E / 2; e++) {
-            x[2 * e] = DT == DT_F16 ? h2f_bits(w[e] & 0xFFFFu) : __uint_as_float(w[e] << 16);
-            x[2 * e + 1] = DT == DT_F16 ? h2f_bits(w[e] >> 16) : __uint_as_float(w[e] & 0xFFFF0000u);
-        }
+        for (int i = 0; i < RAW8<DT>; i++)
+            w[i] = DT == DT_F32 ? *reinterpret_cast<const uint32_t *>(p + 4 * i)
+                                : *reinterpret_cast<const uint16_t *>(p + 4 * i) | (uint32_t) *reinterpret_cast<const uint16_t *>(p + 4 * i + 2) << 16;
     }
 }
-// E consecutive values (lane's dims E * lane ..) of a head into its row: 32 / E lanes share a quant block
-template <int QUANT, int E>
-__device__ __forceinline__ void store_head(uint8_t *head, uint32_t lane, const float (&x)[E]) {
-    if (QUANT == 0) {
+// ... as 4 fp32 pairs
+template <int DT>
+__device__ __forceinline__ void unpack8(const uint32_t (&w)[RAW8<DT>], uint64_t (&x)[4]) {
 #pragma unroll
-        for (int e = 0; e < E; e += 2) *reinterpret_cast<uint32_t *>(head + 2 * (E * lane + e)) = pack_h2(x[e], x[e + 1]);
+    for (int e = 0; e < 4; e++) {
+        if (DT == DT_F32) x[e] = pack_f2(__uint_as_float(w[(2 * e) % RAW8<DT>]), __uint_as_float(w[(2 * e + 1) % RAW8<DT>]));
+        else if (DT == DT_F16) x[e] = pack_f2(h2f_bits(w[e] & 0xFFFFu), h2f_bits(w[e] >> 16));
+        else x[e] = pack_f2(__uint_as_float(w[e] << 16), __uint_as_float(w[e] & 0xFFFF0000u));
+    }
+}
+// 8 consecutive values (dims 8 * l ..) of a head into its row; the 4 lanes of a quant block are neighbours
+template <int QUANT>
+__device__ __forceinline__ void store_head(uint8_t *head, uint32_t l, bool write, const float (&x)[8]) {
+    if (QUANT == 0) {
+        if (write)
+            *reinterpret_cast<uint4 *>(head + 16 * l) = make_uint4(pack_h2(x[0], x[1]), pack_h2(x[2], x[3]), pack_h2(x[4], x[5]), pack_h2(x[6], x[7]));
         return;
     }
-    constexpr int LB = 32 / E, TOP = QUANT == 1 ? 127 : 7;
+    constexpr float TOP = QUANT == 1 ? 127.f : 7.f;
     float am = 0.f;
 #pragma unroll
-    for (int e = 0; e < E; e++) am = fmaxf(am, fabsf(x[e]));
-#pragma unroll
-    for (int w = 1; w < LB; w <<= 1) am = fmaxf(am, __shfl_xor_sync(0xffffffffu, am, w));
-    const __half dh = __float2half_rn(__fdiv_rn(am, (float) TOP));
+    for (int e = 0; e < 8; e++) am = fmaxf(am, fabsf(x[e]));
+    am = fmaxf(am, __shfl_xor_sync(0xffffffffu, am, 1));
+    am = fmaxf(am, __shfl_xor_sync(0xffffffffu, am, 2));
+    const __half dh = __float2half_rn(__fdiv_rn(am, TOP));
     const float df = __half2float(dh), id = df != 0.f ? __frcp_rn(df) : 0.f;
-    uint8_t *blk = head + (lane / LB) * dec::q_group_bytes(QUANT);
-    const uint32_t in = lane % LB;
-    int q[E];
+    uint8_t *blk = head + (l / 4) * dec::q_group_bytes(QUANT);
+    const uint32_t in = l % 4;
+    uint32_t q[8];
 #pragma unroll
-    for (int e = 0; e < E; e++) q[e] = __float2int_rn(fmaxf(-(float) TOP, fminf((float) TOP, __fmul_rn(x[e], id))));
-    if (in == 0) *reinterpret_cast<__half *>(blk) = dh;
-    if (QUANT == 1) {   // blocks start at even bytes: 16-bit stores
+    for (int e = 0; e < 8; e++) q[e] = (uint32_t) __float2int_rn(fmaxf(-TOP, fminf(TOP, __fmul_rn(x[e], id))));
+    if (write && in == 0) *reinterpret_cast<__half *>(blk) = dh;
+    uint16_t *dst = reinterpret_cast<uint16_t *>(blk + 2 + 8 * in);   // blocks start at even bytes: 16-bit stores
+    if (QUANT == 1) {
+        if (write)
 #pragma unroll
-        for (int e = 0; e < E; e += 2)
-            *reinterpret_cast<uint16_t *>(blk + 2 + E * in + e) = (uint16_t) ((q[e] & 0xFF) | (q[e + 1] & 0xFF) << 8);
-    } else {
-        uint32_t n[E];
+            for (int e = 0; e < 8; e += 2) dst[e / 2] = (uint16_t) ((q[e] & 0xFFu) | q[e + 1] << 8);
+    } else {   // byte i: element i, element i + 16 (two lanes on) << 4
+        uint32_t w[4];
 #pragma unroll
-        for (int e = 0; e < E; e++) {
-            const uint32_t own = (uint32_t) (q[e] + 8);
-            n[e] = own | __shfl_down_sync(0xffffffffu, own, LB / 2) << 4;   // element e + 16 is LB / 2 lanes on
+        for (int e = 0; e < 8; e += 2) {
+            const uint32_t own = (q[e] + 8u) | (q[e + 1] + 8u) << 8;
+            w[e / 2] = own | __shfl_down_sync(0xffffffffu, own, 2) << 4;
         }
-        if (in < LB / 2)
+        if (write && in < 2)
 #pragma unroll
-            for (int e = 0; e < E; e += 2) *reinterpret_cast<uint16_t *>(blk + 2 + E * in + e) = (uint16_t) (n[e] | n[e + 1] << 8);
+            for (int i = 0; i < 4; i++) dst[i] = (uint16_t) w[i];
     }
 }
-constexpr int APPEND_WARPS = 8;
-// block = token x group of heads; a warp takes every 8th head of the group (queries, then keys, then values)
-template <int HD, int DT, int QUANT>
-__global__ void __launch_bounds__(32 * APPEND_WARPS) append_kernel(const AppendParams p, uint32_t heads_per_block) {
-    constexpr int E = HD / 32;
-    __shared__ float2 cs[HD / 2];
-    __shared__ float line[APPEND_WARPS][HD];
-    const uint32_t warp = threadIdx.x / 32, lane = threadIdx.x % 32;
-    const uint32_t T = p.view.n_tok, s = blockIdx.x / T, t = blockIdx.x % T;
-    const int start = p.start[s];
-    const int pos = p.pos ? p.pos[blockIdx.x] : clampi((int64_t) start + t, -1, INT32_MAX);
-    const uint32_t nq = p.nkv * p.gqa, h0 = blockIdx.y * heads_per_block, h1 = min(h0 + heads_per_block, nq + 2 * p.nkv);
+constexpr int APPEND_WARPS = 4;
+// heads a block takes in one step of its warps: a lane has 8 dims, so a warp has 2 heads at hd 128 and 1 at hd 256
+__host__ __device__ constexpr int append_heads(int hd) { return APPEND_WARPS * 256 / hd; }
+// Block = token x STEPS * append_heads heads. The heads are numbered queries, then keys, then values, each kind rounded up to
+// whole warps, so that a warp's step is of one kind. A warp loads all its heads before it works on the first, and the loads
+// fly while the block computes the token's angles. Bound: for long prompts memory (the loads alone run at 6 TB/s) and issue
+// (60 instructions a query head's warp step, 160 a key's); for single tokens a chain of a few loads.
+// How a head's pairs meet: halves, by a shuffle to the lane half / 8 away (HALVES: half a multiple of 8); within a lane
+// (PAIRS: interleaved); through shared memory, for any rot, order and alignment (ANY). A template, since the compiler runs
+// the paths not taken as predicated instructions.
+enum { ROT_HALVES = 0, ROT_PAIRS = 1, ROT_ANY = 2 };
+template <int HD, int DT, int QUANT, int STEPS, int ROT>
+__global__ void __launch_bounds__(32 * APPEND_WARPS, 6) append_kernel(const AppendParams p) {
+    constexpr int LPH = HD / 8;   // lanes of a head
+    constexpr int SIZE = DT == DT_F32 ? 4 : 2;
+    __shared__ __align__(16) float2 cs[HD / 2];
+    __shared__ __align__(16) float line[ROT == ROT_ANY ? APPEND_WARPS : 1][256];
+    __shared__ __align__(16) float wsm[2][HD];   // norm weights of queries and keys (1: no norm)
+    __shared__ int64_t s_at;   // byte offset of the new key's row; -1: none is stored
+    const uint32_t warp = threadIdx.x / 32, lane = threadIdx.x % 32, l = lane % LPH;
+    const uint32_t T = p.view.n_tok, s = blockIdx.y, t = blockIdx.x;
+    constexpr uint32_t HPW = 32 / LPH, HPB = append_heads(HD);   // heads of a warp's step, of a block's step
+    const uint32_t uwarp = __shfl_sync(0xffffffffu, warp, 0);    // (known to be the same in all lanes)
+    const uint32_t nq = p.nkv * p.gqa, nqw = (nq + HPW - 1) / HPW * HPW, nkw = (p.nkv + HPW - 1) / HPW * HPW;
+    const uint32_t hw0 = blockIdx.z * (HPB * STEPS) + uwarp * HPW, sub = lane / LPH;
     const uint32_t half = p.rot / 2;
-    if (pos >= 0) {
-        for (uint32_t i = threadIdx.x; i < half; i += 32 * APPEND_WARPS) {
-            const double turn = (double) pos * p.freqs[i] * 0.15915494309189535;   // / (2 pi)
-            float sn, c;
-            sincospif(2.f * (float) (turn - rint(turn)), &sn, &c);
-            cs[i] = make_float2(c, sn);
+    pdl_trigger();
+    pdl_wait();
+    const int start = p.start[s];
+    const int pos = p.pos ? p.pos[(uint64_t) s * T + t] : clampi((int64_t) start + t, -1, INT32_MAX);
+    if (pos < 0) {   // padding: its query rows are zero
+#pragma unroll 1
+        for (uint32_t h = hw0 + sub; h < hw0 + HPB * STEPS && h < nq; h += HPB)
+            *reinterpret_cast<uint4 *>(p.Qs + (((uint64_t) s * nq + h) * T + t) * HD + 8 * l) = make_uint4(0u, 0u, 0u, 0u);
+        return;
+    }
+    const uint8_t *qb = (const uint8_t *) p.q + ((int64_t) s * p.q_set + (int64_t) t * p.q_tok + 8 * l) * SIZE + sub * (HD * SIZE);
+    const uint8_t *kb = (const uint8_t *) p.k + ((int64_t) s * p.k_set + (int64_t) t * p.k_tok + 8 * l) * SIZE + sub * (HD * SIZE);
+    const uint8_t *vb = (const uint8_t *) p.v + ((int64_t) s * p.v_set + (int64_t) t * p.v_tok + 8 * l) * SIZE + sub * (HD * SIZE);
+    uint32_t raw[STEPS][RAW8<DT>];
+#pragma unroll
+    for (int i = 0; i < STEPS; i++) {
+        const uint32_t hw = hw0 + HPB * i;
+#pragma unroll
+        for (int e = 0; e < RAW8<DT>; e++) raw[i][e] = 0;
+        if (hw < nqw) {
+            if (hw + sub < nq) load_raw<DT, ROT != ROT_ANY>(qb + hw * (HD * SIZE), raw[i]);
+        } else if (hw < nqw + nkw) {
+            if (hw - nqw + sub < p.nkv) load_raw<DT, ROT != ROT_ANY>(kb + (hw - nqw) * (HD * SIZE), raw[i]);
+        } else if (hw < nqw + 2 * nkw) {
+            if (hw - nqw - nkw + sub < p.nkv) load_raw<DT, ROT != ROT_ANY>(vb + (hw - nqw - nkw) * (HD * SIZE), raw[i]);
         }
+    }
+    for (uint32_t i = threadIdx.x; i < 2 * HD; i += 32 * APPEND_WARPS) {
+        const void *w = i < HD ? p.wq : p.wk;
+        wsm[i / HD][i % HD] = !w ? 1.f : p.w32 ? load1<DT_F32>(w, i % HD) : load1<DT>(w, i % HD);
+    }
+    if (threadIdx.x == 32 * APPEND_WARPS - 1) {   // the row of the new key
+        const int64_t key = (int64_t) start + t;
+        int64_t at = -1;
+        const int32_t pg = key >= 0 && key < capacity(p.view)
+                               ? __ldg(p.view.table + (uint64_t) s * p.view.max_pages + (uint32_t) key / p.view.page_keys) : -1;
+        if ((uint32_t) pg < p.view.n_pages) at = ((int64_t) pg * p.view.page_keys + (uint32_t) key % p.view.page_keys) * (int64_t) p.rs;
+        else atomicCAS(p.view.status, ST_OK, ST_BAD_ARGS);
+        s_at = at;
+    }
+    for (uint32_t i = threadIdx.x; i < half; i += 32 * APPEND_WARPS) {
+        const double turn = (double) pos * p.freqs[i] * 0.15915494309189535;   // / (2 pi)
+        float sn, c;
+        sincospif(2.f * (float) (turn - rint(turn)), &sn, &c);
+        cs[i] = make_float2(c, sn);
     }
     __syncthreads();
-    // the row of the new key
-    const int64_t key = (int64_t) start + t;
-    bool stored = pos >= 0;
-    if (stored && (key < 0 || key >= capacity(p.view))) {
-        atomicCAS(p.view.status, ST_OK, ST_BAD_ARGS);
-        stored = false;
-    }
-    uint64_t at = 0;
-    if (stored) {
-        const int32_t pg = __ldg(p.view.table + (uint64_t) s * p.view.max_pages + (uint32_t) key / p.view.page_keys);
-        if ((uint32_t) pg < p.view.n_pages) {
-            at = ((uint64_t) pg * p.view.page_keys + (uint32_t) key % p.view.page_keys) * p.rs;
-        } else {
-            atomicCAS(p.view.status, ST_OK, ST_BAD_ARGS);
-            stored = false;
+    const int64_t at = s_at;
+    // a lane has the same dims of every head: their angles stay in registers, the sine with the partner's sign
+    const bool turns = 8 * l < p.rot, second = 8 * l >= half;
+    uint64_t cc[4], sn[4];
+#pragma unroll
+    for (int e = 0; e < 4; e++) {
+        cc[e] = pack_f2(1.f, 1.f);
+        sn[e] = 0;
+        if (ROT == ROT_PAIRS) {
+            const float2 c = turns && 8 * l + 2 * e < p.rot ? cs[4 * l + e] : make_float2(1.f, 0.f);
+            cc[e] = pack_f2(c.x, c.x);
+            sn[e] = pack_f2(-c.y, c.y);
+        } else if (ROT == ROT_HALVES && turns) {
+            const float2 *c = cs + 8 * l - (second ? half : 0) + 2 * e;
+            cc[e] = pack_f2(c[0].x, c[1].x);
+            sn[e] = second ? pack_f2(c[0].y, c[1].y) : pack_f2(-c[0].y, -c[1].y);
         }
     }
-    for (uint32_t h = h0 + warp; h < h1; h += APPEND_WARPS) {
-        const bool isq = h < nq, isk = !isq && h < nq + p.nkv;
-        if (!isq && !stored) continue;
-        const uint32_t hh = isq ? h : isk ? h - nq : h - nq - p.nkv;
-        const void *src = isq ? p.q : isk ? p.k : p.v;
-        const int64_t off = (int64_t) s * (isq ? p.q_set : isk ? p.k_set : p.v_set) +
-                            (int64_t) t * (isq ? p.q_tok : isk ? p.k_tok : p.v_tok) + (int64_t) hh * HD + E * lane;
-        float x[E];
-        if (isq && pos < 0) {
+    const int from = !turns ? (int) lane : second ? (int) lane - (int) (half / 8) : (int) (lane + half / 8);
+    // norm and rotation of a warp's heads; the norm's factor and the scale are multiplied in at the end
+    auto head = [&](uint64_t (&x)[4], const float *w8, bool norm, float f, float (&v)[8]) {
+        if (norm) {
+            uint64_t s2 = mul_f2(x[0], x[0]);
 #pragma unroll
-            for (int e = 0; e < E; e++) x[e] = 0.f;
-        } else {
-            load_e<DT, E>(src, off, p.vec, x);
+            for (int e = 1; e < 4; e++) s2 = fma_f2(x[e], x[e], s2);
+            float ss, s1;
+            unpack_f2(s2, ss, s1);
+            ss += s1;
+#pragma unroll
+            for (int d = LPH / 2; d > 0; d >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, d);
+            f *= rsqrtf(ss * (1.f / HD) + p.eps);
+            const ulonglong2 w0 = reinterpret_cast<const ulonglong2 *>(w8)[0], w1 = reinterpret_cast<const ulonglong2 *>(w8)[1];
+            x[0] = mul_f2(x[0], w0.x);
+            x[1] = mul_f2(x[1], w0.y);
+            x[2] = mul_f2(x[2], w1.x);
+            x[3] = mul_f2(x[3], w1.y);
         }
-        if ((isq || isk) && pos >= 0) {
-            const void *w = isq ? p.wq : p.wk;
-            if (w) {
-                float ss = 0.f;
+        if constexpr (ROT == ROT_ANY) {
+            float *ln = line[warp] + sub * HD;
+            __syncwarp();
 #pragma unroll
-                for (int e = 0; e < E; e++) ss = fmaf(x[e], x[e], ss);
+            for (int e = 0; e < 4; e++) *reinterpret_cast<uint64_t *>(ln + 8 * l + 2 * e) = x[e];
+            __syncwarp();
+            if (turns) {
+                float y[8];
 #pragma unroll
-                for (int d = 16; d > 0; d >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, d);
-                const float inv = rsqrtf(ss * (1.f / HD) + p.eps);
+                for (int e = 0; e < 8; e++) {
+                    const uint32_t d = 8 * l + e;
+                    const bool odd = p.inter ? e % 2 : d >= half;
+                    const uint32_t a = p.inter ? d / 2 : odd ? d - half : d, b = p.inter ? d ^ 1u : odd ? d - half : d + half;
+                    y[e] = ln[d];
+                    if (d < p.rot) y[e] = y[e] * cs[a].x + (odd ? ln[b] : -ln[b]) * cs[a].y;
+                }
 #pragma unroll
-                for (int e = 0; e < E; e++)
-                    x[e] = x[e] * inv * (p.w32 ? load1<DT_F32>(w, E * lane + e) : load1<DT>(w, E * lane + e));
+                for (int e = 0; e < 4; e++) x[e] = pack_f2(y[2 * e], y[2 * e + 1]);
             }
-            // each dim and its partner meet through the warp's line of shared memory
-            __syncwarp();
+        } else {
+            uint64_t y[4];   // the partners
 #pragma unroll
-            for (int e = 0; e < E; e++) line[warp][E * lane + e] = x[e];
-            __syncwarp();
-#pragma unroll
-            for (int e = 0; e < E; e++) {
-                const uint32_t d = E * lane + e;
-                if (d < p.rot) {
-                    const bool second = p.inter ? d & 1 : d >= half;
-                    const float2 c = cs[p.inter ? d / 2 : second ? d - half : d];
-                    const float y = line[warp][p.inter ? d ^ 1u : second ? d - half : d + half];
-                    x[e] = second ? x[e] * c.x + y * c.y : x[e] * c.x - y * c.y;
+            for (int e = 0; e < 4; e++) {
+                if (ROT == ROT_PAIRS) {
+                    float a, b;
+                    unpack_f2(x[e], a, b);
+                    y[e] = pack_f2(b, a);
+                } else {
+                    y[e] = __shfl_sync(0xffffffffu, (unsigned long long) x[e], from);
                 }
             }
-        }
-        if (isq) {
-            const uint32_t kvh = hh / p.gqa, g = hh % p.gqa;
-            uint16_t *dst = p.Qs + ((((uint64_t) s * p.nkv + kvh) * p.gqa + g) * T + t) * HD + E * lane;
+            if (turns)
 #pragma unroll
-            for (int e = 0; e < E; e += 2) *reinterpret_cast<uint32_t *>(dst + e) = pack_h2(x[e] * p.scale, x[e + 1] * p.scale);
-        } else {
-            store_head<QUANT, E>((isk ? p.K : p.V) + at + hh * p.hb, lane, x);
+                for (int e = 0; e < 4; e++)
+                    if (ROT == ROT_HALVES || 8 * l + 2 * e < p.rot) x[e] = fma_f2(y[e], sn[e], mul_f2(x[e], cc[e]));
+        }
+        const uint64_t f2 = pack_f2(f, f);
+#pragma unroll
+        for (int e = 0; e < 4; e++) unpack_f2(mul_f2(x[e], f2), v[2 * e], v[2 * e + 1]);
+    };
+    // row g * n_tok + t of KV head h / gqa
+    uint16_t *dst = p.Qs + (((uint64_t) s * nq + hw0 + sub) * T + t) * HD + 8 * l;
+    const uint64_t dst_step = (uint64_t) HPB * T * HD;
+#pragma unroll
+    for (int i = 0; i < STEPS; i++) {
+        const uint32_t hw = hw0 + HPB * i;
+        uint64_t x[4];
+        float v[8];
+        unpack8<DT>(raw[i], x);
+        if (hw < nqw) {
+            head(x, wsm[0] + 8 * l, p.wq != nullptr, p.scale, v);
+            if (hw + sub < nq)
+                *reinterpret_cast<uint4 *>(dst) = make_uint4(pack_h2(v[0], v[1]), pack_h2(v[2], v[3]), pack_h2(v[4], v[5]), pack_h2(v[6], v[7]));
+            dst += dst_step;
+        } else if (hw < nqw + nkw) {
+            if (at < 0) continue;
+            head(x, wsm[1] + 8 * l, p.wk != nullptr, 1.f, v);
+            const uint32_t h = hw - nqw + sub;
+            store_head<QUANT>(p.K + at + h * p.hb, l, h < p.nkv, v);
+        } else if (hw < nqw + 2 * nkw) {
+            if (at < 0) continue;
+#pragma unroll
+            for (int e = 0; e < 4; e++) unpack_f2(x[e], v[2 * e], v[2 * e + 1]);
+            const uint32_t h = hw - nqw - nkw + sub;
+            store_head<QUANT>(p.V + at + h * p.hb, l, h < p.nkv, v);
         }
     }
 }
 
 // ---------------------------------------------------------------- reading rows back
-// keys first[s] + t, t < n_tok, of every set as f16 values [n_sets][n_tok][nkv][hd]; one warp per head of a key, K and V
+// keys first[s] + t, t < n_tok, of every set as f16 values [n_sets][n_tok][nkv][hd], K and V. A warp takes a key; a lane gives 8
+// values at a time (a 16-byte store), ROWS_UNROLL of them in flight.
+constexpr int ROWS_UNROLL = 4;
 struct RowsParams {
     View v;
     const int32_t *first;
     const uint8_t *K, *V;
     uint16_t *Ko, *Vo;
     uint64_t rs, hb;
-    uint32_t nkv;
+    uint32_t nkv, n;      // n: keys in all
 };
 template <int HD, int QUANT>
 __global__ void __launch_bounds__(256) rows_kernel(const RowsParams p) {
-    constexpr int E = HD / 32;
-    const uint64_t w = (uint64_t) blockIdx.x * 8 + threadIdx.x / 32;
-    const uint32_t lane = threadIdx.x % 32;
-    const uint64_t n = (uint64_t) p.v.n_sets * p.v.n_tok * p.nkv;
-    if (w >= 2 * n) return;
-    const bool isv = w >= n;
-    const uint64_t i = isv ? w - n : w;
-    const uint32_t h = (uint32_t) (i % p.nkv);
-    const uint64_t tok = i / p.nkv;
-    const uint32_t s = (uint32_t) (tok / p.v.n_tok), t = (uint32_t) (tok % p.v.n_tok);
+    const uint32_t i = blockIdx.x * 8 + threadIdx.x / 32, lane = threadIdx.x % 32;
+    pdl_trigger();
+    pdl_wait();
+    if (i >= p.n) return;
+    const uint32_t s = i / p.v.n_tok, t = i % p.v.n_tok, pieces = p.nkv * (HD / 8);
     const int64_t key = (int64_t) p.first[s] + t;
-    float x[E];
     const int32_t pg = key >= 0 && key < capacity(p.v) ? __ldg(p.v.table + (uint64_t) s * p.v.max_pages + (uint32_t) key / p.v.page_keys) : -1;
-    if ((uint32_t) pg < p.v.n_pages) {
-        const uint8_t *head = (isv ? p.V : p.K) + ((uint64_t) pg * p.v.page_keys + (uint32_t) key % p.v.page_keys) * p.rs + h * p.hb;
+    const bool ok = (uint32_t) pg < p.v.n_pages;
+    if (!ok && lane == 0) atomicCAS(p.v.status, ST_OK, ST_BAD_ARGS);
+    const uint64_t at = ok ? ((uint64_t) pg * p.v.page_keys + (uint32_t) key % p.v.page_keys) * p.rs : 0;
+    for (uint32_t c = lane; c < 2 * pieces; c += 32 * ROWS_UNROLL) {   // K's pieces, then V's
+        uint32_t w[ROWS_UNROLL][4], d[ROWS_UNROLL];
 #pragma unroll
-        for (int e = 0; e < E; e++) x[e] = head_value<QUANT>(head, E * lane + e);
-    } else {
-        atomicCAS(p.v.status, ST_OK, ST_BAD_ARGS);
+        for (int u = 0; u < ROWS_UNROLL; u++) {
+            const uint32_t x = c + 32 * u, y = x < pieces ? x : x - pieces;
+            w[u][0] = w[u][1] = w[u][2] = w[u][3] = d[u] = 0;
+            if (x >= 2 * pieces || !ok) continue;
+            const uint32_t piece = y % (HD / 8);
+            const uint8_t *head = (x < pieces ? p.K : p.V) + at + y / (HD / 8) * p.hb;
+            if (QUANT == 0) {
+                const uint4 r = *reinterpret_cast<const uint4 *>(head + 16 * piece);
+                w[u][0] = r.x; w[u][1] = r.y; w[u][2] = r.z; w[u][3] = r.w;
+            } else {   // blocks start at even bytes: 16-bit loads
+                const uint8_t *blk = head + piece / 4 * dec::q_group_bytes(QUANT);
+                const uint16_t *q = reinterpret_cast<const uint16_t *>(blk + 2 + (QUANT == 1 ? 8 * (piece % 4) : 8 * (piece % 2)));
+                d[u] = *reinterpret_cast<const uint16_t *>(blk);
+                w[u][0] = q[0] | (uint32_t) q[1] << 16;
+                w[u][1] = q[2] | (uint32_t) q[3] << 16;
+            }
+        }
 #pragma unroll
-        for (int e = 0; e < E; e++) x[e] = 0.f;
+        for (int u = 0; u < ROWS_UNROLL; u++) {
+            const uint32_t x = c + 32 * u, y = x < pieces ? x : x - pieces;
+            if (x >= 2 * pieces) continue;
+            uint32_t o[4];
+            if (QUANT == 0) {
+                o[0] = w[u][0]; o[1] = w[u][1]; o[2] = w[u][2]; o[3] = w[u][3];
+            } else {
+                const uint32_t s2 = d[u] | d[u] << 16;
+                if (QUANT == 1) {
+                    dec::q8_word(w[u][0], s2, o[0], o[1]);
+                    dec::q8_word(w[u][1], s2, o[2], o[3]);
+                } else {   // low nibbles: the first 16 elements of the block
+#pragma unroll
+                    for (int j = 0; j < 2; j++) {
+                        const uint32_t n = (w[u][j] >> (y % 4 < 2 ? 0 : 4)) & 0x0F0F0F0Fu;
+                        o[2 * j] = hmul2(hsub2(prmt(n, 0x64646464u, 0x4140u), 0x64086408u), s2);
+                        o[2 * j + 1] = hmul2(hsub2(prmt(n, 0x64646464u, 0x4342u), 0x64086408u), s2);
+                    }
+                }
+            }
+            *reinterpret_cast<uint4 *>((x < pieces ? p.Ko : p.Vo) + ((uint64_t) i * pieces + y) * 8) = make_uint4(o[0], o[1], o[2], o[3]);
+        }
     }
-    uint16_t *dst = (isv ? p.Vo : p.Ko) + i * HD + E * lane;
-#pragma unroll
-    for (int e = 0; e < E; e += 2) *reinterpret_cast<uint32_t *>(dst + e) = pack_h2(x[e], x[e + 1]);
 }
 
 // ---------------------------------------------------------------- row moves
@@ -259,6 +367,8 @@ struct CopyParams {
     int *status;
 };
 __global__ void __launch_bounds__(256) copy_pages_kernel(const CopyParams p) {
+    pdl_trigger();
+    pdl_wait();
     const int32_t a = p.src[blockIdx.y], b = p.dst[blockIdx.y];
     if ((uint32_t) a >= p.n_pages || (uint32_t) b >= p.n_pages) {
         if (threadIdx.x == 0) atomicCAS(p.status, ST_OK, ST_BAD_ARGS);
@@ -294,6 +404,8 @@ struct CompactParams {
 __global__ void __launch_bounds__(128) compact_kernel(const CompactParams p) {
     __shared__ uint32_t from[COMPACT_MAX], to[COMPACT_MAX];
     const uint32_t s = blockIdx.y, T = p.v.n_tok;
+    pdl_trigger();
+    pdl_wait();
     const int start = p.start[s], count = p.count[s];
     bool bad = start < 0 || count < 0 || count > (int) T || (int64_t) start + (int64_t) T > capacity(p.v);
     if (!bad)

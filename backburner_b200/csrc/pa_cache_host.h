@@ -19,6 +19,24 @@ struct DeviceScope {
     DeviceScope &operator=(const DeviceScope &) = delete;
 };
 
+// A launch that may start its prologue while the stream's previous kernel ends (every kernel launched so waits for it with
+// pdl_wait before it reads or writes global memory)
+template <class... A>
+cudaError_t launch_pdl(void (*kernel)(A...), dim3 grid, uint32_t threads, size_t smem, cudaStream_t st, const A &...args) {
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = grid;
+    cfg.blockDim = dim3(threads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = st;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, args...);
+    return e != cudaSuccess ? e : cudaGetLastError();
+}
+
 constexpr uint64_t kCacheMaxKeys = 1ull << 30;   // keys a page table reaches: key indexes and sums of them stay in 32 bits
 
 int check_cache(pa_cuda_ctx *ctx, const pa_cuda_shape *sh, const pa_cuda_cache *c) {
@@ -63,21 +81,17 @@ struct pa_cuda_cache_plan {
 
 namespace {
 
-// Least groups of keys a part takes (16-key groups in the split-K kernel, 64-key groups in the tcgen05 kernel).
-constexpr uint32_t kMinGroups16 = 4, kMinGroups64 = 2;
 constexpr uint32_t kGroups64Overhead = 8;   // what a CTA of the tcgen05 kernel costs besides its groups, in groups
 
 template <int HD, int Q, int W>
 cudaError_t launch_decode_paged(const pa_cuda_cache_plan *p, const pa::dec::PagedParams &prm, cudaStream_t st) {
-    pa::dec::decode_kernel<HD, Q, W, true><<<dim3(p->n_parts, p->d.grid_y), 32 * p->d.n_consumers, p->d.smem, st>>>(prm);
-    return cudaGetLastError();
+    return launch_pdl(pa::dec::decode_kernel<HD, Q, W, true>, dim3(p->n_parts, p->d.grid_y), 32 * p->d.n_consumers, p->d.smem, st, prm);
 }
 template <int Q, int NT, int D>
 cudaError_t launch_prefill_paged(const pa_cuda_cache_plan *p, const CUtensorMap &tq, const pa::pre::PagedParams &prm, cudaStream_t st) {
     constexpr int smem = pa::pre::Smem<Q, NT, D>::TOTAL + 1024;
-    pa::pre::prefill_kernel<Q, NT, D, true>
-        <<<p->n_parts * p->sh.nkv * p->n_rt, 32 * pa::pre::cta_warps(NT), smem, st>>>(tq, prm);
-    return cudaGetLastError();
+    return launch_pdl(pa::pre::prefill_kernel<Q, NT, D, true>, dim3(p->n_parts * p->sh.nkv * p->n_rt), 32 * pa::pre::cta_warps(NT), smem,
+                      st, tq, prm);
 }
 // f(kernel instance's constants) for the plan's kernel; f is a generic lambda
 template <int HD, int W, class F>
@@ -109,10 +123,8 @@ cudaError_t launch_cache_merge(const pa_cuda_cache_plan *p, const pa::mrg::Param
     const uint64_t rows = (uint64_t) mp.n_sets * mp.rows_per_set;
     // 8 warps a row where the rows alone leave SMs idle and a set can have many parts (as launch_merge)
     if (rows * 8 <= (uint64_t) p->ctx->n_sm * 128 && p->n_parts >= 8 * p->n_sets)
-        pa::mrg::merge_kernel<HD, 8, REPLY><<<(unsigned) rows, 256, 0, st>>>(mp);
-    else
-        pa::mrg::merge_kernel<HD, 1, REPLY><<<(unsigned) ((rows + 7) / 8), 256, 0, st>>>(mp);
-    return cudaGetLastError();
+        return launch_pdl(pa::mrg::merge_kernel<HD, 8, REPLY>, dim3((unsigned) rows), 256, 0, st, mp);
+    return launch_pdl(pa::mrg::merge_kernel<HD, 1, REPLY>, dim3((unsigned) ((rows + 7) / 8)), 256, 0, st, mp);
 }
 
 // O, m, l or Oh, lse: one of the two forms
@@ -147,7 +159,6 @@ int cache_attn(pa_cuda_cache_plan *p, uint32_t layer, const uint16_t *Qs, const 
     pg.vr = p->cache.v + layer * layer_bytes(sh, p->cache);
     pg.row0 = layer * p->cache.n_pages * p->cache.page_keys;
     pg.n_parts = p->n_parts;
-    pg.min_groups = p->tc ? kMinGroups64 : kMinGroups16;
     pg.crange = p->d_crange;
     cudaError_t e;
     if (p->tc) {
@@ -266,24 +277,38 @@ int shape_cache_plan(pa_cuda_cache_plan *p) {
     return PA_CUDA_OK;
 }
 
+template <int HD, int DT, int Q, int STEPS, int ROT>
+cudaError_t launch_append_s(const pa::pg::AppendParams &a, cudaStream_t st) {
+    constexpr uint32_t w = 256 / HD, per = pa::pg::append_heads(HD) * STEPS;   // heads of a warp's step, of a block
+    const uint32_t heads = (a.nkv * a.gqa + w - 1) / w * w + 2 * ((a.nkv + w - 1) / w * w);
+    const dim3 grid(a.view.n_tok, a.view.n_sets, (heads + per - 1) / per);
+    return launch_pdl(pa::pg::append_kernel<HD, DT, Q, STEPS, ROT>, grid, 32 * pa::pg::APPEND_WARPS, 0, st, a);
+}
+template <int HD, int DT, int Q>
+cudaError_t launch_append_h(const pa::pg::AppendParams &a, uint32_t steps, int rot, cudaStream_t st) {
+    using namespace pa::pg;
+    if (rot == ROT_ANY) return launch_append_s<HD, DT, Q, 1, ROT_ANY>(a, st);
+    if (steps == 1) return rot == ROT_PAIRS ? launch_append_s<HD, DT, Q, 1, ROT_PAIRS>(a, st) : launch_append_s<HD, DT, Q, 1, ROT_HALVES>(a, st);
+    constexpr int S = DT == DT_F32 ? 4 : 8;   // (8 heads of fp32 do not fit the registers)
+    return rot == ROT_PAIRS ? launch_append_s<HD, DT, Q, S, ROT_PAIRS>(a, st) : launch_append_s<HD, DT, Q, S, ROT_HALVES>(a, st);
+}
 template <int HD, int DT>
-void launch_append_q(const pa::pg::AppendParams &a, uint32_t quant, dim3 grid, uint32_t hpb, cudaStream_t st) {
-    constexpr int threads = 32 * pa::pg::APPEND_WARPS;
-    if (quant == PA_CUDA_Q8_0) pa::pg::append_kernel<HD, DT, 1><<<grid, threads, 0, st>>>(a, hpb);
-    else if (quant == PA_CUDA_Q4_0) pa::pg::append_kernel<HD, DT, 2><<<grid, threads, 0, st>>>(a, hpb);
-    else pa::pg::append_kernel<HD, DT, 0><<<grid, threads, 0, st>>>(a, hpb);
+cudaError_t launch_append_q(const pa::pg::AppendParams &a, uint32_t quant, uint32_t steps, int rot, cudaStream_t st) {
+    return quant == PA_CUDA_Q8_0   ? launch_append_h<HD, DT, 1>(a, steps, rot, st)
+           : quant == PA_CUDA_Q4_0 ? launch_append_h<HD, DT, 2>(a, steps, rot, st)
+                                   : launch_append_h<HD, DT, 0>(a, steps, rot, st);
 }
 template <int HD>
-void launch_append(const pa::pg::AppendParams &a, uint32_t dtype, uint32_t quant, dim3 grid, uint32_t hpb, cudaStream_t st) {
-    if (dtype == PA_CUDA_T_F16) launch_append_q<HD, pa::pg::DT_F16>(a, quant, grid, hpb, st);
-    else if (dtype == PA_CUDA_T_BF16) launch_append_q<HD, pa::pg::DT_BF16>(a, quant, grid, hpb, st);
-    else launch_append_q<HD, pa::pg::DT_F32>(a, quant, grid, hpb, st);
+cudaError_t launch_append(const pa::pg::AppendParams &a, uint32_t dtype, uint32_t quant, uint32_t steps, int rot, cudaStream_t st) {
+    return dtype == PA_CUDA_T_F16    ? launch_append_q<HD, pa::pg::DT_F16>(a, quant, steps, rot, st)
+           : dtype == PA_CUDA_T_BF16 ? launch_append_q<HD, pa::pg::DT_BF16>(a, quant, steps, rot, st)
+                                     : launch_append_q<HD, pa::pg::DT_F32>(a, quant, steps, rot, st);
 }
 template <int HD>
-void launch_rows(const pa::pg::RowsParams &a, uint32_t quant, unsigned blocks, cudaStream_t st) {
-    if (quant == PA_CUDA_Q8_0) pa::pg::rows_kernel<HD, 1><<<blocks, 256, 0, st>>>(a);
-    else if (quant == PA_CUDA_Q4_0) pa::pg::rows_kernel<HD, 2><<<blocks, 256, 0, st>>>(a);
-    else pa::pg::rows_kernel<HD, 0><<<blocks, 256, 0, st>>>(a);
+cudaError_t launch_rows(const pa::pg::RowsParams &a, uint32_t quant, cudaStream_t st) {
+    const dim3 grid((a.n + 7) / 8);
+    return launch_pdl(quant == PA_CUDA_Q8_0 ? pa::pg::rows_kernel<HD, 1> : quant == PA_CUDA_Q4_0 ? pa::pg::rows_kernel<HD, 2> : pa::pg::rows_kernel<HD, 0>,
+                      grid, 256, 0, st, a);
 }
 
 }  // namespace
@@ -420,17 +445,19 @@ int pa_cuda_cache_append(pa_cuda_ctx *ctx, const pa_cuda_shape *shape, const pa_
     a.scale = in->scale;
     a.inter = in->interleaved != 0;
     a.w32 = in->w_dtype == PA_CUDA_T_F32;
-    // a lane's hd / 32 elements in one load where every head starts on such a boundary
-    const uint64_t size = in->dtype == PA_CUDA_T_F32 ? 4 : 2, vec = std::min<uint64_t>(16, shape->hd / 32 * size);
-    uint64_t odd = (uintptr_t) in->q | (uintptr_t) in->k | (uintptr_t) in->v;
-    for (int64_t s : {in->q_set, in->q_tok, in->k_set, in->k_tok, in->v_set, in->v_tok}) odd |= (uint64_t) s * size;
-    a.vec = odd % vec == 0;
-    const uint32_t heads = shape->nkv * (a.gqa + 2), hpb = std::min<uint32_t>(heads, 8);
-    const dim3 grid(n_sets * n_tok, (heads + hpb - 1) / hpb);
-    if (grid.y > 65535) return fail(ctx, PA_CUDA_EUNSUPPORTED, "too many heads");
-    if (shape->hd == 128) launch_append<128>(a, in->dtype, shape->quant, grid, hpb, pick(ctx, stream));
-    else launch_append<256>(a, in->dtype, shape->quant, grid, hpb, pick(ctx, stream));
-    PA_CK(cudaGetLastError(), "append launch");
+    // 16-byte loads where every head and the weights start on such a boundary
+    const uint64_t size = in->dtype == PA_CUDA_T_F32 ? 4 : 2;
+    uint64_t odd = (uintptr_t) in->q | (uintptr_t) in->k | (uintptr_t) in->v | (uintptr_t) in->wq | (uintptr_t) in->wk;
+    for (int64_t x : {in->q_set, in->q_tok, in->k_set, in->k_tok, in->v_set, in->v_tok}) odd |= (uint64_t) x * size;
+    const int rot = odd % 16 ? pa::pg::ROT_ANY : a.inter ? pa::pg::ROT_PAIRS : a.rot % 16 ? pa::pg::ROT_ANY : pa::pg::ROT_HALVES;
+    const uint64_t tokens = (uint64_t) n_sets * n_tok, heads = (uint64_t) shape->nkv * (a.gqa + 2);
+    if (heads > 65535) return fail(ctx, PA_CUDA_EUNSUPPORTED, "too many heads");
+    // steps of a block's warps: one while the blocks that gives run at once (latency), else eight (64 heads at hd 128)
+    const uint64_t per = pa::pg::append_heads((int) shape->hd);
+    const uint32_t steps = tokens * ((heads + per - 1) / per) <= 8ull * ctx->n_sm ? 1 : 8;
+    PA_CK(shape->hd == 128 ? launch_append<128>(a, in->dtype, shape->quant, steps, rot, pick(ctx, stream))
+                           : launch_append<256>(a, in->dtype, shape->quant, steps, rot, pick(ctx, stream)),
+          "append launch");
     ctx->launches++;
     return PA_CUDA_OK;
 }
@@ -445,8 +472,8 @@ int pa_cuda_cache_rows(pa_cuda_ctx *ctx, const pa_cuda_shape *shape, const pa_cu
     if (n_sets == 0 || n_tok == 0) return PA_CUDA_OK;
     if (!table || !first || !K || !V) return fail(ctx, PA_CUDA_EINVAL, "null argument");
     if (((uintptr_t) K | (uintptr_t) V) & 15) return fail(ctx, PA_CUDA_EINVAL, "K and V must be 16-byte aligned");
-    const uint64_t warps = 2ull * n_sets * n_tok * shape->nkv;
-    if ((warps + 7) / 8 > 0x7FFFFFFFull) return fail(ctx, PA_CUDA_EUNSUPPORTED, "too many rows in one call");
+    const uint64_t keys = (uint64_t) n_sets * n_tok;
+    if (keys > 0x7FFFFFFFull) return fail(ctx, PA_CUDA_EUNSUPPORTED, "too many rows in one call");
     DeviceScope dev(ctx->device);
     if (!dev.ok) return fail(ctx, PA_CUDA_ECUDA, "cudaSetDevice");
     pa::pg::RowsParams a{};
@@ -465,10 +492,9 @@ int pa_cuda_cache_rows(pa_cuda_ctx *ctx, const pa_cuda_shape *shape, const pa_cu
     a.rs = shape->rs;
     a.hb = shape->hb;
     a.nkv = shape->nkv;
-    const unsigned blocks = (unsigned) ((warps + 7) / 8);
-    if (shape->hd == 128) launch_rows<128>(a, shape->quant, blocks, pick(ctx, stream));
-    else launch_rows<256>(a, shape->quant, blocks, pick(ctx, stream));
-    PA_CK(cudaGetLastError(), "cache rows launch");
+    a.n = (uint32_t) keys;
+    PA_CK(shape->hd == 128 ? launch_rows<128>(a, shape->quant, pick(ctx, stream)) : launch_rows<256>(a, shape->quant, pick(ctx, stream)),
+          "cache rows launch");
     ctx->launches++;
     return PA_CUDA_OK;
 }
@@ -495,8 +521,7 @@ int pa_cuda_cache_copy_pages(pa_cuda_ctx *ctx, const pa_cuda_shape *shape, const
         a.src = src + i;
         a.dst = dst + i;
         const dim3 grid((unsigned) x, std::min<uint32_t>(65535, n - i), 2 * cache->n_layers);
-        pa::pg::copy_pages_kernel<<<grid, 256, 0, pick(ctx, stream)>>>(a);
-        PA_CK(cudaGetLastError(), "copy pages launch");
+        PA_CK(launch_pdl(pa::pg::copy_pages_kernel, grid, 256, 0, pick(ctx, stream), a), "copy pages launch");
         ctx->launches++;
     }
     return PA_CUDA_OK;
@@ -531,8 +556,7 @@ int pa_cuda_cache_compact(pa_cuda_ctx *ctx, const pa_cuda_shape *shape, const pa
     a.n_layers = cache->n_layers;
     const uint64_t threads = shape->rs / 16 * 2 * cache->n_layers;
     const dim3 grid((unsigned) ((threads + 127) / 128), n_sets);
-    pa::pg::compact_kernel<<<grid, 128, 0, pick(ctx, stream)>>>(a);
-    PA_CK(cudaGetLastError(), "compact launch");
+    PA_CK(launch_pdl(pa::pg::compact_kernel, grid, 128, 0, pick(ctx, stream), a), "compact launch");
     ctx->launches++;
     return PA_CUDA_OK;
 }

@@ -213,6 +213,8 @@ __global__ void __launch_bounds__(32 * W, min_ctas(HD, W)) decode_kernel(const t
     __shared__ pg::Part s_part;   // PAGED: what this CTA works on, and what its tokens see together
     __shared__ pg::Tile s_tile;
     if constexpr (PAGED) {
+        pdl_trigger();
+        pdl_wait();
         if (warp == 0) {
             const pg::Part f = pg::find_part<STAGE_KEYS>(p.pg, blockIdx.x, blockIdx.x == 0 && blockIdx.y == 0, lane);
             const pg::Tile tl = pg::tile_of(p.pg.v, f.st, f.set, 0, p.pg.v.n_tok - 1, lane);
@@ -239,16 +241,21 @@ __global__ void __launch_bounds__(32 * W, min_ctas(HD, W)) decode_kernel(const t
         if constexpr (PAGED) return pgn;
         else return (p.jobs[jn].nk + STAGE_KEYS - 1) / STAGE_KEYS;
     };
+    // PAGED: the pool row of stage `it`
+    auto row_of_stage = [&](uint32_t it) -> uint32_t {
+        if constexpr (PAGED) return pg::row_at(p.pg.v, s_part.set, (uint32_t) span.group((int) (pg0 + it)) * STAGE_KEYS);
+        else return 0u;
+    };
     // stage `it` of job `jn` as stream stage g, into buffer g % NSTAGE: K rows then V rows, one bulk copy per pair of
-    // key rows (warp-collective)
-    auto issue = [&](uint32_t jn, uint32_t it, uint32_t g) {
+    // key rows (warp-collective); PAGED: prow is the stage's pool row
+    auto issue = [&](uint32_t jn, uint32_t it, uint32_t g, uint32_t prow = 0) {
         const uint32_t s = g % NSTAGE;
         Job jb;
         uint32_t valid;
         if constexpr (PAGED) {
             jb.k = p.pg.k;
             jb.v = p.pg.vr;
-            jb.key0 = pg::row_at(p.pg.v, s_part.set, (uint32_t) span.group((int) (pg0 + it)) * STAGE_KEYS) - it * STAGE_KEYS;
+            jb.key0 = prow - it * STAGE_KEYS;
             valid = STAGE_KEYS;
         } else {
             jb = p.jobs[jn];
@@ -280,7 +287,7 @@ __global__ void __launch_bounds__(32 * W, min_ctas(HD, W)) decode_kernel(const t
     };
     // stream stage g + NSTAGE, found from the caller's place in the stream (job jc, which starts at stream stage g0 and
     // has nc stages): later in job jc, or in one of the CTA's next jobs (each has at least one stage)
-    auto issue_ahead = [&](uint32_t jc, uint32_t g0, uint32_t nc, uint32_t g) {
+    auto issue_ahead = [&](uint32_t jc, uint32_t g0, uint32_t nc, uint32_t g, uint32_t prow) {
         uint32_t target = g + NSTAGE - g0, jn = jc, n = nc;
         while (target >= n) {
             target -= n;
@@ -289,7 +296,7 @@ __global__ void __launch_bounds__(32 * W, min_ctas(HD, W)) decode_kernel(const t
             if (jn >= p.n_jobs) return;
             n = stages_of(jn);
         }
-        issue(jn, target, g + NSTAGE);
+        issue(jn, target, g + NSTAGE, prow);
     };
     // after a wait gave up: every copy issued so far lands before the CTA exits (warp 0 waits for them, bounded)
     auto abort_and_drain = [&]() {
@@ -310,7 +317,7 @@ __global__ void __launch_bounds__(32 * W, min_ctas(HD, W)) decode_kernel(const t
     if (warp == 0) {   // the first NSTAGE stream stages
         uint32_t jn = blockIdx.x, it = 0, n = stages_of(jn);
         for (uint32_t g = 0; g < NSTAGE && n > 0; g++) {
-            issue(jn, it, g);
+            issue(jn, it, g, row_of_stage(it));
             if (++it == n) {
                 if constexpr (PAGED) break;
                 it = 0;
@@ -403,6 +410,10 @@ __global__ void __launch_bounds__(32 * W, min_ctas(HD, W)) decode_kernel(const t
 
     for (uint32_t it = 0; it < n_stages; it++, gst++) {
         const uint32_t s = gst % NSTAGE;
+        uint32_t ahead = 0;   // PAGED: the page of the stage that will refill this one, looked up under the tile's work
+        if constexpr (PAGED) {
+            if (it + NSTAGE < n_stages) ahead = row_of_stage(it + NSTAGE);
+        }
         if (!mbar_wait_bounded(&full[s], (gst / NSTAGE) & 1, p.timeout_ns, abort_flag)) { ok = false; break; }
         uint32_t valid = STAGE_KEYS;
         if constexpr (!PAGED) valid = min((uint32_t) STAGE_KEYS, job.nk - it * STAGE_KEYS);
@@ -678,7 +689,7 @@ __global__ void __launch_bounds__(32 * W, min_ctas(HD, W)) decode_kernel(const t
         if (last) {
             __threadfence_block();
             fence_proxy_async();     // ... and before the bulk copies (async proxy) that overwrite it
-            issue_ahead(jc, g0, n_stages, gst);
+            issue_ahead(jc, g0, n_stages, gst, ahead);
         }
     }
     if (!ok) break;

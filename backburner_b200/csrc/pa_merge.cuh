@@ -41,6 +41,8 @@ __global__ void __launch_bounds__(256) merge_kernel(const Params p) {
     __shared__ float s_m[8];
     __shared__ float s_l[8];
     __shared__ __align__(16) float s_acc[SPLIT > 1 ? 8 * HD : 4];
+    pdl_trigger();
+    pdl_wait();   // launched behind the paged attention kernels before they end
     const uint32_t warp = threadIdx.x / 32, lane = threadIdx.x % 32, sw = warp % SPLIT;
     const uint64_t gw = (uint64_t) blockIdx.x * RPB + warp / SPLIT;
     const bool active = gw < (uint64_t) p.n_sets * p.rows_per_set;

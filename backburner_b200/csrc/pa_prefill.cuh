@@ -137,25 +137,7 @@ __device__ __forceinline__ void tmem_st32u(uint32_t taddr, const uint32_t (&v)[3
 }
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
-// fp32 pairs (sm_100 .f32x2 arithmetic) and the three-input max
-__device__ __forceinline__ uint64_t pack_f2(float a, float b) {
-    uint64_t r;
-    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
-    return r;
-}
-__device__ __forceinline__ void unpack_f2(uint64_t x, float &a, float &b) {
-    asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(x));
-}
-__device__ __forceinline__ uint64_t fma_f2(uint64_t a, uint64_t b, uint64_t c) {
-    uint64_t r;
-    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
-    return r;
-}
-__device__ __forceinline__ uint64_t add_f2(uint64_t a, uint64_t b) {
-    uint64_t r;
-    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-    return r;
-}
+// the three-input max
 __device__ __forceinline__ float max3(float a, float b, float c) {
     float r;
     asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
@@ -346,6 +328,8 @@ __global__ void __launch_bounds__(32 * cta_warps(NT), 1) prefill_kernel(const __
     pg::Span span{};
     uint32_t pg0 = 0, pgn = 0;   // PAGED: this CTA's groups [pg0, pg0 + pgn) of its row tile's span
     if constexpr (PAGED) {
+        pdl_trigger();
+        pdl_wait();
         // the tokens of the tile's rows (row r: token r % n_tok): all of them when the rows pass the last token
         const uint32_t T = p.pg.v.n_tok, n = min((uint32_t) (NT * BM), p.rows - row0), a = row0 % T;
         const uint32_t t0 = a + n > T ? 0u : a, t1 = a + n > T ? T - 1 : a + n - 1;
@@ -412,9 +396,15 @@ __global__ void __launch_bounds__(32 * cta_warps(NT), 1) prefill_kernel(const __
             uint32_t issued = 0;
             for (uint32_t j = 0; j < nblk; j++) {
                 const uint32_t st = j % NRS;
-                if (j >= NRS && !wait(&raw_empty[st], ((j / NRS) - 1) & 1)) break;
-                // PAGED: the last block may hold one group fewer
+                // PAGED: the last block may hold one group fewer; the pages are looked up before the wait
                 const uint32_t copies = PAGED ? min((uint32_t) (B / BN), pgn - j * (B / BN)) : (uint32_t) (B / BN);
+                uint32_t prow[B / BN];
+                if constexpr (PAGED) {
+#pragma unroll
+                    for (int c = 0; c < B / BN; c++)
+                        prow[c] = c < (int) copies ? p.pg.row0 + pg::row_at(p.pg.v, job.set, (uint32_t) span.group((int) (pg0 + j * (B / BN)) + c) * BN) : 0u;
+                }
+                if (j >= NRS && !wait(&raw_empty[st], ((j / NRS) - 1) & 1)) break;
                 mbar_arrive_expect_tx(&raw_full[st], 2 * copies * BN * RAWB);
                 uint8_t *dst = smem + L::RAW + st * L::RAW_STAGE;
 #pragma unroll
@@ -422,8 +412,7 @@ __global__ void __launch_bounds__(32 * cta_warps(NT), 1) prefill_kernel(const __
                     int key;
                     if constexpr (PAGED) {
                         if (c >= (int) copies) break;
-                        key = (int) (p.pg.row0 + pg::row_at(p.pg.v, job.set,
-                                                            (uint32_t) span.group((int) (pg0 + j * (B / BN)) + c) * BN));
+                        key = (int) prow[c];
                     } else {
                         key = (int) (job.key0 + j * B) + c * BN;
                     }
@@ -705,88 +694,101 @@ __global__ void __launch_bounds__(32 * cta_warps(NT), 1) prefill_kernel(const __
                     live[c] = gi >= pgn ? 0ull : s_tile.full(k0, 64) ? ~0ull : pg::vis64(s_tile.any, k0);
                 }
             }
+            // Items of the block for this warp: 64-key chunk kc, key half (8 warps) or pass (4 warps), quant block of the
+            // warp; K's, then V's. An item's words are loaded while the one before it is converted (the loads and stores are
+            // ordered among themselves, so without this every item waits out its own shared-memory latency: 64-key blocks of a
+            // 305-row tree over 131,072 Q8_0 keys took 2,500 cycles, 2,100 of them in these warps).
+            constexpr int NI = (B / 64) * (8 / NDQ) * (D / 128);
+            uint32_t W[2][12], S2[2];
+            auto qblk_of = [&](int it) -> uint32_t { return dw % 4 + 4 * (uint32_t) (it / ((8 / NDQ) * (B / 64))); };
+            auto key_of = [&](int it) -> uint32_t {
+                return 64 * (uint32_t) (it / (8 / NDQ) % (B / 64)) + (NDQ == 8 ? dw / 4 : (uint32_t) (it % (8 / NDQ))) * 32 + lane;
+            };
+            auto load = [&](int x, uint32_t (&w)[12], uint32_t &sc2) {
+                const int kv = x / NI, it = x % NI;
+                const uint32_t bo = hoff + GB * qblk_of(it);   // block start inside the raw window row
+                const uint32_t w16 = bo & ~15u;                // 16-byte aligned start of the words covering it
+                const uint32_t rb = raw + kv * B * RAWB + key_of(it) * RAWB;
+                uint32_t s2 = lds16(rb + bo);
+                if constexpr (PAGED) {
+                    if (kv == 1 && !(live[it / (8 / NDQ) % (B / 64)] >> (key_of(it) % 64) & 1ull)) s2 = 0u;
+                }
+                sc2 = s2 | (s2 << 16);
+                // q8_0: the block's 34 bytes lie within 3 aligned 16-byte chunks; q4_0: 18 bytes within 2
 #pragma unroll
-            for (int kv = 0; kv < 2; kv++) {
-                if (j >= KVB && !wait(kv == 0 ? &k_free[b] : &v_free[b], ((j / KVB) - 1) & 1)) break;
-                const uint32_t src = raw + kv * B * RAWB;
-                // items: 64-key chunk kc of the block, key half (8 warps) or pass (4 warps), quant block of the warp
+                for (int i = 0; i < (QUANT == 1 ? 3 : 2); i++) lds128(rb + w16 + 16 * i, w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
+                if (QUANT != 1) w[8] = w[9] = w[10] = w[11] = 0u;
+            };
+            load(0, W[0], S2[0]);
 #pragma unroll
-                for (int it = 0; it < (B / 64) * (8 / NDQ) * (D / 128); it++) {
-                    const int pass = it % (8 / NDQ), kc = it / (8 / NDQ) % (B / 64);
-                    const uint32_t qblk = dw % 4 + 4 * (uint32_t) (it / ((8 / NDQ) * (B / 64)));
-                    const uint32_t bo = hoff + GB * qblk;               // block start inside the raw window row
-                    const uint32_t w16 = bo & ~15u;                     // 16-byte aligned start of the words covering it
-                    const uint32_t ds = bo + 2;                         // first data byte
-                    const uint32_t w0 = (ds - w16) / 4, shift = 8 * (ds % 4);
-                    // atom column of this block's d's
-                    const uint32_t dst = sbase + (kv == 0 ? L::K : L::V) + b * B * D * 2 + (qblk / 2) * B * 128;
-                    const uint32_t key = 64 * (uint32_t) kc + (NDQ == 8 ? dw / 4 : (uint32_t) pass) * 32 + lane;
-                    const uint32_t rb = src + key * RAWB;
-                    uint32_t s2 = lds16(rb + bo);
-                    if constexpr (PAGED) {
-                        if (kv == 1 && !(live[kc] >> (key % 64) & 1ull)) s2 = 0u;
-                    }
-                    const uint32_t sc2 = s2 | (s2 << 16);
-                    uint32_t W[12];
-                    // q8_0: the block's 34 bytes lie within 3 aligned 16-byte chunks; q4_0: 18 bytes within 2
-#pragma unroll
-                    for (int i = 0; i < (QUANT == 1 ? 3 : 2); i++)
-                        lds128(rb + w16 + 16 * i, W[4 * i], W[4 * i + 1], W[4 * i + 2], W[4 * i + 3]);
-                    if (QUANT != 1) W[8] = W[9] = W[10] = W[11] = 0u;
-                    const uint32_t kbase = dst + (key / 8) * 1024 + (key % 8) * 128;
-                    if (QUANT == 1) {
-                        uint32_t A[8];
-                        switch (w0) {   // uniform across the warp
+            for (int x = 0; x < 2 * NI; x++) {
+                const int kv = x / NI, it = x % NI;
+                if (it == 0 && j >= KVB && !wait(kv == 0 ? &k_free[b] : &v_free[b], ((j / KVB) - 1) & 1)) break;
+                if (x + 1 < 2 * NI) {
+                    load(x + 1, W[(x + 1) & 1], S2[(x + 1) & 1]);
+                } else {   // the raw stage is read
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&raw_empty[st]);
+                }
+                const uint32_t (&w)[12] = W[x & 1];
+                const uint32_t sc2 = S2[x & 1], qblk = qblk_of(it), key = key_of(it);
+                const uint32_t bo = hoff + GB * qblk, ds = bo + 2;                       // first data byte
+                const uint32_t w0 = (ds - (bo & ~15u)) / 4, shift = 8 * (ds % 4);
+                // atom column of this block's d's
+                const uint32_t dst = sbase + (kv == 0 ? L::K : L::V) + b * B * D * 2 + (qblk / 2) * B * 128;
+                const uint32_t kbase = dst + (key / 8) * 1024 + (key % 8) * 128;
+                if (QUANT == 1) {
+                    uint32_t A[8];
+                    switch (w0) {   // uniform across the warp
 #define PA_ALIGN8(W0)                                                                        \
     case W0:                                                                                 \
-        _Pragma("unroll") for (int i = 0; i < 8; i++) A[i] = __funnelshift_r(W[W0 + i], W[(W0 + i + 1 < 12) ? W0 + i + 1 : 11], shift); \
+        _Pragma("unroll") for (int i = 0; i < 8; i++) A[i] = __funnelshift_r(w[W0 + i], w[(W0 + i + 1 < 12) ? W0 + i + 1 : 11], shift); \
         break;
-                            PA_ALIGN8(0) PA_ALIGN8(1) PA_ALIGN8(2) PA_ALIGN8(3) default: PA_ALIGN8(4)
+                        PA_ALIGN8(0) PA_ALIGN8(1) PA_ALIGN8(2) PA_ALIGN8(3) default: PA_ALIGN8(4)
 #undef PA_ALIGN8
-                        }
+                    }
 #pragma unroll
-                        for (int cc = 0; cc < 4; cc++) {
-                            uint32_t h0, h1, h2, h3;
-                            dec::q8_word(A[2 * cc], sc2, h0, h1);
-                            dec::q8_word(A[2 * cc + 1], sc2, h2, h3);
-                            const uint32_t c = 4 * (qblk % 2) + cc;
-                            sts128(kbase + ((c ^ (key % 8)) * 16), h0, h1, h2, h3);
-                        }
-                    } else {
-                        uint32_t AW[4];
-                        switch (w0) {
+                    for (int cc = 0; cc < 4; cc++) {
+                        uint32_t h0, h1, h2, h3;
+                        dec::q8_word(A[2 * cc], sc2, h0, h1);
+                        dec::q8_word(A[2 * cc + 1], sc2, h2, h3);
+                        const uint32_t c = 4 * (qblk % 2) + cc;
+                        sts128(kbase + ((c ^ (key % 8)) * 16), h0, h1, h2, h3);
+                    }
+                } else {
+                    uint32_t AW[4];
+                    switch (w0) {
 #define PA_ALIGN4(W0)                                                                        \
     case W0:                                                                                 \
-        _Pragma("unroll") for (int i = 0; i < 4; i++) AW[i] = __funnelshift_r(W[W0 + i], W[W0 + i + 1], shift); \
+        _Pragma("unroll") for (int i = 0; i < 4; i++) AW[i] = __funnelshift_r(w[W0 + i], w[W0 + i + 1], shift); \
         break;
-                            PA_ALIGN4(0) PA_ALIGN4(1) PA_ALIGN4(2) PA_ALIGN4(3) default: PA_ALIGN4(4)
+                        PA_ALIGN4(0) PA_ALIGN4(1) PA_ALIGN4(2) PA_ALIGN4(3) default: PA_ALIGN4(4)
 #undef PA_ALIGN4
-                        }
-                        // byte i: element i (low nibble), element i + 16 (high nibble)
-                        uint32_t lo[8], hi[8];   // f16x2 of elements (2i, 2i+1) and (16+2i, 17+2i)
-                        const uint32_t m = 0x000F000Fu, magic = 0x64006400u, off8 = 0x64086408u;
-#pragma unroll
-                        for (int i = 0; i < 4; i++) {
-                            const uint32_t y = prmt(AW[i], AW[i], 0x3120u);   // bytes (x0, x2, x1, x3)
-                            lo[2 * i] = hmul2(hsub2(and_or(y, m, magic), off8), sc2);
-                            lo[2 * i + 1] = hmul2(hsub2(and_or(y >> 8, m, magic), off8), sc2);
-                            hi[2 * i] = hmul2(hsub2(and_or(y >> 4, m, magic), off8), sc2);
-                            hi[2 * i + 1] = hmul2(hsub2(and_or(y >> 12, m, magic), off8), sc2);
-                        }
-                        const uint32_t c0 = 4 * (qblk % 2);
-                        sts128(kbase + (((c0 + 0) ^ (key % 8)) * 16), lo[0], lo[1], lo[2], lo[3]);
-                        sts128(kbase + (((c0 + 1) ^ (key % 8)) * 16), lo[4], lo[5], lo[6], lo[7]);
-                        sts128(kbase + (((c0 + 2) ^ (key % 8)) * 16), hi[0], hi[1], hi[2], hi[3]);
-                        sts128(kbase + (((c0 + 3) ^ (key % 8)) * 16), hi[4], hi[5], hi[6], hi[7]);
                     }
+                    // byte i: element i (low nibble), element i + 16 (high nibble)
+                    uint32_t lo[8], hi[8];   // f16x2 of elements (2i, 2i+1) and (16+2i, 17+2i)
+                    const uint32_t m = 0x000F000Fu, magic = 0x64006400u, off8 = 0x64086408u;
+#pragma unroll
+                    for (int i = 0; i < 4; i++) {
+                        const uint32_t y = prmt(AW[i], AW[i], 0x3120u);   // bytes (x0, x2, x1, x3)
+                        lo[2 * i] = hmul2(hsub2(and_or(y, m, magic), off8), sc2);
+                        lo[2 * i + 1] = hmul2(hsub2(and_or(y >> 8, m, magic), off8), sc2);
+                        hi[2 * i] = hmul2(hsub2(and_or(y >> 4, m, magic), off8), sc2);
+                        hi[2 * i + 1] = hmul2(hsub2(and_or(y >> 12, m, magic), off8), sc2);
+                    }
+                    const uint32_t c0 = 4 * (qblk % 2);
+                    sts128(kbase + (((c0 + 0) ^ (key % 8)) * 16), lo[0], lo[1], lo[2], lo[3]);
+                    sts128(kbase + (((c0 + 1) ^ (key % 8)) * 16), lo[4], lo[5], lo[6], lo[7]);
+                    sts128(kbase + (((c0 + 2) ^ (key % 8)) * 16), hi[0], hi[1], hi[2], hi[3]);
+                    sts128(kbase + (((c0 + 3) ^ (key % 8)) * 16), hi[4], hi[5], hi[6], hi[7]);
                 }
-                fence_proxy_async();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(kv == 0 ? &k_full[b] : &v_full[b]);
+                if (it + 1 == NI) {
+                    fence_proxy_async();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(kv == 0 ? &k_full[b] : &v_full[b]);
+                }
             }
             if (!ok) break;
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&raw_empty[st]);
         }
     }
 
