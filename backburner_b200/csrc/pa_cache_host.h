@@ -44,7 +44,8 @@ int check_cache(pa_cuda_ctx *ctx, const pa_cuda_shape *sh, const pa_cuda_cache *
     if (rc) return rc;
     if (!c || !c->k || !c->v) return fail(ctx, PA_CUDA_EINVAL, "cache is null");
     if (((uintptr_t) c->k | (uintptr_t) c->v) & 15) return fail(ctx, PA_CUDA_EINVAL, "cache K/V must be 16-byte aligned");
-    if (c->page_keys == 0 || c->page_keys % 64) return fail(ctx, PA_CUDA_EUNSUPPORTED, "page_keys must be a multiple of 64");
+    if (c->page_keys == 0 || c->page_keys % 64 || c->page_keys > (1u << 22))
+        return fail(ctx, PA_CUDA_EUNSUPPORTED, "page_keys must be a multiple of 64, at most 2^22");
     if (c->n_layers == 0 || c->n_pages == 0) return fail(ctx, PA_CUDA_EINVAL, "a cache needs a layer and a page");
     if (c->n_layers > 32767) return fail(ctx, PA_CUDA_EUNSUPPORTED, "more than 32,767 layers");
     // rows of the whole cache are numbered in 31 bits (tensor-map coordinates)
@@ -58,6 +59,7 @@ int check_table(pa_cuda_ctx *ctx, const pa_cuda_cache *c, uint32_t n_sets, uint3
     if (n_sets > 65535) return fail(ctx, PA_CUDA_EUNSUPPORTED, "more than 65,535 sequences");
     return PA_CUDA_OK;
 }
+uint64_t page_mul(uint32_t page_keys) { return ((1ull << 40) + page_keys / 64 - 1) / (page_keys / 64); }
 uint64_t layer_bytes(const pa_cuda_shape &sh, const pa_cuda_cache &c) { return (uint64_t) c.n_pages * c.page_keys * sh.rs; }
 
 }  // namespace
@@ -71,11 +73,11 @@ struct pa_cuda_cache_plan {
     pa_cuda_plan d;                  // launch shape of the split-K kernel
     bool tc = false;                 // the tcgen05 kernel
     int nt = 1;                      // ... with nt tiles of 128 rows per CTA, n_rt groups of them per head
-    uint32_t n_rt = 1;
+    uint32_t n_rt = 1, unit_rows = 1;   // units of a set (row tiles; the split-K kernel: one) and their rows
     uint32_t n_parts = 1;            // CTAs along the keys = slots of partials (pa_mask.cuh)
     CUtensorMap *d_maps = nullptr;   // K and V rows of the whole cache
-    float *d_part = nullptr;         // O [slot][nkv][rows][hd], then m, then l
-    uint32_t *d_crange = nullptr;    // [n_sets + 1]: slots of each set, written by every call
+    float *d_part = nullptr;         // O [slot][nkv][unit_rows][hd], then m, then l
+    uint32_t *d_crange = nullptr;    // [units + 1]: slots of each unit, written by every call
     const char *kernel = "";
 };
 
@@ -90,7 +92,7 @@ cudaError_t launch_decode_paged(const pa_cuda_cache_plan *p, const pa::dec::Page
 template <int Q, int NT, int D>
 cudaError_t launch_prefill_paged(const pa_cuda_cache_plan *p, const CUtensorMap &tq, const pa::pre::PagedParams &prm, cudaStream_t st) {
     constexpr int smem = pa::pre::Smem<Q, NT, D>::TOTAL + 1024;
-    return launch_pdl(pa::pre::prefill_kernel<Q, NT, D, true>, dim3(p->n_parts * p->sh.nkv * p->n_rt), 32 * pa::pre::cta_warps(NT), smem,
+    return launch_pdl(pa::pre::prefill_kernel<Q, NT, D, true>, dim3(p->n_parts * p->sh.nkv), 32 * pa::pre::cta_warps(NT), smem,
                       st, tq, prm);
 }
 // f(kernel instance's constants) for the plan's kernel; f is a generic lambda
@@ -123,8 +125,8 @@ cudaError_t launch_cache_merge(const pa_cuda_cache_plan *p, const pa::mrg::Param
     const uint64_t rows = (uint64_t) mp.n_sets * mp.rows_per_set;
     // 8 warps a row where the rows alone leave SMs idle and a set can have many parts (as launch_merge)
     if (rows * 8 <= (uint64_t) p->ctx->n_sm * 128 && p->n_parts >= 8 * p->n_sets)
-        return launch_pdl(pa::mrg::merge_kernel<HD, 8, REPLY>, dim3((unsigned) rows), 256, 0, st, mp);
-    return launch_pdl(pa::mrg::merge_kernel<HD, 1, REPLY>, dim3((unsigned) ((rows + 7) / 8)), 256, 0, st, mp);
+        return launch_pdl(pa::mrg::merge_kernel<HD, 8, true, REPLY>, dim3((unsigned) rows), 256, 0, st, mp);
+    return launch_pdl(pa::mrg::merge_kernel<HD, 1, true, REPLY>, dim3((unsigned) ((rows + 7) / 8)), 256, 0, st, mp);
 }
 
 // O, m, l or Oh, lse: one of the two forms
@@ -140,8 +142,8 @@ int cache_attn(pa_cuda_cache_plan *p, uint32_t layer, const uint16_t *Qs, const 
     if (!dev.ok) return fail(ctx, PA_CUDA_ECUDA, "cudaSetDevice");
     cudaStream_t st = pick(ctx, stream);
     const pa_cuda_shape &sh = p->sh;
-    const uint64_t rows_all = (uint64_t) sh.nkv * sh.rows;
-    float *Op = p->d_part, *Mp = Op + p->n_parts * rows_all * sh.hd, *Lp = Mp + p->n_parts * rows_all;
+    const uint64_t rows_all = (uint64_t) sh.nkv * sh.rows, slot_rows = (uint64_t) sh.nkv * p->unit_rows;
+    float *Op = p->d_part, *Mp = Op + p->n_parts * slot_rows * sh.hd, *Lp = Mp + p->n_parts * slot_rows;
     pa::pg::Paged pg{};
     pg.v.table = table;
     pg.v.n_keys = n_keys;
@@ -151,6 +153,7 @@ int cache_attn(pa_cuda_cache_plan *p, uint32_t layer, const uint16_t *Qs, const 
     pg.v.max_pages = p->max_pages;
     pg.v.n_pages = p->cache.n_pages;
     pg.v.page_keys = p->cache.page_keys;
+    pg.v.page_mul = page_mul(p->cache.page_keys);
     pg.v.n_tok = p->mask.n_tok;
     pg.v.window = p->mask.window;
     pg.v.sinks = p->mask.sinks;
@@ -159,6 +162,10 @@ int cache_attn(pa_cuda_cache_plan *p, uint32_t layer, const uint16_t *Qs, const 
     pg.vr = p->cache.v + layer * layer_bytes(sh, p->cache);
     pg.row0 = layer * p->cache.n_pages * p->cache.page_keys;
     pg.n_parts = p->n_parts;
+    pg.rows = sh.rows;
+    pg.tile_rows = p->unit_rows;
+    pg.half_rows = p->tc && p->nt == 2 ? (uint32_t) pa::pre::BM : 0u;
+    pg.n_rt = p->n_rt;
     pg.crange = p->d_crange;
     cudaError_t e;
     if (p->tc) {
@@ -176,7 +183,7 @@ int cache_attn(pa_cuda_cache_plan *p, uint32_t layer, const uint16_t *Qs, const 
         prm.hb = sh.hb;
         prm.nkv = sh.nkv;
         prm.rows = sh.rows;
-        prm.n_rt = p->n_rt;
+        prm.n_rt = 1;
         prm.timeout_ns = ctx->timeout_ns;
         prm.stall = ctx->stall_test;
         e = with_prefill(p, [&](auto q, auto nt, auto d) { return launch_prefill_paged<q.value, nt.value, d.value>(p, tq, prm, st); });
@@ -210,8 +217,11 @@ int cache_attn(pa_cuda_cache_plan *p, uint32_t layer, const uint16_t *Qs, const 
     mp.Lp = Lp;
     mp.c_range = p->d_crange;
     mp.n_parts = p->n_parts;
-    mp.op_stride = rows_all * sh.hd;
-    mp.ml_stride = rows_all;
+    mp.op_stride = slot_rows * sh.hd;
+    mp.ml_stride = slot_rows;
+    mp.rows = sh.rows;
+    mp.unit_rows = p->unit_rows;
+    mp.n_rt = p->n_rt;
     mp.O = O;
     mp.M = m;
     mp.L = l;
@@ -244,22 +254,27 @@ int shape_cache_plan(pa_cuda_cache_plan *p) {
     uint64_t groups = cap / G;
     if (p->mask.window)
         groups = std::min(groups, ((uint64_t) p->mask.window + p->mask.n_tok + G - 1) / G + 1 + std::min<uint64_t>((p->mask.sinks + (uint64_t) G - 1) / G, groups));
-    const uint64_t spare = p->n_sets > 1 ? p->n_sets : 0;   // find_part: parts lost to the sets' remainders
-    uint64_t parts;
+    uint64_t parts, units;
     if (p->tc) {
         p->nt = sh.hd == 128 && sh.rows > (uint32_t) pa::pre::BM ? 2 : 1;
-        p->n_rt = (sh.rows + pa::pre::BM * p->nt - 1) / (pa::pre::BM * p->nt);
+        p->unit_rows = (uint32_t) (pa::pre::BM * p->nt);
+        p->n_rt = (sh.rows + p->unit_rows - 1) / p->unit_rows;
+        units = (uint64_t) p->n_sets * p->n_rt;
         p->kernel = p->nt == 2 ? "pa::pre::prefill_kernel<2 tiles, paged>" : "pa::pre::prefill_kernel<1 tile, paged>";
-        // the count that minimises waves x (groups of a part + a CTA's overhead), the sets as long as they can be
-        const uint64_t y = (uint64_t) sh.nkv * p->n_rt;
+        // the count that minimises waves x (groups of a part + a CTA's overhead), all units as long as they can be; parts
+        // that are left over by equal units' remainders are counted out
+        const uint64_t spare = units > 1 ? units : 0;
         uint64_t best = ~0ull;
-        parts = spare + 1;
-        for (uint64_t c = spare + 1; c <= spare + std::max<uint64_t>(1, 8ull * ctx->n_sm / y); c++) {
-            const uint64_t per = (groups * p->n_sets + (c - spare) - 1) / (c - spare);
-            const uint64_t cost = ((c * y + ctx->n_sm - 1) / ctx->n_sm) * (per + kGroups64Overhead);
+        parts = units;
+        for (uint64_t c = std::max<uint64_t>(1, units); c <= spare + std::max<uint64_t>(1, 8ull * ctx->n_sm / sh.nkv); c++) {
+            const uint64_t per = (groups + c / units - 1) / (c / units);
+            const uint64_t cost = ((c / units * units * sh.nkv + ctx->n_sm - 1) / ctx->n_sm) * (per + kGroups64Overhead);
             if (cost < best) { best = cost; parts = c; }
         }
-        if (parts * y > 0x7FFFFFFFull) return fail(ctx, PA_CUDA_EUNSUPPORTED, "too many rows and sets in one call");
+        // as many as the waves hold anyway (units differ in length)
+        const uint64_t waves = (parts * sh.nkv + ctx->n_sm - 1) / ctx->n_sm;
+        parts = std::max(parts, waves * ctx->n_sm / sh.nkv);
+        if (2 * units * sh.nkv + parts * sh.nkv > 0x7FFFFFFFull) return fail(ctx, PA_CUDA_EUNSUPPORTED, "too many rows and sets in one call");
     } else {
         if (p->d.grid_y > 65535) return fail(ctx, PA_CUDA_EUNSUPPORTED, "too many head/row groups");
         p->kernel = "pa::dec::decode_kernel<paged>";
@@ -270,10 +285,12 @@ int shape_cache_plan(pa_cuda_cache_plan *p) {
             return cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, k, 32 * (int) p->d.n_consumers, p->d.smem);
         });
         // as many CTAs as run at once
-        parts = std::max<uint64_t>(spare + 1, (uint64_t) ctx->n_sm * std::max(1, per_sm) / p->d.grid_y);
+        parts = std::max<uint64_t>(1, (uint64_t) ctx->n_sm * std::max(1, per_sm) / p->d.grid_y);
+        units = p->n_sets;
+        p->unit_rows = sh.rows;
     }
-    parts = std::min(parts, spare + p->n_sets * std::max<uint64_t>(1, groups));
-    p->n_parts = (uint32_t) std::max<uint64_t>(parts, 2 * spare);
+    parts = std::min(parts, units * std::max<uint64_t>(1, groups));
+    p->n_parts = (uint32_t) (units > 1 ? std::max(parts, units + 1) : parts);   // find_part: one more than the units
     return PA_CUDA_OK;
 }
 
@@ -343,9 +360,8 @@ int pa_cuda_cache_plan_create(pa_cuda_ctx *ctx, const pa_cuda_shape *shape, cons
         delete p;
         return rc;
     }
-    const uint64_t rows_all = (uint64_t) shape->nkv * shape->rows;
-    cudaError_t e = cudaMalloc((void **) &p->d_part, p->n_parts * rows_all * (shape->hd + 2) * sizeof(float));
-    if (e == cudaSuccess) e = cudaMalloc((void **) &p->d_crange, (n_sets + 1) * sizeof(uint32_t));
+    cudaError_t e = cudaMalloc((void **) &p->d_part, (uint64_t) p->n_parts * shape->nkv * p->unit_rows * (shape->hd + 2) * sizeof(float));
+    if (e == cudaSuccess) e = cudaMalloc((void **) &p->d_crange, ((uint64_t) n_sets * p->n_rt + 1) * sizeof(uint32_t));
     if (e == cudaSuccess && p->tc) {
         const uint32_t rows = cache->n_layers * cache->n_pages * cache->page_keys;
         const uint32_t raw = (uint32_t) pa::pre::raw_row_bytes((int) shape->quant, (int) shape->hd);
@@ -431,6 +447,7 @@ int pa_cuda_cache_append(pa_cuda_ctx *ctx, const pa_cuda_shape *shape, const pa_
     a.view.max_pages = max_pages;
     a.view.n_pages = cache->n_pages;
     a.view.page_keys = cache->page_keys;
+    a.view.page_mul = page_mul(cache->page_keys);
     a.view.n_tok = n_tok;
     a.view.status = ctx->d_status;
     a.K = cache->k + layer * layer_bytes(*shape, *cache);
@@ -482,6 +499,7 @@ int pa_cuda_cache_rows(pa_cuda_ctx *ctx, const pa_cuda_shape *shape, const pa_cu
     a.v.max_pages = max_pages;
     a.v.n_pages = cache->n_pages;
     a.v.page_keys = cache->page_keys;
+    a.v.page_mul = page_mul(cache->page_keys);
     a.v.n_tok = n_tok;
     a.v.status = ctx->d_status;
     a.first = first;
@@ -544,6 +562,7 @@ int pa_cuda_cache_compact(pa_cuda_ctx *ctx, const pa_cuda_shape *shape, const pa
     a.v.max_pages = max_pages;
     a.v.n_pages = cache->n_pages;
     a.v.page_keys = cache->page_keys;
+    a.v.page_mul = page_mul(cache->page_keys);
     a.v.n_tok = n_tok;
     a.v.status = ctx->d_status;
     a.K = cache->k;

@@ -217,7 +217,7 @@ __global__ void __launch_bounds__(32 * W, min_ctas(HD, W)) decode_kernel(const t
         pdl_wait();
         if (warp == 0) {
             const pg::Part f = pg::find_part<STAGE_KEYS>(p.pg, blockIdx.x, blockIdx.x == 0 && blockIdx.y == 0, lane);
-            const pg::Tile tl = pg::tile_of(p.pg.v, f.st, f.set, 0, p.pg.v.n_tok - 1, lane);
+            const pg::Tile tl = pg::tile_of(p.pg.v, f.st, f.set, f.t0, f.t1, lane);
             if (lane == 0) {
                 s_part = f;
                 s_tile = tl;
@@ -231,10 +231,9 @@ __global__ void __launch_bounds__(32 * W, min_ctas(HD, W)) decode_kernel(const t
     uint32_t pg0 = 0, pgn = 0;
     if constexpr (PAGED) {
         if (s_part.of == 0) return;
-        span = pg::span_of<STAGE_KEYS>(p.pg.v, s_part.st, 0, p.pg.v.n_tok - 1);
-        const uint32_t per = ((uint32_t) span.n + s_part.of - 1) / s_part.of;
-        pg0 = min(s_part.index * per, (uint32_t) span.n);
-        pgn = min(per, (uint32_t) span.n - pg0);
+        span = pg::span_of<STAGE_KEYS>(p.pg.v, s_part.st, s_part.t0, s_part.t1);
+        pg0 = s_part.begin((uint32_t) span.n);
+        pgn = s_part.end((uint32_t) span.n) - pg0;
     }
 
     auto stages_of = [&](uint32_t jn) -> uint32_t {

@@ -15,7 +15,11 @@ struct View {
     const int32_t *table, *n_keys, *q_pos;   // [n_sets][max_pages], [n_sets], [n_sets] or null
     const uint64_t *tree;                    // [n_sets][n_tok] or null
     uint32_t n_sets, max_pages, n_pages, page_keys, n_tok, window, sinks;
+    uint64_t page_mul;                       // ceil(2^40 / (page_keys / 64))
     int *status;
+    // the page of a key: (key / 64) / (page_keys / 64) by a product, exact for keys below 2^30 and pages of up to 2^22 keys
+    // (quotient g * m / 2^40 with m <= 2^40 / d + 1: too large by at most g / 2^40 < 2^-16 <= 1 / d, so never by a whole)
+    __host__ __device__ __forceinline__ uint32_t page_index(uint32_t key) const { return (uint32_t) ((uint64_t) (key >> 6) * page_mul >> 40); }
 };
 struct Set {
     int nk, q0;   // keys held, clamped to the table's reach; key of token 0 (may be negative or past nk)
@@ -30,7 +34,7 @@ struct Row {
 PA_HD int capacity(const View &v) { return (int) (v.max_pages * v.page_keys); }   // <= 2^30
 PA_HD int clampi(int64_t x, int lo, int hi) { return x < lo ? lo : x > hi ? hi : (int) x; }
 // the low n bits
-PA_HD uint64_t low_bits(int64_t n) { return n <= 0 ? 0ull : n >= 64 ? ~0ull : (1ull << n) - 1; }
+PA_HD uint64_t low_bits(int n) { return n <= 0 ? 0ull : n >= 64 ? ~0ull : ~(~0ull << n); }
 
 __device__ __forceinline__ Set set_of(const View &v, uint32_t s) {
     const int n = v.n_keys[s];
@@ -51,23 +55,38 @@ PA_HD Row row_from(const View &v, Set st, int64_t at, int hi, uint64_t bits) {
     r.hi = hi;
     r.lo = v.window ? clampi(at - (int64_t) v.window + 1, 0, hi) : 0;
     r.sink = sink_end(v, hi);
-    r.q0 = st.q0;
-    r.bits = bits & low_bits((int64_t) st.nk - st.q0) & ~low_bits(-(int64_t) st.q0);   // drafted keys that exist
+    // drafted keys that exist; none does where q0 is 64 or more before key 0 or behind the keys, so that q0 fits 31 bits
+    r.q0 = clampi(st.q0, -64, 1 << 30);
+    r.bits = bits & low_bits(st.nk - r.q0) & ~low_bits(-r.q0);
     return r;
 }
 PA_HD Row row_of(const View &v, Set st, uint32_t s, uint32_t t) {
     if (!v.tree) return row_from(v, st, (int64_t) st.q0 + t, clampi((int64_t) st.q0 + t + 1, 0, st.nk), 0);
     const uint64_t b = v.tree[(uint64_t) s * v.n_tok + t] & low_bits(v.n_tok);
-    if (!b) return Row{0, 0, 0, st.q0, 0};
+    if (!b) return Row{0, 0, 0, 0, 0};
     return row_from(v, st, (int64_t) st.q0 + bit_count(b) - 1, clampi(st.q0, 0, st.nk), b);
 }
-// bit i: the row sees key k0 + i
-PA_HD uint64_t vis64(const Row &r, int k0) {
-    uint64_t m = (low_bits((int64_t) r.hi - k0) & ~low_bits((int64_t) r.lo - k0)) | low_bits((int64_t) r.sink - k0);
-    const int64_t d = (int64_t) r.q0 - k0;
-    if (d >= 0) m |= d < 64 ? r.bits << d : 0;
-    else m |= d > -64 ? r.bits >> -d : 0;
+// bits [0, n) of 32
+PA_HD uint32_t low32(int n) {
+#ifdef __CUDA_ARCH__
+    uint32_t m;
+    asm("bmsk.clamp.b32 %0, 0, %1;" : "=r"(m) : "r"(n > 0 ? n : 0));
     return m;
+#else
+    return (uint32_t) low_bits(n < 32 ? n : 32);
+#endif
+}
+// bit i: the row sees key k0 + i (in halves, which is short code: it stands in loops that have to stay in the instruction cache)
+PA_HD uint64_t vis64(const Row &r, int k0) {
+    uint32_t m[2];
+    for (int h = 0; h < 2; h++) {
+        const int k = k0 + 32 * h;
+        m[h] = (low32(r.hi - k) & ~low32(r.lo - k)) | low32(r.sink - k);
+    }
+    const int d = r.q0 - k0;
+    uint64_t drafts = 0;
+    if (d > -64 && d < 64) drafts = d >= 0 ? r.bits << d : r.bits >> -d;
+    return (((uint64_t) m[1] << 32) | m[0]) | drafts;
 }
 
 // The groups of G keys that tokens [t0, t1] of a set see together: the sinks' groups 0 .. a-1, then groups b, b+1, ...
@@ -88,65 +107,98 @@ PA_HD Span span_of(const View &v, Set st, uint32_t t0, uint32_t t1) {
     return p;
 }
 
-// the page of the 64-key group that holds key `key` (a page id outside the pool is reported and replaced by page 0)
-__device__ __forceinline__ uint32_t page_of(const View &v, uint32_t s, uint32_t key) {
-    const int32_t p = __ldg(v.table + (uint64_t) s * v.max_pages + key / v.page_keys);
+// page `index` of a set (a page id outside the pool is reported and replaced by page 0)
+__device__ __forceinline__ uint32_t page_of(const View &v, uint32_t s, uint32_t index) {
+    const int32_t p = __ldg(v.table + (uint64_t) s * v.max_pages + index);
     if ((uint32_t) p < v.n_pages) return (uint32_t) p;
     atomicCAS(v.status, ST_OK, ST_BAD_ARGS);
     return 0;
 }
 // row of the pool (within a layer) that holds key `key`
 __device__ __forceinline__ uint32_t row_at(const View &v, uint32_t s, uint32_t key) {
-    return page_of(v, s, key) * v.page_keys + key % v.page_keys;
+    const uint32_t i = v.page_index(key);
+    return page_of(v, s, i) * v.page_keys + (key - i * v.page_keys);
 }
 
 // ---------------------------------------------------------------- parts
-// The CTAs of a launch along the keys ("parts") are dealt out over the sets in proportion to the groups each has to read,
-// on the device, since the lengths are only known there: `per` groups a part, so that all sets fit n_parts. (One group a
-// part where the groups are few: 777 keys, window 512, us a call: 1 group 14.4, 4 groups 18.5, 8 groups 22.6.) Part c of the
-// launch is also the slot its partial goes to; crange [n_sets + 1] (what the merge reads) gets the parts of every set.
+// The work of a launch is its units, a set's row tiles (tile_rows rows of a head each; the split-K kernel's unit is the whole
+// set), each over the groups of keys its own tokens see. The CTAs along the keys ("parts") are dealt out over the units in
+// proportion to their cost, on the device, since the lengths are only known there: the least `per` for which all units fit
+// n_parts, by bisection. A part takes at least sqrt(groups of a unit) / 4 groups: with fewer, the merge of more parts costs
+// what the shorter parts gain (split-K kernel, us a call: 777 keys, window 512: 1 group a part 14.4, 4 groups 18.5; 4,096
+// keys: 1 group 24.0, 4 groups 18.5). Part c of the launch is also the slot its partial goes to, rows of one unit;
+// crange [units + 1] (what the merge reads) gets the parts of every unit.
 struct Paged {
     View v;
     const uint8_t *k, *vr;     // the layer's rows
     uint32_t row0;             // the layer's first row in the cache's tensor maps
     uint32_t n_parts;
+    uint32_t rows, tile_rows;  // query rows per head, and of a unit
+    uint32_t half_rows;        // a unit with at most so many rows leaves one of the kernel's two row tiles out
+    uint32_t n_rt;             // row tiles of a set
     uint32_t *crange;
 };
-// what a CTA works on (in shared memory)
+// a unit's part: what a CTA works on
 struct Part {
-    uint32_t set, index, of;   // part `index` of the set's `of` (0: none for this CTA)
+    uint32_t set, rt;          // the unit
+    uint32_t index, of;        // part `index` of the unit's `of` (0: none for this CTA)
+    uint32_t t0, t1;           // tokens of the unit's rows
     Set st;
+    // the part's groups of the unit's n (n >= of: at least one)
+    PA_HD uint32_t begin(uint32_t n) const { return (uint32_t) ((uint64_t) index * n / of); }
+    PA_HD uint32_t end(uint32_t n) const { return (uint32_t) ((uint64_t) (index + 1) * n / of); }
 };
-// warp-collective; every lane gets the result
+// the tokens of row tile rt (row r: token r % n_tok): all of them when its rows pass the last token
+PA_HD void tokens_of(const Paged &p, uint32_t rt, uint32_t &t0, uint32_t &t1) {
+    const uint32_t T = p.v.n_tok, r0 = rt * p.tile_rows, n = p.rows - r0 < p.tile_rows ? p.rows - r0 : p.tile_rows, a = r0 % T;
+    t0 = a + n > T ? 0u : a;
+    t1 = a + n > T ? T - 1 : a + n - 1;
+}
+// warp-collective; every lane gets the result. G keys a group; a group of a unit with one row tile costs 7/8 of one with two.
 template <int G>
 __device__ __forceinline__ Part find_part(const Paged &p, uint32_t c, bool write, uint32_t lane) {
     const View &v = p.v;
-    Part r{0, 0, 0, {0, 0}};
-    if (v.n_sets == 1) {
-        const Set st = set_of(v, 0);
-        const uint32_t n = (uint32_t) span_of<G>(v, st, 0, v.n_tok - 1).n;
-        const uint32_t per = max(1u, (n + p.n_parts - 1) / p.n_parts), cnt = (n + per - 1) / per;
-        if (write && lane < 2) p.crange[lane] = lane ? cnt : 0u;
-        if (c < cnt) r = Part{0, c, cnt, st};
-        return r;
-    }
+    const uint32_t units = v.n_sets * p.n_rt;
+    // unit u, and the cost of its groups
+    auto unit = [&](uint32_t u, Part &r) -> uint32_t {
+        r.set = u / p.n_rt;
+        r.rt = u - r.set * p.n_rt;
+        tokens_of(p, r.rt, r.t0, r.t1);
+        r.st = set_of(v, r.set);
+        return (uint32_t) span_of<G>(v, r.st, r.t0, r.t1).n * (p.rows - r.rt * p.tile_rows <= p.half_rows ? 7u : 8u);
+    };
+    Part mine{};                       // the lane's unit of the last round (the only one with up to 32 units)
+    uint32_t cost = 0;
     uint64_t total = 0;
-    for (uint32_t s = lane; s < v.n_sets; s += 32) total += (uint32_t) span_of<G>(v, set_of(v, s), 0, v.n_tok - 1).n;
+    for (uint32_t u = lane; u < units; u += 32) total += cost = unit(u, mine);
 #pragma unroll
     for (int x = 16; x > 0; x >>= 1) total += __shfl_xor_sync(0xffffffffu, total, x);
-    // sum of ceil(n_s / per) < total / per + n_sets <= n_parts (n_parts > n_sets, by the plan)
-    const uint64_t room = p.n_parts - v.n_sets;
-    const uint32_t per = max(1u, (uint32_t) ((total + room - 1) / room));
+    const uint32_t least = max(1u, (uint32_t) sqrtf((float) total / (float) (8 * units)) / 4) * 8;
+    uint32_t lo = max(least, (uint32_t) ((total + p.n_parts - 1) / p.n_parts)), hi = lo;
+    if (units > 1) {
+        // sum of ceil(cost / per) < total / per + units <= n_parts at hi (n_parts > units, by the plan)
+        hi = max(lo, (uint32_t) ((total + (p.n_parts - units) - 1) / (p.n_parts - units)));
+        while (lo < hi) {
+            const uint32_t mid = lo + (hi - lo) / 2;
+            uint32_t need = 0;
+            if (units <= 32) {
+                need = (cost + mid - 1) / mid;
+            } else {
+                Part r;
+                for (uint32_t u = lane; u < units; u += 32) need += (unit(u, r) + mid - 1) / mid;
+            }
+            need = __reduce_add_sync(0xffffffffu, need);
+            if (need <= p.n_parts) hi = mid;
+            else lo = mid + 1;
+        }
+    }
+    Part r{};
     uint32_t base = 0;
     if (write && lane == 0) p.crange[0] = 0;
-    for (uint32_t s0 = 0; s0 < v.n_sets; s0 += 32) {
-        const uint32_t s = s0 + lane;
-        Set st{0, 0};
-        uint32_t cnt = 0;
-        if (s < v.n_sets) {
-            st = set_of(v, s);
-            cnt = ((uint32_t) span_of<G>(v, st, 0, v.n_tok - 1).n + per - 1) / per;
-        }
+    for (uint32_t u0 = 0; u0 < units; u0 += 32) {
+        const uint32_t u = u0 + lane;
+        if (units > 32) cost = u < units ? unit(u, mine) : 0;
+        const uint32_t cnt = u < units ? (cost + hi - 1) / hi : 0;
         uint32_t end = cnt;
 #pragma unroll
         for (int x = 1; x < 32; x <<= 1) {
@@ -154,15 +206,18 @@ __device__ __forceinline__ Part find_part(const Paged &p, uint32_t c, bool write
             if (lane >= (uint32_t) x) end += y;
         }
         end += base;
-        if (write && s < v.n_sets) p.crange[s + 1] = end;
+        if (write && u < units) p.crange[u + 1] = end;
         const uint32_t hit = __ballot_sync(0xffffffffu, c < end && c >= end - cnt);
         if (hit) {
             const int src = __ffs((int) hit) - 1;
-            r.set = s0 + (uint32_t) src;
+            r.set = __shfl_sync(0xffffffffu, mine.set, src);
+            r.rt = __shfl_sync(0xffffffffu, mine.rt, src);
+            r.t0 = __shfl_sync(0xffffffffu, mine.t0, src);
+            r.t1 = __shfl_sync(0xffffffffu, mine.t1, src);
             r.of = __shfl_sync(0xffffffffu, cnt, src);
             r.index = c - (__shfl_sync(0xffffffffu, end, src) - r.of);
-            r.st.nk = __shfl_sync(0xffffffffu, st.nk, src);
-            r.st.q0 = __shfl_sync(0xffffffffu, st.q0, src);
+            r.st.nk = __shfl_sync(0xffffffffu, mine.st.nk, src);
+            r.st.q0 = __shfl_sync(0xffffffffu, mine.st.q0, src);
             if (!write) return r;
         }
         base = __shfl_sync(0xffffffffu, end, 31);

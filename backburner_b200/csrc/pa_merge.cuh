@@ -24,6 +24,8 @@ struct Params {
     uint64_t rows_per_set;       // nkv * rows
     uint32_t n_sets;
     int fold;                    // 1: (O, M, L) already hold a partial to fold in
+    uint32_t rows, unit_rows, n_rt;   // UNITS: rows per head; of a unit; units of a set: c_range is by unit, and a slot holds
+                                      // the [nkv][unit_rows] rows of one unit
     uint16_t *Oh;                // REPLY: f16(O / l) and lse = m + log l instead of O, M, L (normalize_kernel's)
     float *lse;
 };
@@ -34,7 +36,7 @@ struct Params {
 // memory, and every warp accumulates sum_c w_c O_c, sum_c w_c l_c against that same M, so the warps' sums simply add.
 // Weights are computed 32 parts at a time (one per lane) and broadcast; the O loads of a batch do not depend on one
 // another, and a part with l <= 0 (no keys) gets weight 0 and its O is not used.
-template <int HD, int SPLIT, bool REPLY = false>
+template <int HD, int SPLIT, bool UNITS = false, bool REPLY = false>
 __global__ void __launch_bounds__(256) merge_kernel(const Params p) {
     constexpr int V = HD / 32;          // floats per lane
     constexpr int RPB = 8 / SPLIT;      // rows per block
@@ -48,10 +50,16 @@ __global__ void __launch_bounds__(256) merge_kernel(const Params p) {
     const bool active = gw < (uint64_t) p.n_sets * p.rows_per_set;
     const uint32_t s = active ? (uint32_t) (gw / p.rows_per_set) : 0;
     const uint64_t R = active ? gw % p.rows_per_set : 0;
-    const uint32_t c0 = !active ? 0 : p.c_range ? p.c_range[s] : 0;
-    const uint32_t c1 = !active ? 0 : p.c_range ? p.c_range[s + 1] : p.n_parts;
+    uint32_t u = s;
+    uint64_t rr = (uint64_t) s * p.set_rows + R;
+    if constexpr (UNITS) {
+        const uint32_t h = (uint32_t) R / p.rows, r = (uint32_t) R % p.rows, rt = r / p.unit_rows;
+        u = s * p.n_rt + rt;
+        rr = (uint64_t) h * p.unit_rows + (r - rt * p.unit_rows);
+    }
+    const uint32_t c0 = !active ? 0 : p.c_range ? p.c_range[u] : 0;
+    const uint32_t c1 = !active ? 0 : p.c_range ? p.c_range[u + 1] : p.n_parts;
     const uint64_t orow = (uint64_t) s * p.rows_per_set + R;
-    const uint64_t rr = (uint64_t) s * p.set_rows + R;
 
     // ---- the row maximum over the parts with keys (and the partial already in O, M, L when folding)
     float m_in = -INFINITY, l_in = 0.f;

@@ -277,13 +277,42 @@ __global__ void __launch_bounds__(32 * cta_warps(NT), 1) prefill_kernel(const __
 
     // CTA order (a 1-D grid): row-tile group fastest, then KV head, then job, so the CTAs that read the same K/V
     // blocks (all row groups and heads of one chunk of keys) run at the same time and share them through L2
+    // (PAGED: a part's row tile is its unit's, so only KV head, then part)
     const uint32_t cid = blockIdx.x;
-    const uint32_t rt = cid % p.n_rt, h = (cid / p.n_rt) % p.nkv;
+    const uint32_t h = PAGED ? cid % p.nkv : (cid / p.n_rt) % p.nkv;
     const uint32_t warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+    uint32_t rt = cid % p.n_rt;
     dec::Job job;
     uint32_t nblk = 0;
+    __shared__ pg::Part s_part;
+    __shared__ pg::Tile s_tile;
+    // PAGED, from the TMA warp, 32 groups of 64 keys at a time: a group's row in the tensor maps; its first key, with bit 31 where
+    // not every row of the tile sees all of it (NO_GROUP: none); and then the keys that some row sees. The dequantisers and the
+    // softmax read them when they need them: values kept in registers for the few masked blocks, or worked out in place, cost
+    // every block spills and instruction-cache misses (64-key blocks of two tiles 3,700 cycles, and 3,250 so). Slots are
+    // written again 32 groups behind the block that is loaded; the softmax is at most raw stages + operand buffers + 1 blocks
+    // (12 groups) behind it.
+    constexpr uint32_t NO_GROUP = 0xFFFFFFFFu;
+    __shared__ uint32_t s_group[64], s_grow[64];
+    __shared__ uint64_t s_live[64];
+    __shared__ pg::Row s_row[PAGED ? NT * BM : 1];   // what each row sees (kept here: the loop's code stays short)
     if constexpr (PAGED) {
-        job.slot = cid / (p.n_rt * p.nkv);
+        pdl_trigger();
+        pdl_wait();
+        if (warp == 2) {
+            const pg::Part f = pg::find_part<64>(p.pg, cid / p.nkv, cid == 0, lane);
+            const pg::Tile tl = pg::tile_of(p.pg.v, f.st, f.set, f.t0, f.t1, lane);
+            if (lane == 0) {
+                s_part = f;
+                s_tile = tl;
+            }
+        }
+        __syncthreads();
+        if (__shfl_sync(0xffffffffu, s_part.of, 0) == 0) return;
+        const uint32_t n = (uint32_t) pg::span_of<64>(p.pg.v, s_part.st, s_part.t0, s_part.t1).n;
+        // (through a shuffle, so that the compiler knows them to be the same in all lanes and keeps the loops uniform)
+        rt = __shfl_sync(0xffffffffu, s_part.rt, 0);
+        nblk = __shfl_sync(0xffffffffu, (s_part.end(n) - s_part.begin(n) + B / 64 - 1) / (B / 64), 0);
     } else {
         job = p.jobs[cid / (p.n_rt * p.nkv)];
         nblk = (job.nk + B - 1) / B;
@@ -292,6 +321,8 @@ __global__ void __launch_bounds__(32 * cta_warps(NT), 1) prefill_kernel(const __
     const int hx = (int) (hbyte & ~15u);          // window start (16-byte aligned) of this head in a key row
     const uint32_t hoff = hbyte & 15u;            // head start inside the window
     const uint32_t row0 = rt * NT * BM;           // first query row of this CTA (within the head)
+    // row tiles with real rows (PAGED: the last unit of a head may fill one of two)
+    const int nt = PAGED && NT > 1 && p.rows - row0 <= BM ? 1 : NT;
     const uint64_t tmo = p.timeout_ns;
     bool ok = true;
 
@@ -323,36 +354,8 @@ __global__ void __launch_bounds__(32 * cta_warps(NT), 1) prefill_kernel(const __
         *abort_flag = *(volatile int *) p.status != ST_OK;
         fence_mbar_init();
     }
-    __shared__ pg::Part s_part;
-    __shared__ pg::Tile s_tile;
-    pg::Span span{};
-    uint32_t pg0 = 0, pgn = 0;   // PAGED: this CTA's groups [pg0, pg0 + pgn) of its row tile's span
-    if constexpr (PAGED) {
-        pdl_trigger();
-        pdl_wait();
-        // the tokens of the tile's rows (row r: token r % n_tok): all of them when the rows pass the last token
-        const uint32_t T = p.pg.v.n_tok, n = min((uint32_t) (NT * BM), p.rows - row0), a = row0 % T;
-        const uint32_t t0 = a + n > T ? 0u : a, t1 = a + n > T ? T - 1 : a + n - 1;
-        if (warp == 2) {
-            const pg::Part f = pg::find_part<64>(p.pg, job.slot, cid == 0, lane);
-            const pg::Tile tl = pg::tile_of(p.pg.v, f.st, f.set, t0, t1, lane);
-            if (lane == 0) {
-                s_part = f;
-                s_tile = tl;
-            }
-        }
-        __syncthreads();
-        job.set = s_part.set;
-        span = pg::span_of<64>(p.pg.v, s_part.st, t0, t1);
-        if (s_part.of) {
-            const uint32_t per = ((uint32_t) span.n + s_part.of - 1) / s_part.of;
-            pg0 = min(s_part.index * per, (uint32_t) span.n);
-            pgn = min(per, (uint32_t) span.n - pg0);
-        }
-        nblk = (pgn + B / 64 - 1) / (B / 64);
-    }
     __syncthreads();
-    if (*abort_flag || (PAGED && s_part.of == 0)) return;   // uniform: before TMEM is allocated
+    if (*abort_flag) return;   // uniform: before TMEM is allocated
     if (warp == 1) {   // TMEM: per tile S, two P buffers and O; one tile: a second S
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)),
                      "r"(TCOLS)
@@ -381,46 +384,68 @@ __global__ void __launch_bounds__(32 * cta_warps(NT), 1) prefill_kernel(const __
       // 16 warps launched with 128 registers each at NT = 1 and 2; each warpgroup resizes its share (NT = 1, 64-key
       // blocks: control 160, softmax 168, two dequant warpgroups 88; 128-key blocks: control 128, softmax 200 (the 128
       // scores of a row), dequant 88: 128 x (160 + 168 + 88 + 88) or 128 x (128 + 200 + 88 + 88) = 64,512 <= 65,536)
-      if constexpr (NT == 1 && B == 64) asm volatile("setmaxnreg.inc.sync.aligned.u32 160;");
+      // (PAGED: the dequantisers hold the live masks too: control 96, dequant 112 (NT = 2) or 104; hd 256: control 128, dequant
+      // 104. 128 x (96 + 152 + 152 + 112), 128 x (96 + 200 + 104 + 104), 128 x (128 + 168 + 104 + 104) <= 65,536)
+      if constexpr (PAGED && !(NT == 1 && B == 64)) asm volatile("setmaxnreg.dec.sync.aligned.u32 96;");
+      else if constexpr (!PAGED && NT == 1 && B == 64) asm volatile("setmaxnreg.inc.sync.aligned.u32 160;");
       if (warp == 0) {
         // ------------------------------------------------ TMA producer
         if (lane == 0) {
             if constexpr (!QT) {
-                const int qrow = (int) (((uint64_t) job.set * p.nkv + h) * p.rows + row0);
-                mbar_arrive_expect_tx(q_full, NT * BM * D * 2);
-                for (int t = 0; t < NT; t++)
+                const int qrow = (int) (((uint64_t) (PAGED ? s_part.set : job.set) * p.nkv + h) * p.rows + row0);
+                mbar_arrive_expect_tx(q_full, nt * BM * D * 2);
+                for (int t = 0; t < nt; t++)
                     for (int c = 0; c < D / 64; c++)
                         tma_2d(smem + L::Q + t * BM * D * 2 + c * BM * 128, &tq, c * 64, qrow + t * BM, q_full);
             }
-            const CUtensorMap *km = p.kv_maps + 2 * job.seg, *vm = km + 1;
-            uint32_t issued = 0;
-            for (uint32_t j = 0; j < nblk; j++) {
-                const uint32_t st = j % NRS;
-                // PAGED: the last block may hold one group fewer; the pages are looked up before the wait
-                const uint32_t copies = PAGED ? min((uint32_t) (B / BN), pgn - j * (B / BN)) : (uint32_t) (B / BN);
-                uint32_t prow[B / BN];
-                if constexpr (PAGED) {
-#pragma unroll
-                    for (int c = 0; c < B / BN; c++)
-                        prow[c] = c < (int) copies ? p.pg.row0 + pg::row_at(p.pg.v, job.set, (uint32_t) span.group((int) (pg0 + j * (B / BN)) + c) * BN) : 0u;
+        }
+        const CUtensorMap *km = p.kv_maps + (PAGED ? 0 : 2 * job.seg), *vm = km + 1;
+        pg::Span span{};
+        uint32_t pg0 = 0, pgn = 0;   // PAGED: this CTA's groups [pg0, pg0 + pgn) of its unit's span
+        if constexpr (PAGED) {
+            span = pg::span_of<64>(p.pg.v, s_part.st, s_part.t0, s_part.t1);
+            pg0 = s_part.begin((uint32_t) span.n);
+            pgn = s_part.end((uint32_t) span.n) - pg0;
+        }
+        uint32_t issued = 0;
+        for (uint32_t j = 0; j < nblk; j++) {
+            const uint32_t st = j % NRS;
+            if constexpr (PAGED) {
+                if (j % (32 / (B / BN)) == 0) {
+                    const uint32_t g = j * (B / BN) + lane;
+                    const int k0 = span.group((int) (pg0 + g)) * BN;
+                    const bool some = g < pgn, full = some && s_tile.full(k0, BN);
+                    s_grow[g % 64] = some ? p.pg.row0 + pg::row_at(p.pg.v, s_part.set, (uint32_t) k0) : 0u;
+                    s_group[g % 64] = !some ? NO_GROUP : full ? (uint32_t) k0 : (uint32_t) k0 | 0x80000000u;
+                    if (!full) s_live[g % 64] = some ? pg::vis64(s_tile.any, k0) : 0ull;
+                    __syncwarp();
                 }
-                if (j >= NRS && !wait(&raw_empty[st], ((j / NRS) - 1) & 1)) break;
-                mbar_arrive_expect_tx(&raw_full[st], 2 * copies * BN * RAWB);
-                uint8_t *dst = smem + L::RAW + st * L::RAW_STAGE;
-#pragma unroll
-                for (int c = 0; c < B / BN; c++) {   // the tensor maps' boxes hold 64 keys
-                    int key;
-                    if constexpr (PAGED) {
-                        if (c >= (int) copies) break;
-                        key = (int) prow[c];
-                    } else {
-                        key = (int) (job.key0 + j * B) + c * BN;
-                    }
-                    tma_2d(dst + c * BN * RAWB, km, hx / 2, key, &raw_full[st]);
-                    tma_2d(dst + (B + c * BN) * RAWB, vm, hx / 2, key, &raw_full[st]);
-                }
-                issued = j + 1;
             }
+            if (lane == 0) {
+                if (j >= NRS) wait(&raw_empty[st], ((j / NRS) - 1) & 1);
+                if (ok) {
+                    // PAGED: the last block may hold one group fewer
+                    const uint32_t copies = PAGED ? min((uint32_t) (B / BN), pgn - j * (B / BN)) : (uint32_t) (B / BN);
+                    mbar_arrive_expect_tx(&raw_full[st], 2 * copies * BN * RAWB);
+                    uint8_t *dst = smem + L::RAW + st * L::RAW_STAGE;
+#pragma unroll
+                    for (int c = 0; c < B / BN; c++) {   // the tensor maps' boxes hold 64 keys
+                        int key;
+                        if constexpr (PAGED) {
+                            if (c >= (int) copies) break;
+                            key = (int) s_grow[(j * (B / BN) + c) % 64];
+                        } else {
+                            key = (int) (job.key0 + j * B) + c * BN;
+                        }
+                        tma_2d(dst + c * BN * RAWB, km, hx / 2, key, &raw_full[st]);
+                        tma_2d(dst + (B + c * BN) * RAWB, vm, hx / 2, key, &raw_full[st]);
+                    }
+                    issued = j + 1;
+                }
+            }
+            if (!__shfl_sync(0xffffffffu, ok, 0)) break;
+        }
+        if (lane == 0) {
             // on an abort, every issued copy lands before the CTA exits
             if (!ok) {
                 const uint64_t drain = tmo > dec::DRAIN_NS ? tmo : dec::DRAIN_NS;
@@ -447,6 +472,7 @@ __global__ void __launch_bounds__(32 * cta_warps(NT), 1) prefill_kernel(const __
                     const uint64_t dk = dk0 + b * (uint32_t) (B * D * 2 / 16);
 #pragma unroll
                     for (int t = 0; t < NT; t++) {
+                        if (PAGED && t >= nt) break;
                         const uint32_t sb = t * NSB + j % NSB;   // the block's S buffer
                         if (j >= NSB && !wait(&s_empty[sb], ((j / NSB) - 1) & 1)) break;
                         tc_fence_after();
@@ -475,6 +501,7 @@ __global__ void __launch_bounds__(32 * cta_warps(NT), 1) prefill_kernel(const __
                 const uint64_t dv = dv0 + b * (uint32_t) (B * D * 2 / 16);
 #pragma unroll
                 for (int t = 0; t < NT; t++) {
+                    if (PAGED && t >= nt) break;
                     const uint32_t pb = jj % NPB;   // P buffer
                     if (!wait(&p_full[t * NPB + pb], (jj / NPB) & 1)) break;
                     tc_fence_after();
@@ -512,14 +539,15 @@ __global__ void __launch_bounds__(32 * cta_warps(NT), 1) prefill_kernel(const __
         // S, P and Q barriers count only the warps with a real row, its rows' O is never written and MMA rows are
         // independent, so its S, P and Q may stay as they are. (It must not arrive at all: a warp that does no work can
         // run ahead of the real warps, and its arrival for a later block would complete an earlier block's phase.)
-        const bool pad = NT == 1 && row0 + t * BM + wq * 32 >= p.rows;
+        // (PAGED: a second tile without rows sits out as a whole)
+        const bool pad = (NT == 1 && row0 + t * BM + wq * 32 >= p.rows) || (PAGED && t >= nt);
         // Q in tensor memory: each warp with a real row writes its lanes' Q rows (rows past the call's rows as zeros)
         // into the Q columns, then arrives on q_full, which the S issuer waits for
         if constexpr (QT) {
             if (!pad && ok) {
                 const uint32_t row = row0 + r;
                 const uint4 *src =
-                    reinterpret_cast<const uint4 *>(p.Qs + (((uint64_t) job.set * p.nkv + h) * p.rows + row) * D);
+                    reinterpret_cast<const uint4 *>(p.Qs + (((uint64_t) (PAGED ? s_part.set : job.set) * p.nkv + h) * p.rows + row) * D);
 #pragma unroll
                 for (int c = 0; c < D / 64; c++) {   // 64 dims (32 columns) at a time
                     uint32_t qv[32];
@@ -538,8 +566,7 @@ __global__ void __launch_bounds__(32 * cta_warps(NT), 1) prefill_kernel(const __
         }
         float m_used = -INFINITY, l = 0.f;
         float m_row = -INFINITY;   // the row's exact maximum (log2 units); O and l are reported against it
-        pg::Row mine{};
-        if constexpr (PAGED) mine = pg::row_of(p.pg.v, s_part.st, job.set, (row0 + t * BM + r) % p.pg.v.n_tok);
+        if constexpr (PAGED) s_row[t * BM + r] = pg::row_of(p.pg.v, s_part.st, s_part.set, (row0 + t * BM + r) % p.pg.v.n_tok);
         for (uint32_t j = 0; j < nblk && !pad; j++) {
             const uint32_t b = j % NPB;                    // the block's P buffer
             const uint32_t sb = t * NSB + j % NSB;         // the block's S buffer
@@ -563,10 +590,10 @@ __global__ void __launch_bounds__(32 * cta_warps(NT), 1) prefill_kernel(const __
             if constexpr (PAGED) {
 #pragma unroll
                 for (int c = 0; c < B / 64; c++) {
-                    const uint32_t gi = j * (B / 64) + c;   // the group within the CTA's
-                    const int k0 = span.group((int) (pg0 + gi)) * 64;
-                    if (gi >= pgn || !s_tile.full(k0, 64)) {
-                        const uint64_t see = gi < pgn ? pg::vis64(mine, k0) : 0ull;
+                    const uint32_t group = *(volatile uint32_t *) &s_group[(j * (B / 64) + c) % 64];
+                    if ((int) group < 0) {
+                        uint64_t see = 0;
+                        if (group != NO_GROUP) see = pg::vis64(s_row[t * BM + r], (int) (group & 0x7FFFFFFFu));
                         const uint32_t lo = (uint32_t) see, hi = (uint32_t) (see >> 32);
 #pragma unroll
                         for (int i = 0; i < 32; i++) {
@@ -583,10 +610,15 @@ __global__ void __launch_bounds__(32 * cta_warps(NT), 1) prefill_kernel(const __
                     if (i >= nvalid) s[i] = -INFINITY;
             }
             }
-            float mx = s[0];
+            float mx4[4];   // four chains: one would be B / 2 dependent steps long
 #pragma unroll
-            for (int i = 1; i + 1 < B; i += 2) mx = max3(mx, s[i], s[i + 1]);
-            mx = fmaxf(mx, s[B - 1]);
+            for (int q = 0; q < 4; q++) {
+                mx4[q] = s[q * (B / 4)];
+#pragma unroll
+                for (int i = 1; i + 1 < B / 4; i += 2) mx4[q] = max3(mx4[q], s[q * (B / 4) + i], s[q * (B / 4) + i + 1]);
+                mx4[q] = fmaxf(mx4[q], s[q * (B / 4) + B / 4 - 1]);
+            }
+            float mx = fmaxf(max3(mx4[0], mx4[1], mx4[2]), mx4[3]);
             mx *= LOG2E;
             m_row = fmaxf(m_row, mx);
             float alpha = 1.f;
@@ -644,9 +676,11 @@ __global__ void __launch_bounds__(32 * cta_warps(NT), 1) prefill_kernel(const __
         if (ok && !pad && nblk > 0 && wait(&o_ready[t], 0)) {
             tc_fence_after();
             const uint32_t row = row0 + t * BM + r;
-            const uint64_t orow = ((uint64_t) job.slot * p.nkv + h) * p.rows + row;
+            // PAGED: a slot holds one unit's rows
+            const uint64_t orow = PAGED ? ((uint64_t) (cid / p.nkv) * p.nkv + h) * (NT * BM) + t * BM + r
+                                        : ((uint64_t) job.slot * p.nkv + h) * p.rows + row;
             if constexpr (PAGED) {   // a padding token's row is empty, whatever its scores were
-                if (pg::is_padding(p.pg.v, job.set, row % p.pg.v.n_tok)) l = 0.f;
+                if (pg::is_padding(p.pg.v, s_part.set, row % p.pg.v.n_tok)) l = 0.f;
             }
             const float fix = m_row > -INFINITY ? ex2(m_used - m_row) : 1.f;
 #pragma unroll
@@ -666,33 +700,23 @@ __global__ void __launch_bounds__(32 * cta_warps(NT), 1) prefill_kernel(const __
                 p.Lp[orow] = l * fix;
             }
         }
-        if constexpr (PAGED) {   // a part of the set that holds nothing for this row tile
-            const uint32_t row = row0 + t * BM + r;
-            if (nblk == 0 && row < p.rows) {
-                const uint64_t orow = ((uint64_t) job.slot * p.nkv + h) * p.rows + row;
-                p.Mp[orow] = -INFINITY;
-                p.Lp[orow] = 0.f;
-            }
-        }
     } else {
         // ------------------------------------------------ dequantisers: warp dw owns quant blocks dw % 4 (+ 4 at
         // D = 256) of every key (4 warps: both 32-key halves of each 64 keys; 8 warps, NT = 1: key half dw / 4 of each
         // 64 keys)
-        if (NT == 2) asm volatile("setmaxnreg.dec.sync.aligned.u32 80;");
+        if constexpr (PAGED && NT == 2) asm volatile("setmaxnreg.dec.sync.aligned.u32 112;");
+        else if constexpr (PAGED) asm volatile("setmaxnreg.dec.sync.aligned.u32 104;");
+        else if constexpr (NT == 2) asm volatile("setmaxnreg.dec.sync.aligned.u32 80;");
         else asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
         const uint32_t dw = warp - DQ0;
         for (uint32_t j = 0; j < nblk; j++) {
             const uint32_t st = j % NRS, b = j % KVB;
             if (!wait(&raw_full[st], (j / NRS) & 1)) break;
             const uint32_t raw = sbase + L::RAW + st * L::RAW_STAGE;
-            uint64_t live[B / 64];   // PAGED: keys of each group that some row of the tile sees
+            bool edge = false;   // PAGED: some row of the tile does not see all of the block
             if constexpr (PAGED) {
 #pragma unroll
-                for (int c = 0; c < B / 64; c++) {
-                    const uint32_t gi = j * (B / 64) + c;
-                    const int k0 = span.group((int) (pg0 + gi)) * 64;
-                    live[c] = gi >= pgn ? 0ull : s_tile.full(k0, 64) ? ~0ull : pg::vis64(s_tile.any, k0);
-                }
+                for (int c = 0; c < B / 64; c++) edge |= (int) *(volatile uint32_t *) &s_group[(j * (B / 64) + c) % 64] < 0;
             }
             // Items of the block for this warp: 64-key chunk kc, key half (8 warps) or pass (4 warps), quant block of the
             // warp; K's, then V's. An item's words are loaded while the one before it is converted (the loads and stores are
@@ -709,10 +733,7 @@ __global__ void __launch_bounds__(32 * cta_warps(NT), 1) prefill_kernel(const __
                 const uint32_t bo = hoff + GB * qblk_of(it);   // block start inside the raw window row
                 const uint32_t w16 = bo & ~15u;                // 16-byte aligned start of the words covering it
                 const uint32_t rb = raw + kv * B * RAWB + key_of(it) * RAWB;
-                uint32_t s2 = lds16(rb + bo);
-                if constexpr (PAGED) {
-                    if (kv == 1 && !(live[it / (8 / NDQ) % (B / 64)] >> (key_of(it) % 64) & 1ull)) s2 = 0u;
-                }
+                const uint32_t s2 = lds16(rb + bo);
                 sc2 = s2 | (s2 << 16);
                 // q8_0: the block's 34 bytes lie within 3 aligned 16-byte chunks; q4_0: 18 bytes within 2
 #pragma unroll
@@ -783,6 +804,19 @@ __global__ void __launch_bounds__(32 * cta_warps(NT), 1) prefill_kernel(const __
                     sts128(kbase + (((c0 + 3) ^ (key % 8)) * 16), hi[4], hi[5], hi[6], hi[7]);
                 }
                 if (it + 1 == NI) {
+                    if constexpr (PAGED) {
+                        if (kv == 1 && edge) {   // V rows that no row sees may hold anything (NaN): cleared (rolled: rare)
+#pragma unroll 1
+                            for (int z = 0; z < NI; z++) {
+                                const uint32_t k = key_of(z), qb = qblk_of(z);
+                                const uint32_t g = (j * (B / 64) + k / 64) % 64;
+                                if ((int) *(volatile uint32_t *) &s_group[g] >= 0 || (s_live[g] >> (k % 64) & 1ull)) continue;
+                                const uint32_t kb = sbase + L::V + b * B * D * 2 + (qb / 2) * B * 128 + (k / 8) * 1024 + (k % 8) * 128;
+#pragma unroll 1
+                                for (uint32_t c = 4 * (qb % 2); c < 4 * (qb % 2) + 4; c++) sts128(kb + ((c ^ (k % 8)) * 16), 0u, 0u, 0u, 0u);
+                            }
+                        }
+                    }
                     fence_proxy_async();
                     __syncwarp();
                     if (lane == 0) mbar_arrive(kv == 0 ? &k_full[b] : &v_full[b]);

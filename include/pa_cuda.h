@@ -255,7 +255,7 @@ uint64_t pa_cuda_graph_calls(const pa_cuda_ctx *ctx);
  * (pa_cuda_cache_attn), and after a verify keeps the accepted rows (pa_cuda_cache_compact); pa_cuda_cache_copy_pages forks.
  *
  * Row of layer i, page p, position j: k + (((uint64_t) i * n_pages + p) * page_keys + j) * rs, v alike (rs, hb of the
- * shape; device pointers, 16-byte aligned). page_keys: a multiple of 64. At most 2^31 - 1 rows in all layers.
+ * shape; device pointers, 16-byte aligned). page_keys: a multiple of 64, at most 2^22. At most 2^31 - 1 rows in all layers.
  * Sequences ("sets") number their keys 0, 1, ...: key j of set s lies in page table[s][j / page_keys] (int32, device,
  * [n_sets][max_pages]; entries no key needs are not read and may hold anything). Rows past a sequence's keys, and rows no
  * token of the call sees, may hold anything, NaN included; a row that some tokens of a call see has to be finite.

@@ -14,7 +14,7 @@ ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 SRC = r'''
 #include <cstdio>
 #include <cstdlib>
-#include "pa_cache.cuh"
+#include "pa_mask.cuh"
 using namespace pa::pg;
 template <int G> void spans(const View &v, Set st, unsigned t0, unsigned t1) {
   Span p = span_of<G>(v, st, t0, t1);
