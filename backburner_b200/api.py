@@ -635,28 +635,32 @@ class CachePlan:
         """The unnormalised partial (O, m, l) (pa_cuda_cache_attn). Qs: f16(q * scale) [n_sets][nkv][gqa * n_tok][hd],
         row g * n_tok + t; table int32 [n_sets][max_pages]; n_keys, q_pos int32 [n_sets]; tree int64 [n_sets][n_tok]."""
         import torch
-        args, f32 = self._args(layer, Qs, table, n_keys, q_pos, tree), torch.float32
+        ctx, f32 = self.ctx, torch.float32
+        args = self._args(layer, Qs, table, n_keys, q_pos, tree)
         if out is None:
-            O = torch.empty(Qs.shape, dtype=f32, device=Qs.device)
-            m = torch.empty(self._rows, dtype=f32, device=Qs.device)
-            out = (O, m, torch.empty_like(m))
+            m = Qs.new_empty(self._rows, dtype=f32)
+            out = Qs.new_empty(self._full, dtype=f32), m, torch.empty_like(m)
+        else:
+            for t, name, shape in zip(out, ("O", "m", "l"), (self._full, self._rows, self._rows)):
+                _want(ctx, t, name, f32, shape)
         O, m, l = out
-        self.ctx.check(lib().pa_cuda_cache_attn(*args, _want(self.ctx, O, "O", f32, self._full),
-                                                _want(self.ctx, m, "m", f32, self._rows),
-                                                _want(self.ctx, l, "l", f32, self._rows), _stream_on(self.ctx, stream)),
-                       "cache_attn")
+        ctx.check(lib().pa_cuda_cache_attn(*args, O.data_ptr(), m.data_ptr(), l.data_ptr(), _stream_on(ctx, stream)),
+                  "cache_attn")
         return O, m, l
 
     def reply(self, layer: int, Qs, table, n_keys, q_pos=None, tree=None, out=None, stream=None):
         """The same, normalised: (f16 O / l, lse) (pa_cuda_cache_attn_reply)."""
         import torch
+        ctx = self.ctx
         args = self._args(layer, Qs, table, n_keys, q_pos, tree)
         if out is None:
             out = torch.empty_like(Qs), Qs.new_empty(self._rows, dtype=torch.float32)
+        else:
+            _want(ctx, out[0], "Oh", torch.float16, self._full)
+            _want(ctx, out[1], "lse", torch.float32, self._rows)
         Oh, lse = out
-        self.ctx.check(lib().pa_cuda_cache_attn_reply(*args, _want(self.ctx, Oh, "Oh", torch.float16, self._full),
-                                                      _want(self.ctx, lse, "lse", torch.float32, self._rows),
-                                                      _stream_on(self.ctx, stream)), "cache_attn_reply")
+        ctx.check(lib().pa_cuda_cache_attn_reply(*args, Oh.data_ptr(), lse.data_ptr(), _stream_on(ctx, stream)),
+                  "cache_attn_reply")
         return Oh, lse
 
     def close(self):
@@ -716,12 +720,13 @@ def cache_append(ctx: Context, cache: Cache, layer: int, q, k, v, table, start, 
     rows = (S, cache.nkv, n_rows, hd)
     if out is None:
         out = q.new_empty(rows, dtype=torch.float16)
+    else:
+        _want(ctx, out, "out", torch.float16, rows)
     pages = table.shape[-1]
     ctx.check(lib().pa_cuda_cache_append(ctx.handle, cache.shape(n_rows or 1), cache.on(ctx), layer, ctypes.byref(a), S, T,
                                          _want(ctx, table, "table", torch.int32, (S, pages)), pages,
                                          _want(ctx, start, "start", torch.int32, (S,)),
-                                         _want(ctx, out, "out", torch.float16, rows), _stream_on(ctx, stream)),
-              "cache_append")
+                                         out.data_ptr(), _stream_on(ctx, stream)), "cache_append")
     return out
 
 
@@ -734,11 +739,13 @@ def cache_rows(ctx: Context, cache: Cache, layer: int, table, first, n: int, out
     if out is None:
         K = table.new_empty(shape, dtype=torch.float16)
         out = (K, torch.empty_like(K))
+    else:
+        _want(ctx, out[0], "K", torch.float16, shape)
+        _want(ctx, out[1], "V", torch.float16, shape)
     ctx.check(lib().pa_cuda_cache_rows(ctx.handle, cache.shape(1), cache.on(ctx), layer, S, n,
                                        _want(ctx, table, "table", torch.int32, (S, table.shape[1])), table.shape[1],
                                        _want(ctx, first, "first", torch.int32, (S,)),
-                                       _want(ctx, out[0], "K", torch.float16, shape),
-                                       _want(ctx, out[1], "V", torch.float16, shape), _stream_on(ctx, stream)), "cache_rows")
+                                       out[0].data_ptr(), out[1].data_ptr(), _stream_on(ctx, stream)), "cache_rows")
     return out
 
 
@@ -760,7 +767,7 @@ def cache_compact(ctx: Context, cache: Cache, table, start, path, count, out=Non
     import torch
     S, T = path.shape
     if out is None:
-        out = torch.empty((S,), dtype=torch.int32, device=path.device)
+        out = torch.empty_like(start)
     ctx.check(lib().pa_cuda_cache_compact(ctx.handle, cache.shape(1), cache.on(ctx), S, T,
                                           _want(ctx, table, "table", torch.int32, (S, table.shape[1])), table.shape[1],
                                           _want(ctx, start, "start", torch.int32, (S,)),

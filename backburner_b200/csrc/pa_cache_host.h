@@ -157,7 +157,7 @@ int cache_attn(pa_cuda_cache_plan *p, uint32_t layer, const uint16_t *Qs, const 
     pg.v.n_tok = p->mask.n_tok;
     pg.v.window = p->mask.window;
     pg.v.sinks = p->mask.sinks;
-    pg.v.status = ctx->d_status;
+    pg.v.status = ctx->d_status + 1;
     pg.k = p->cache.k + layer * layer_bytes(sh, p->cache);
     pg.vr = p->cache.v + layer * layer_bytes(sh, p->cache);
     pg.row0 = layer * p->cache.n_pages * p->cache.page_keys;
@@ -347,6 +347,8 @@ int pa_cuda_cache_plan_create(pa_cuda_ctx *ctx, const pa_cuda_shape *shape, cons
         return fail(ctx, PA_CUDA_EUNSUPPORTED, "a tree needs a window of at least n_tok keys");
     if (ctx->qk_domain == PA_CUDA_QK_INT8)
         return fail(ctx, PA_CUDA_EUNSUPPORTED, "the int8-domain QK does not cover the paged cache");
+    if ((uint64_t) n_sets * shape->nkv * shape->rows > 0x7FFFFFFFull)
+        return fail(ctx, PA_CUDA_EUNSUPPORTED, "more than 2^31 - 1 query rows in a call");
     auto *p = new pa_cuda_cache_plan();
     p->ctx = ctx;
     p->sh = *shape;
@@ -449,7 +451,7 @@ int pa_cuda_cache_append(pa_cuda_ctx *ctx, const pa_cuda_shape *shape, const pa_
     a.view.page_keys = cache->page_keys;
     a.view.page_mul = page_mul(cache->page_keys);
     a.view.n_tok = n_tok;
-    a.view.status = ctx->d_status;
+    a.view.status = ctx->d_status + 1;
     a.K = cache->k + layer * layer_bytes(*shape, *cache);
     a.V = cache->v + layer * layer_bytes(*shape, *cache);
     a.Qs = Qs;
@@ -501,7 +503,7 @@ int pa_cuda_cache_rows(pa_cuda_ctx *ctx, const pa_cuda_shape *shape, const pa_cu
     a.v.page_keys = cache->page_keys;
     a.v.page_mul = page_mul(cache->page_keys);
     a.v.n_tok = n_tok;
-    a.v.status = ctx->d_status;
+    a.v.status = ctx->d_status + 1;
     a.first = first;
     a.K = cache->k + layer * layer_bytes(*shape, *cache);
     a.V = cache->v + layer * layer_bytes(*shape, *cache);
@@ -532,7 +534,7 @@ int pa_cuda_cache_copy_pages(pa_cuda_ctx *ctx, const pa_cuda_shape *shape, const
     a.page_bytes = cache->page_keys * shape->rs;
     a.n_pages = cache->n_pages;
     a.n_layers = cache->n_layers;
-    a.status = ctx->d_status;
+    a.status = ctx->d_status + 1;
     const uint64_t per = 256ull * 16 * pa::pg::COPY_UNROLL, x = (a.page_bytes + per - 1) / per;
     if (x > 0x7FFFFFFFull) return fail(ctx, PA_CUDA_EUNSUPPORTED, "pages too large");
     for (uint32_t i = 0; i < n; i += 65535) {
@@ -564,7 +566,7 @@ int pa_cuda_cache_compact(pa_cuda_ctx *ctx, const pa_cuda_shape *shape, const pa
     a.v.page_keys = cache->page_keys;
     a.v.page_mul = page_mul(cache->page_keys);
     a.v.n_tok = n_tok;
-    a.v.status = ctx->d_status;
+    a.v.status = ctx->d_status + 1;
     a.K = cache->k;
     a.V = cache->v;
     a.start = start;

@@ -77,7 +77,7 @@ struct pa_cuda_ctx {
     int device = 0;
     int n_sm = 148;
     cudaStream_t stream = nullptr;
-    int *d_status = nullptr;
+    int *d_status = nullptr;      // [0] bounded waits that gave up; [1] arguments only the device sees out of range
     int *h_status = nullptr;      // pinned: the status word read back by pa_cuda_status
     uint64_t timeout_ns = 2000000000ull;
     uint64_t launches = 0;
@@ -789,13 +789,13 @@ int pa_cuda_status(pa_cuda_ctx *ctx, void *stream) {
     // the read and the clear stay on the caller's stream (no legacy-stream copy that would wait for every blocking
     // stream of the process, or fail under another thread's global-mode capture)
     PA_CK(cudaSetDevice(ctx->device), "cudaSetDevice");
-    PA_CK(cudaMemcpyAsync(ctx->h_status, ctx->d_status, sizeof(int), cudaMemcpyDeviceToHost, st), "status read");
+    PA_CK(cudaMemcpyAsync(ctx->h_status, ctx->d_status, 2 * sizeof(int), cudaMemcpyDeviceToHost, st), "status read");
     PA_CK(cudaStreamSynchronize(st), "stream synchronize");
-    const int h = *ctx->h_status;
-    if (h != pa::ST_OK) {
-        PA_CK(cudaMemsetAsync(ctx->d_status, 0, sizeof h, st), "status clear");
+    const int h = ctx->h_status[0], args = ctx->h_status[1];
+    if (h != pa::ST_OK || args != pa::ST_OK) {
+        PA_CK(cudaMemsetAsync(ctx->d_status, 0, 2 * sizeof h, st), "status clear");
         PA_CK(cudaStreamSynchronize(st), "stream synchronize");
-        if (h == pa::ST_BAD_ARGS)
+        if (h == pa::ST_OK)
             return fail(ctx, PA_CUDA_EINVAL, "a cache call met a page id, length or path out of range on the device");
         return fail(ctx, PA_CUDA_ETIMEOUT, "a kernel gave up a bounded wait (code " + std::to_string(h) + ")");
     }

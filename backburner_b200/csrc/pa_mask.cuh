@@ -176,8 +176,9 @@ __device__ __forceinline__ Part find_part(const Paged &p, uint32_t c, bool write
     const uint32_t least = max(1u, (uint32_t) sqrtf((float) total / (float) (8 * units)) / 4) * 8;
     uint32_t lo = max(least, (uint32_t) ((total + p.n_parts - 1) / p.n_parts)), hi = lo;
     if (units > 1) {
-        // sum of ceil(cost / per) < total / per + units <= n_parts at hi (n_parts > units, by the plan)
-        hi = max(lo, (uint32_t) ((total + (p.n_parts - units) - 1) / (p.n_parts - units)));
+        // sum of ceil(cost / per) < total / per + units <= n_parts at hi (n_parts > units, by the plan); 2^30 is past any
+        // unit's cost
+        hi = max(lo, (uint32_t) min((uint64_t) 1 << 30, (total + (p.n_parts - units) - 1) / (p.n_parts - units)));
         while (lo < hi) {
             const uint32_t mid = lo + (hi - lo) / 2;
             uint32_t need = 0;

@@ -207,6 +207,15 @@ def test_positions_of_the_queries(ctx, kernel, bits, window, sinks):
     _run(ctx, sq, tok, 5, kernel, window, sinks, q_pos, _tree(np.random.default_rng(1), 9, tok, 0.1) if bits else None)
 
 
+@pytest.mark.parametrize("kernel,quant", [(0, pa.Q8_0), (1, pa.Q4_0), (2, pa.Q8_0)])
+def test_many_ragged_sequences(ctx, kernel, quant):
+    """more units than a warp has lanes: their parts are found in rounds, and every length keeps its own"""
+    rng = np.random.default_rng(5)
+    sq = Seqs(6, [int(x) for x in np.exp(rng.uniform(0, np.log(900), 71))] + [0], 128, 2, quant, 64, layers=1)
+    _run(ctx, sq, 3, 5, kernel)
+    _run(ctx, sq, 30, 9, kernel, 50, 5)
+
+
 @pytest.mark.parametrize("kernel,quant", [(0, pa.Q8_0), (1, pa.Q4_0), (2, pa.Q4_0), (0, pa.F16)])
 def test_many_rows_and_a_long_cache(ctx, kernel, quant):
     """several row tiles, several parts of a sequence, wide pages, rows with padding bytes"""
@@ -469,8 +478,12 @@ def test_arguments_only_the_device_sees(ctx):
         for n in (-1, sq.max_pages * 64 + 1, 2 ** 31 - 1, -2 ** 31):
             plan.reply(0, Qs, torch.zeros_like(sq.table), torch.tensor([100, n], **i32))
             _invalid(ctx)
+        # a call after a bad one is as good as any, whether the status was looked at or not
+        bad = sq.table.clone()
+        bad[0, 0] = total
+        plan.reply(0, Qs, bad, sq.n_keys)
         out = plan.reply(sq.layer, Qs, sq.table, sq.n_keys)
-        ctx.status()
+        _invalid(ctx)
         _check(sq, Qs, out, 2, 5)
         plan.close()
     x = [torch.randn(2, 2, n, 128, generator=sq.g, device="cuda") for n in (40, 8, 8)]
@@ -515,6 +528,7 @@ def test_refusals(ctx):
     no(U, P, ctx, c, 1, 65, 5, 4, tree=True)
     no(U, P, ctx, c, 1, 9, 5, 4, 8, tree=True)
     no(U, P, ctx, c, 65536, 1, 5, 4)
+    no(U, P, ctx, c, 65535, 1 << 14, 1, 4)
     no(U, P, ctx, pa.Cache(128, 8, pa.Q8_0, 1, 4, 96), 1, 1, 5, 4)
     no(U, P, ctx, pa.Cache(64, 8, pa.Q8_0, 1, 4, 64), 1, 1, 5, 4)
     no(I, P, ctx, pa.Cache(128, 8, pa.Q8_0, 1, 4, 64, rs=1024), 1, 1, 5, 4)
