@@ -14,6 +14,133 @@
 namespace pa {
 namespace pg {
 
+// ---------------------------------------------------------------- merge of the paged attention's partials
+// The log-sum-exp merge of a unit's parts (pa_merge.cuh's, over this cache's slots), giving O, m, l or f16(O / l) and lse. A
+// call's merge is a chain of dependent loads (the parts' range, their l and m, their O) behind the attention kernel, so the
+// first MERGE_AHEAD parts' O are loaded beside their l and m rather than after them; SPLIT warps share a row's parts.
+struct MergeParams {
+    const float *Op, *Mp, *Lp;      // slot c: [nkv][unit_rows][HD], [nkv][unit_rows]
+    const uint32_t *crange;         // [units + 1]
+    uint32_t n_sets, nkv, rows, unit_rows, n_rt;
+    float *O, *M, *L;               // [n_sets][nkv][rows]...
+    uint16_t *Oh;                   // or these
+    float *lse;
+};
+template <int HD> constexpr int MERGE_AHEAD = HD == 128 ? 4 : 2;
+template <int HD, int SPLIT, bool REPLY>
+__global__ void __launch_bounds__(256) cache_merge_kernel(const MergeParams p) {
+    constexpr int V = HD / 32, RPB = 8 / SPLIT, AHEAD = MERGE_AHEAD<HD>;
+    __shared__ float s_m[8], s_l[8];
+    __shared__ __align__(16) float s_acc[SPLIT > 1 ? 8 * HD : 4];
+    const uint32_t warp = threadIdx.x / 32, lane = threadIdx.x % 32, sw = warp % SPLIT;
+    const uint64_t row = (uint64_t) blockIdx.x * RPB + warp / SPLIT, per_set = (uint64_t) p.nkv * p.rows;
+    const bool active = row < p.n_sets * per_set;
+    const uint32_t s = active ? (uint32_t) (row / per_set) : 0, R = active ? (uint32_t) (row % per_set) : 0;
+    const uint32_t h = R / p.rows, r = R - h * p.rows, rt = p.n_rt == 1 ? 0 : r / p.unit_rows;
+    const uint64_t rr = (uint64_t) h * p.unit_rows + (r - rt * p.unit_rows), stride = (uint64_t) p.nkv * p.unit_rows;
+    pdl_trigger();
+    pdl_wait();
+    const uint32_t c0 = active ? p.crange[s * p.n_rt + rt] : 0, c1 = active ? p.crange[s * p.n_rt + rt + 1] : 0;
+    // this warp's parts: c0 + sw + SPLIT * i
+    const uint32_t mine = c0 + sw < c1 ? (c1 - c0 - sw + SPLIT - 1) / SPLIT : 0;
+    auto part = [&](uint32_t i) -> uint64_t { return (uint64_t) (c0 + sw + SPLIT * i) * stride + rr; };
+    auto load_o = [&](uint32_t i, float (&o)[V]) {
+        const float4 *src = reinterpret_cast<const float4 *>(p.Op + part(i) * HD + lane * V);
+#pragma unroll
+        for (int q = 0; q < V / 4; q++) {
+            const float4 x = src[q];
+            o[4 * q] = x.x; o[4 * q + 1] = x.y; o[4 * q + 2] = x.z; o[4 * q + 3] = x.w;
+        }
+    };
+    float ahead[AHEAD][V], l0 = 0.f, m0 = -INFINITY;
+    if (lane < mine) {
+        l0 = p.Lp[part(lane)];
+        m0 = p.Mp[part(lane)];
+    }
+#pragma unroll
+    for (int i = 0; i < AHEAD; i++)
+        if ((uint32_t) i < mine) load_o((uint32_t) i, ahead[i]);
+    float M = l0 > 0.f ? m0 : -INFINITY;
+    for (uint32_t i = lane + 32; i < mine; i += 32) {
+        const float l = p.Lp[part(i)], m = p.Mp[part(i)];
+        if (l > 0.f) M = fmaxf(M, m);
+    }
+#pragma unroll
+    for (int x = 16; x > 0; x >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, x));
+    if (SPLIT > 1) {
+        if (lane == 0) s_m[warp] = M;
+        __syncthreads();
+#pragma unroll
+        for (int w = 0; w < SPLIT; w++) M = fmaxf(M, s_m[warp / SPLIT * SPLIT + w]);
+    }
+    float acc[V], L = 0.f;
+#pragma unroll
+    for (int q = 0; q < V; q++) acc[q] = 0.f;
+    for (uint32_t b = 0; b < mine; b += 32) {
+        float l = l0, m = m0;
+        if (b > 0) {
+            l = b + lane < mine ? p.Lp[part(b + lane)] : 0.f;
+            m = b + lane < mine ? p.Mp[part(b + lane)] : -INFINITY;
+        }
+        const float w = l > 0.f ? ex2((m - M) * LOG2E) : 0.f;   // a part without keys may hold anything in O: not used
+        L = fmaf(w, l, L);
+        const uint32_t n = min(32u, mine - b);
+        if (b == 0) {
+#pragma unroll
+            for (int i = 0; i < AHEAD; i++) {
+                const float wi = __shfl_sync(0xffffffffu, w, i);
+                if (wi != 0.f)
+#pragma unroll
+                    for (int q = 0; q < V; q++) acc[q] = fmaf(wi, ahead[i][q], acc[q]);
+            }
+        }
+#pragma unroll 4
+        for (uint32_t i = b == 0 ? AHEAD : 0; i < n; i++) {
+            const float wi = __shfl_sync(0xffffffffu, w, i);
+            float o[V];
+            load_o(b + i, o);
+            if (wi != 0.f)
+#pragma unroll
+                for (int q = 0; q < V; q++) acc[q] = fmaf(wi, o[q], acc[q]);
+        }
+    }
+#pragma unroll
+    for (int x = 16; x > 0; x >>= 1) L += __shfl_xor_sync(0xffffffffu, L, x);
+    if (SPLIT > 1) {   // the warps' sums, against the same M, add up in the row's first warp
+#pragma unroll
+        for (int q = 0; q < V / 4; q++)
+            reinterpret_cast<float4 *>(s_acc + warp * HD + lane * V)[q] = make_float4(acc[4 * q], acc[4 * q + 1], acc[4 * q + 2], acc[4 * q + 3]);
+        if (lane == 0) s_l[warp] = L;
+        __syncthreads();
+        if (sw != 0) return;
+#pragma unroll
+        for (int w = 1; w < SPLIT; w++) {
+#pragma unroll
+            for (int q = 0; q < V / 4; q++) {
+                const float4 x = reinterpret_cast<const float4 *>(s_acc + (warp + w) * HD + lane * V)[q];
+                acc[4 * q] += x.x; acc[4 * q + 1] += x.y; acc[4 * q + 2] += x.z; acc[4 * q + 3] += x.w;
+            }
+            L += s_l[warp + w];
+        }
+    }
+    if (!active) return;
+    if constexpr (REPLY) {
+        const float inv = L > 0.f ? 1.f / L : 0.f;
+#pragma unroll
+        for (int q = 0; q < V; q += 2)
+            *reinterpret_cast<uint32_t *>(p.Oh + row * HD + lane * V + q) = pack_h2(acc[q] * inv, acc[q + 1] * inv);
+        if (lane == 0) p.lse[row] = L > 0.f ? M + logf(L) : -INFINITY;
+    } else {
+#pragma unroll
+        for (int q = 0; q < V / 4; q++)
+            reinterpret_cast<float4 *>(p.O + row * HD + lane * V)[q] = make_float4(acc[4 * q], acc[4 * q + 1], acc[4 * q + 2], acc[4 * q + 3]);
+        if (lane == 0) {
+            p.M[row] = L > 0.f ? M : -INFINITY;
+            p.L[row] = L;
+        }
+    }
+}
+
 // ---------------------------------------------------------------- append: head norm, rotation, scale, quantised store
 // q, k: y = x * rsqrt(mean(x^2) + eps) * w (no weight: y = x); the first `rot` dims turned in pairs by angle pos * freq;
 // queries leave as f16(y * scale) in the attention calls' layout [set][nkv][gqa * n_tok][hd] (row g * n_tok + t), keys and the

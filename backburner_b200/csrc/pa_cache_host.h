@@ -121,12 +121,12 @@ auto with_prefill(const pa_cuda_cache_plan *p, F &&f) {
 }
 
 template <int HD, bool REPLY>
-cudaError_t launch_cache_merge(const pa_cuda_cache_plan *p, const pa::mrg::Params &mp, cudaStream_t st) {
-    const uint64_t rows = (uint64_t) mp.n_sets * mp.rows_per_set;
-    // 8 warps a row where the rows alone leave SMs idle and a set can have many parts (as launch_merge)
-    if (rows * 8 <= (uint64_t) p->ctx->n_sm * 128 && p->n_parts >= 8 * p->n_sets)
-        return launch_pdl(pa::mrg::merge_kernel<HD, 8, true, REPLY>, dim3((unsigned) rows), 256, 0, st, mp);
-    return launch_pdl(pa::mrg::merge_kernel<HD, 1, true, REPLY>, dim3((unsigned) ((rows + 7) / 8)), 256, 0, st, mp);
+cudaError_t launch_cache_merge(const pa_cuda_cache_plan *p, const pa::pg::MergeParams &mp, cudaStream_t st) {
+    const uint64_t rows = (uint64_t) mp.n_sets * mp.nkv * mp.rows;
+    // 8 warps a row where the rows alone leave SMs idle and a unit can have many parts (as launch_merge)
+    if (rows * 8 <= (uint64_t) p->ctx->n_sm * 128 && p->n_parts >= 8 * p->n_sets * p->n_rt)
+        return launch_pdl(pa::pg::cache_merge_kernel<HD, 8, REPLY>, dim3((unsigned) rows), 256, 0, st, mp);
+    return launch_pdl(pa::pg::cache_merge_kernel<HD, 1, REPLY>, dim3((unsigned) ((rows + 7) / 8)), 256, 0, st, mp);
 }
 
 // O, m, l or Oh, lse: one of the two forms
@@ -211,22 +211,19 @@ int cache_attn(pa_cuda_cache_plan *p, uint32_t layer, const uint16_t *Qs, const 
         e = with_decode(p, [&](auto hd, auto q, auto w) { return launch_decode_paged<hd.value, q.value, w.value>(p, prm, st); });
     }
     if (e != cudaSuccess) return cuda_fail(ctx, e, "cache attention launch");
-    pa::mrg::Params mp{};
+    pa::pg::MergeParams mp{};
     mp.Op = Op;
     mp.Mp = Mp;
     mp.Lp = Lp;
-    mp.c_range = p->d_crange;
-    mp.n_parts = p->n_parts;
-    mp.op_stride = slot_rows * sh.hd;
-    mp.ml_stride = slot_rows;
+    mp.crange = p->d_crange;
+    mp.n_sets = p->n_sets;
+    mp.nkv = sh.nkv;
     mp.rows = sh.rows;
     mp.unit_rows = p->unit_rows;
     mp.n_rt = p->n_rt;
     mp.O = O;
     mp.M = m;
     mp.L = l;
-    mp.rows_per_set = rows_all;
-    mp.n_sets = p->n_sets;
     mp.Oh = Oh;
     mp.lse = lse;
     if (sh.hd == 128) e = Oh ? launch_cache_merge<128, true>(p, mp, st) : launch_cache_merge<128, false>(p, mp, st);

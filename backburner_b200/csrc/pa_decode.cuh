@@ -232,8 +232,7 @@ __global__ void __launch_bounds__(32 * W, min_ctas(HD, W)) decode_kernel(const t
     if constexpr (PAGED) {
         if (s_part.of == 0) return;
         span = pg::span_of<STAGE_KEYS>(p.pg.v, s_part.st, s_part.t0, s_part.t1);
-        pg0 = s_part.begin((uint32_t) span.n);
-        pgn = s_part.end((uint32_t) span.n) - pg0;
+        s_part.share((uint32_t) span.n, pg0, pgn);
     }
 
     auto stages_of = [&](uint32_t jn) -> uint32_t {

@@ -144,13 +144,17 @@ struct Part {
     uint32_t index, of;        // part `index` of the unit's `of` (0: none for this CTA)
     uint32_t t0, t1;           // tokens of the unit's rows
     Set st;
-    // the part's groups of the unit's n (n >= of: at least one)
-    PA_HD uint32_t begin(uint32_t n) const { return (uint32_t) ((uint64_t) index * n / of); }
-    PA_HD uint32_t end(uint32_t n) const { return (uint32_t) ((uint64_t) (index + 1) * n / of); }
+    // the part's groups of the unit's n (n >= of: at least one): the first n % of parts take one more
+    PA_HD void share(uint32_t n, uint32_t &first, uint32_t &count) const {
+        const uint32_t per = n / of, more = n - per * of;
+        first = index * per + (index < more ? index : more);
+        count = per + (index < more);
+    }
 };
 // the tokens of row tile rt (row r: token r % n_tok): all of them when its rows pass the last token
 PA_HD void tokens_of(const Paged &p, uint32_t rt, uint32_t &t0, uint32_t &t1) {
-    const uint32_t T = p.v.n_tok, r0 = rt * p.tile_rows, n = p.rows - r0 < p.tile_rows ? p.rows - r0 : p.tile_rows, a = r0 % T;
+    const uint32_t T = p.v.n_tok, r0 = rt * p.tile_rows, n = p.rows - r0 < p.tile_rows ? p.rows - r0 : p.tile_rows;
+    const uint32_t a = r0 ? r0 % T : 0;
     t0 = a + n > T ? 0u : a;
     t1 = a + n > T ? T - 1 : a + n - 1;
 }
@@ -161,7 +165,7 @@ __device__ __forceinline__ Part find_part(const Paged &p, uint32_t c, bool write
     const uint32_t units = v.n_sets * p.n_rt;
     // unit u, and the cost of its groups
     auto unit = [&](uint32_t u, Part &r) -> uint32_t {
-        r.set = u / p.n_rt;
+        r.set = p.n_rt == 1 ? u : u / p.n_rt;
         r.rt = u - r.set * p.n_rt;
         tokens_of(p, r.rt, r.t0, r.t1);
         r.st = set_of(v, r.set);
@@ -174,8 +178,11 @@ __device__ __forceinline__ Part find_part(const Paged &p, uint32_t c, bool write
 #pragma unroll
     for (int x = 16; x > 0; x >>= 1) total += __shfl_xor_sync(0xffffffffu, total, x);
     const uint32_t least = max(1u, (uint32_t) sqrtf((float) total / (float) (8 * units)) / 4) * 8;
-    uint32_t lo = max(least, (uint32_t) ((total + p.n_parts - 1) / p.n_parts)), hi = lo;
-    if (units > 1) {
+    uint32_t lo, hi;
+    if (units == 1) {   // (below 2^30)
+        lo = hi = max(least, ((uint32_t) total + p.n_parts - 1) / p.n_parts);
+    } else {
+        lo = hi = max(least, (uint32_t) ((total + p.n_parts - 1) / p.n_parts));
         // sum of ceil(cost / per) < total / per + units <= n_parts at hi (n_parts > units, by the plan); 2^30 is past any
         // unit's cost
         hi = max(lo, (uint32_t) min((uint64_t) 1 << 30, (total + (p.n_parts - units) - 1) / (p.n_parts - units)));

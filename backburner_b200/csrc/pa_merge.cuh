@@ -24,10 +24,6 @@ struct Params {
     uint64_t rows_per_set;       // nkv * rows
     uint32_t n_sets;
     int fold;                    // 1: (O, M, L) already hold a partial to fold in
-    uint32_t rows, unit_rows, n_rt;   // UNITS: rows per head; of a unit; units of a set: c_range is by unit, and a slot holds
-                                      // the [nkv][unit_rows] rows of one unit
-    uint16_t *Oh;                // REPLY: f16(O / l) and lse = m + log l instead of O, M, L (normalize_kernel's)
-    float *lse;
 };
 
 // SPLIT warps per output row (1: 8 rows per 256-thread block; 8: one row per block, for calls with few rows and many
@@ -36,30 +32,22 @@ struct Params {
 // memory, and every warp accumulates sum_c w_c O_c, sum_c w_c l_c against that same M, so the warps' sums simply add.
 // Weights are computed 32 parts at a time (one per lane) and broadcast; the O loads of a batch do not depend on one
 // another, and a part with l <= 0 (no keys) gets weight 0 and its O is not used.
-template <int HD, int SPLIT, bool UNITS = false, bool REPLY = false>
+template <int HD, int SPLIT>
 __global__ void __launch_bounds__(256) merge_kernel(const Params p) {
     constexpr int V = HD / 32;          // floats per lane
     constexpr int RPB = 8 / SPLIT;      // rows per block
     __shared__ float s_m[8];
     __shared__ float s_l[8];
     __shared__ __align__(16) float s_acc[SPLIT > 1 ? 8 * HD : 4];
-    pdl_trigger();
-    pdl_wait();   // launched behind the paged attention kernels before they end
     const uint32_t warp = threadIdx.x / 32, lane = threadIdx.x % 32, sw = warp % SPLIT;
     const uint64_t gw = (uint64_t) blockIdx.x * RPB + warp / SPLIT;
     const bool active = gw < (uint64_t) p.n_sets * p.rows_per_set;
     const uint32_t s = active ? (uint32_t) (gw / p.rows_per_set) : 0;
     const uint64_t R = active ? gw % p.rows_per_set : 0;
-    uint32_t u = s;
-    uint64_t rr = (uint64_t) s * p.set_rows + R;
-    if constexpr (UNITS) {
-        const uint32_t h = (uint32_t) R / p.rows, r = (uint32_t) R % p.rows, rt = r / p.unit_rows;
-        u = s * p.n_rt + rt;
-        rr = (uint64_t) h * p.unit_rows + (r - rt * p.unit_rows);
-    }
-    const uint32_t c0 = !active ? 0 : p.c_range ? p.c_range[u] : 0;
-    const uint32_t c1 = !active ? 0 : p.c_range ? p.c_range[u + 1] : p.n_parts;
+    const uint32_t c0 = !active ? 0 : p.c_range ? p.c_range[s] : 0;
+    const uint32_t c1 = !active ? 0 : p.c_range ? p.c_range[s + 1] : p.n_parts;
     const uint64_t orow = (uint64_t) s * p.rows_per_set + R;
+    const uint64_t rr = (uint64_t) s * p.set_rows + R;
 
     // ---- the row maximum over the parts with keys (and the partial already in O, M, L when folding)
     float m_in = -INFINITY, l_in = 0.f;
@@ -148,14 +136,6 @@ __global__ void __launch_bounds__(256) merge_kernel(const Params p) {
         }
     }
     if (!active) return;
-    if constexpr (REPLY) {
-        const float inv = Ls > 0.f ? 1.f / Ls : 0.f;
-#pragma unroll
-        for (int i = 0; i < V; i += 2)
-            *reinterpret_cast<uint32_t *>(p.Oh + orow * HD + lane * V + i) = pack_h2(acc[i] * inv, acc[i + 1] * inv);
-        if (lane == 0) p.lse[orow] = Ls > 0.f ? M + logf(Ls) : -INFINITY;
-        return;
-    }
     float4 *dst = reinterpret_cast<float4 *>(p.O + orow * HD + lane * V);
 #pragma unroll
     for (int i = 0; i < V / 4; i++) dst[i] = make_float4(acc[4 * i], acc[4 * i + 1], acc[4 * i + 2], acc[4 * i + 3]);

@@ -309,10 +309,11 @@ __global__ void __launch_bounds__(32 * cta_warps(NT), 1) prefill_kernel(const __
         }
         __syncthreads();
         if (__shfl_sync(0xffffffffu, s_part.of, 0) == 0) return;
-        const uint32_t n = (uint32_t) pg::span_of<64>(p.pg.v, s_part.st, s_part.t0, s_part.t1).n;
+        uint32_t first, count = 0;
+        if (s_part.of) s_part.share((uint32_t) pg::span_of<64>(p.pg.v, s_part.st, s_part.t0, s_part.t1).n, first, count);
         // (through a shuffle, so that the compiler knows them to be the same in all lanes and keeps the loops uniform)
         rt = __shfl_sync(0xffffffffu, s_part.rt, 0);
-        nblk = __shfl_sync(0xffffffffu, (s_part.end(n) - s_part.begin(n) + B / 64 - 1) / (B / 64), 0);
+        nblk = __shfl_sync(0xffffffffu, (count + B / 64 - 1) / (B / 64), 0);
     } else {
         job = p.jobs[cid / (p.n_rt * p.nkv)];
         nblk = (job.nk + B - 1) / B;
@@ -404,8 +405,7 @@ __global__ void __launch_bounds__(32 * cta_warps(NT), 1) prefill_kernel(const __
         uint32_t pg0 = 0, pgn = 0;   // PAGED: this CTA's groups [pg0, pg0 + pgn) of its unit's span
         if constexpr (PAGED) {
             span = pg::span_of<64>(p.pg.v, s_part.st, s_part.t0, s_part.t1);
-            pg0 = s_part.begin((uint32_t) span.n);
-            pgn = s_part.end((uint32_t) span.n) - pg0;
+            s_part.share((uint32_t) span.n, pg0, pgn);
         }
         uint32_t issued = 0;
         for (uint32_t j = 0; j < nblk; j++) {
