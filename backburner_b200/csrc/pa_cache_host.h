@@ -59,6 +59,12 @@ int check_table(pa_cuda_ctx *ctx, const pa_cuda_cache *c, uint32_t n_sets, uint3
     if (n_sets > 65535) return fail(ctx, PA_CUDA_EUNSUPPORTED, "more than 65,535 sequences");
     return PA_CUDA_OK;
 }
+// whether every pointer is a multiple of n bytes (a misaligned one would fault on the device)
+bool aligned(uintptr_t n, std::initializer_list<const void *> ptrs) {
+    uintptr_t x = 0;
+    for (const void *p : ptrs) x |= (uintptr_t) p;
+    return x % n == 0;
+}
 uint64_t page_mul(uint32_t page_keys) { return ((1ull << 40) + page_keys / 64 - 1) / (page_keys / 64); }
 uint64_t layer_bytes(const pa_cuda_shape &sh, const pa_cuda_cache &c) { return (uint64_t) c.n_pages * c.page_keys * sh.rs; }
 
@@ -66,6 +72,7 @@ uint64_t layer_bytes(const pa_cuda_shape &sh, const pa_cuda_cache &c) { return (
 
 struct pa_cuda_cache_plan {
     pa_cuda_ctx *ctx = nullptr;
+    int device = 0;
     pa_cuda_shape sh{};
     pa_cuda_cache cache{};
     pa_cuda_mask mask{};
@@ -137,7 +144,8 @@ int cache_attn(pa_cuda_cache_plan *p, uint32_t layer, const uint16_t *Qs, const 
     if (layer >= p->cache.n_layers) return fail(ctx, PA_CUDA_EINVAL, "layer out of range");
     if (!Qs || !table || !n_keys) return fail(ctx, PA_CUDA_EINVAL, "null argument");
     if ((p->mask.tree != 0) != (tree != nullptr)) return fail(ctx, PA_CUDA_EINVAL, "a tree plan takes the tree's masks, another plan none");
-    if (((uintptr_t) Qs | (uintptr_t) O | (uintptr_t) Oh) & 15) return fail(ctx, PA_CUDA_EINVAL, "Q and O must be 16-byte aligned");
+    if (!aligned(16, {Qs, O, Oh}) || !aligned(8, {tree}) || !aligned(4, {table, n_keys, q_pos, m, l, lse}))
+        return fail(ctx, PA_CUDA_EINVAL, "misaligned pointer (Q and O to 16 bytes, the others to their elements)");
     DeviceScope dev(ctx->device);
     if (!dev.ok) return fail(ctx, PA_CUDA_ECUDA, "cudaSetDevice");
     cudaStream_t st = pick(ctx, stream);
@@ -346,8 +354,10 @@ int pa_cuda_cache_plan_create(pa_cuda_ctx *ctx, const pa_cuda_shape *shape, cons
         return fail(ctx, PA_CUDA_EUNSUPPORTED, "the int8-domain QK does not cover the paged cache");
     if ((uint64_t) n_sets * shape->nkv * shape->rows > 0x7FFFFFFFull)
         return fail(ctx, PA_CUDA_EUNSUPPORTED, "more than 2^31 - 1 query rows in a call");
-    auto *p = new pa_cuda_cache_plan();
+    auto *p = new (std::nothrow) pa_cuda_cache_plan();
+    if (!p) return fail(ctx, PA_CUDA_ENOMEM, "plan");
     p->ctx = ctx;
+    p->device = ctx->device;
     p->sh = *shape;
     p->cache = *cache;
     p->mask = *mask;
@@ -389,7 +399,7 @@ int pa_cuda_cache_plan_create(pa_cuda_ctx *ctx, const pa_cuda_shape *shape, cons
 const char *pa_cuda_cache_plan_kernel(const pa_cuda_cache_plan *plan) { return plan ? plan->kernel : ""; }
 void pa_cuda_cache_plan_destroy(pa_cuda_cache_plan *plan) {
     if (!plan) return;
-    DeviceScope dev(plan->ctx->device);
+    DeviceScope dev(plan->device);
     if (plan->d_part) cudaFree(plan->d_part);
     if (plan->d_crange) cudaFree(plan->d_crange);
     if (plan->d_maps) cudaFree(plan->d_maps);
@@ -423,7 +433,10 @@ int pa_cuda_cache_append(pa_cuda_ctx *ctx, const pa_cuda_shape *shape, const pa_
         return fail(ctx, PA_CUDA_EUNSUPPORTED, "inputs are f16, bf16 or f32; weights of the inputs' type or f32");
     if (in->rot % 2 || in->rot > shape->hd || (in->rot && !in->freqs))
         return fail(ctx, PA_CUDA_EINVAL, "rot must be even, at most hd, with rot / 2 frequencies");
-    if ((uintptr_t) Qs & 15) return fail(ctx, PA_CUDA_EINVAL, "Q must be 16-byte aligned");
+    const uint64_t size = in->dtype == PA_CUDA_T_F32 ? 4 : 2;
+    if (!aligned(16, {Qs}) || !aligned(8, {in->freqs}) || !aligned(4, {table, start, in->pos}) || !aligned(size, {in->q, in->k, in->v}) ||
+        !aligned(in->w_dtype == PA_CUDA_T_F32 ? 4 : 2, {in->wq, in->wk}))
+        return fail(ctx, PA_CUDA_EINVAL, "misaligned pointer (Q to 16 bytes, the others to their elements)");
     DeviceScope dev(ctx->device);
     if (!dev.ok) return fail(ctx, PA_CUDA_ECUDA, "cudaSetDevice");
     pa::pg::AppendParams a{};
@@ -462,7 +475,6 @@ int pa_cuda_cache_append(pa_cuda_ctx *ctx, const pa_cuda_shape *shape, const pa_
     a.inter = in->interleaved != 0;
     a.w32 = in->w_dtype == PA_CUDA_T_F32;
     // 16-byte loads where every head and the weights start on such a boundary
-    const uint64_t size = in->dtype == PA_CUDA_T_F32 ? 4 : 2;
     uint64_t odd = (uintptr_t) in->q | (uintptr_t) in->k | (uintptr_t) in->v | (uintptr_t) in->wq | (uintptr_t) in->wk;
     for (int64_t x : {in->q_set, in->q_tok, in->k_set, in->k_tok, in->v_set, in->v_tok}) odd |= (uint64_t) x * size;
     const int rot = odd % 16 ? pa::pg::ROT_ANY : a.inter ? pa::pg::ROT_PAIRS : a.rot % 16 ? pa::pg::ROT_ANY : pa::pg::ROT_HALVES;
@@ -487,7 +499,7 @@ int pa_cuda_cache_rows(pa_cuda_ctx *ctx, const pa_cuda_shape *shape, const pa_cu
     if (layer >= cache->n_layers) return fail(ctx, PA_CUDA_EINVAL, "layer out of range");
     if (n_sets == 0 || n_tok == 0) return PA_CUDA_OK;
     if (!table || !first || !K || !V) return fail(ctx, PA_CUDA_EINVAL, "null argument");
-    if (((uintptr_t) K | (uintptr_t) V) & 15) return fail(ctx, PA_CUDA_EINVAL, "K and V must be 16-byte aligned");
+    if (!aligned(16, {K, V}) || !aligned(4, {table, first})) return fail(ctx, PA_CUDA_EINVAL, "misaligned pointer (K and V to 16 bytes, the others to 4)");
     const uint64_t keys = (uint64_t) n_sets * n_tok;
     if (keys > 0x7FFFFFFFull) return fail(ctx, PA_CUDA_EUNSUPPORTED, "too many rows in one call");
     DeviceScope dev(ctx->device);
@@ -523,6 +535,7 @@ int pa_cuda_cache_copy_pages(pa_cuda_ctx *ctx, const pa_cuda_shape *shape, const
     if (rc) return rc;
     if (n == 0) return PA_CUDA_OK;
     if (!src || !dst) return fail(ctx, PA_CUDA_EINVAL, "null argument");
+    if (!aligned(4, {src, dst})) return fail(ctx, PA_CUDA_EINVAL, "misaligned pointer");
     DeviceScope dev(ctx->device);
     if (!dev.ok) return fail(ctx, PA_CUDA_ECUDA, "cudaSetDevice");
     pa::pg::CopyParams a{};
@@ -553,6 +566,7 @@ int pa_cuda_cache_compact(pa_cuda_ctx *ctx, const pa_cuda_shape *shape, const pa
     if (n_sets == 0) return PA_CUDA_OK;
     if (n_tok == 0 || n_tok > pa::pg::COMPACT_MAX) return fail(ctx, PA_CUDA_EUNSUPPORTED, "a path has 1 to 1,024 tokens");
     if (!table || !start || !path || !count) return fail(ctx, PA_CUDA_EINVAL, "null argument");
+    if (!aligned(4, {table, start, path, count, n_keys_out})) return fail(ctx, PA_CUDA_EINVAL, "misaligned pointer");
     DeviceScope dev(ctx->device);
     if (!dev.ok) return fail(ctx, PA_CUDA_ECUDA, "cudaSetDevice");
     pa::pg::CompactParams a{};

@@ -16,6 +16,8 @@
 #include <cstdio>
 #include <cstdlib>
 #include <cstring>
+#include <initializer_list>
+#include <new>
 #include <string>
 #include <type_traits>
 #include <unordered_map>

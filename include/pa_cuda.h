@@ -280,7 +280,8 @@ typedef struct pa_cuda_mask {
 
 typedef struct pa_cuda_cache_plan pa_cuda_cache_plan;
 /* A plan fixes the geometry (shape->rows = GQA group x n_tok rows per KV head, row g * n_tok + t) and owns the workspace
- * of its calls: calls of one plan must not overlap (two streams, two captured graphs replayed at once: two plans).
+ * of its calls: calls of one plan must not overlap (two streams, two captured graphs replayed at once: two plans). The
+ * cache's memory outlives the plan.
  * Reads pa_cuda_set_kernel (0, 1 or 2) as pa_cuda_plan_create does; the int8-domain QK is refused. */
 int pa_cuda_cache_plan_create(pa_cuda_ctx *ctx, const pa_cuda_shape *shape, const pa_cuda_cache *cache, uint32_t n_sets,
                               uint32_t max_pages, const pa_cuda_mask *mask, pa_cuda_cache_plan **out);
@@ -333,7 +334,8 @@ int pa_cuda_cache_copy_pages(pa_cuda_ctx *ctx, const pa_cuda_shape *shape, const
 /* After a verify: the rows of keys start[s] + path[s][i], i < count[s], move to start[s] + i in place, in every layer, K and
  * V; path [n_sets][n_tok] rises strictly (an accepted path of a tree whose tokens follow their parents). n_keys_out[s] =
  * start[s] + count[s] (may be NULL). n_tok <= 1,024, start[s] + n_tok within the table's reach; a set with a bad path, count
- * or page keeps its rows, and n_keys_out[s] = start[s]. Rows behind the kept ones stay as they are. */
+ * or page keeps its rows, and n_keys_out[s] = start[s]. Rows behind the kept ones stay as they are. Sets share no page that
+ * rows move in. */
 int pa_cuda_cache_compact(pa_cuda_ctx *ctx, const pa_cuda_shape *shape, const pa_cuda_cache *cache, uint32_t n_sets,
                           uint32_t n_tok, const int32_t *table, uint32_t max_pages, const int32_t *start, const int32_t *path,
                           const int32_t *count, int32_t *n_keys_out, void *stream);

@@ -289,6 +289,84 @@ def test_partials_of_two_caches_merge_to_the_whole(ctx):
     assert float((got[1] - want[1]).abs().max()) <= 1e-4
 
 
+def test_two_plans_on_two_streams(ctx):
+    import torch
+    sq = Seqs(41, [1500, 700, 30], page=64)
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    plans = [pa.CachePlan(ctx, sq.cache, 3, tok, 5, sq.max_pages) for tok in (1, 9)]
+    Qs = [sq.q(tok, 5) for tok in (1, 9)]
+    torch.cuda.synchronize()
+    outs = [[], []]
+    for _ in range(8):
+        for i in range(2):
+            with torch.cuda.stream(streams[i]):
+                outs[i].append(plans[i].reply(sq.layer, Qs[i], sq.table, sq.n_keys))
+    torch.cuda.synchronize()
+    ctx.status()
+    for i, tok in enumerate((1, 9)):
+        _check(sq, Qs[i], outs[i][0], tok, 5)
+        for o in outs[i][1:]:   # and every call gives the same bits
+            assert torch.equal(o[0], outs[i][0][0]) and torch.equal(o[1], outs[i][0][1])
+        plans[i].close()
+
+
+@pytest.mark.parametrize("kernel", [1, 2])
+def test_a_wait_that_runs_out_is_reported_and_the_next_call_is_right(ctx, kernel):
+    sq = Seqs(43, [300, 80], page=64)
+    ctx.set_kernel(kernel)
+    plan = pa.CachePlan(ctx, sq.cache, 2, 3, 5, sq.max_pages)
+    ctx.set_kernel(0)
+    Qs = sq.q(3, 5)
+    ctx.set_timeout_ns(20_000_000)
+    ctx.set_stall_test(True)
+    try:
+        plan.reply(sq.layer, Qs, sq.table, sq.n_keys)
+        with pytest.raises(pa.PaCudaError) as e:
+            ctx.status()
+        assert e.value.code == api.ETIMEOUT
+    finally:
+        ctx.set_stall_test(False)
+        ctx.set_timeout_ns(2_000_000_000)
+    out = plan.reply(sq.layer, Qs, sq.table, sq.n_keys)
+    ctx.status()
+    _check(sq, Qs, out, 3, 5)
+    plan.close()
+
+
+@pytest.mark.parametrize("kernel", [1, 2])
+def test_pages_past_four_gigabytes(ctx, kernel):
+    """row offsets that pass 32 bits: every call on the last pages of a layer of 4.6 GB"""
+    import torch
+    n_pages = 1040
+    c = pa.Cache(128, 8, pa.Q8_0, 1, n_pages, 4096)
+    assert n_pages * 4096 * c.rs > 1 << 32
+    g = torch.Generator(device="cuda")
+    g.manual_seed(3)
+    i32 = dict(dtype=torch.int32, device="cuda")
+    far, near = torch.tensor([[n_pages - 1]], **i32), torch.tensor([[2]], **i32)
+    x = [torch.randn(1, 300, k, 128, generator=g, device="cuda") for k in (40, 8, 8)]
+    start = torch.tensor([0], **i32)
+    ctx.set_kernel(kernel)
+    plan = pa.CachePlan(ctx, c, 1, 300, 5, 1)
+    ctx.set_kernel(0)
+    out = []
+    for t in (far, near):
+        Qs = pa.cache_append(ctx, c, 0, *x, t, start, scale=128 ** -0.5)
+        out.append((*pa.cache_rows(ctx, c, 0, t, start, 300), *plan.reply(0, Qs, t, torch.tensor([300], **i32))))
+    for a, b in zip(*out):
+        assert torch.equal(a, b) and bool(a.float().abs().max() > 0)
+    path = torch.zeros(1, 300, **i32)   # of 300 tokens every third is kept
+    path[0, :100] = torch.arange(0, 300, 3)
+    for t in (far, near):
+        pa.cache_compact(ctx, c, t, start, path, torch.tensor([100], **i32))
+    a, b = (pa.cache_rows(ctx, c, 0, t, start, 100) for t in (far, near))
+    assert torch.equal(a[0], out[0][0][:, ::3]) and all(torch.equal(u, v) for u, v in zip(a, b))
+    pa.cache_copy_pages(ctx, c, far[0], torch.tensor([5], **i32))
+    ctx.status()
+    assert torch.equal(c.K[0, 5], c.K[0, n_pages - 1]) and torch.equal(c.V[0, 5], c.V[0, n_pages - 1])
+    plan.close()
+
+
 # ------------------------------------------------------------------------------------------------- append
 def _turned(torch, y, pos, freqs, inter):
     """float64 [S][T][H][hd], the first 2 * len(freqs) dims turned"""
@@ -528,6 +606,11 @@ def test_refusals(ctx):
     no(U, P, ctx, c, 1, 65, 5, 4, tree=True)
     no(U, P, ctx, c, 1, 9, 5, 4, 8, tree=True)
     no(U, P, ctx, c, 65536, 1, 5, 4)
+    ctx.set_kernel(3)
+    no(U, P, ctx, c, 1, 1, 5, 4)
+    ctx.set_kernel(2)
+    no(U, P, ctx, pa.Cache(128, 8, pa.F16, 1, 4, 64), 1, 1, 5, 4)
+    ctx.set_kernel(0)
     no(U, P, ctx, c, 65535, 1 << 14, 1, 4)
     no(U, P, ctx, pa.Cache(128, 8, pa.Q8_0, 1, 4, 96), 1, 1, 5, 4)
     no(U, P, ctx, pa.Cache(64, 8, pa.Q8_0, 1, 4, 64), 1, 1, 5, 4)
@@ -549,6 +632,10 @@ def test_refusals(ctx):
     flat = torch.zeros(5 * 8 * 128 + 1, dtype=torch.float16, device="cuda")[1:]
     no(I, plan.reply, 0, flat.view(1, 8, 5, 128), t, n)   # 16-byte alignment
     no(I, plan.run, 0, Q, t, n, out=(Q, Q, Q))
+    L, q, i, o, z = pa.lib(), Q.data_ptr(), t.data_ptr(), torch.zeros(1, 8, 5, device="cuda").data_ptr(), n.data_ptr()
+    for a in ((q, i + 2, z, 0, 0, q, o), (q, i, z + 1, 0, 0, q, o), (q, i, z, z + 2, 0, q, o), (q, i, z, 0, 0, q + 8, o),
+              (q, i, z, 0, 0, q, o + 2), (0, i, z, 0, 0, q, o), (q, 0, z, 0, 0, q, o), (q, i, z, 0, 0, 0, o)):
+        assert L.pa_cuda_cache_attn_reply(plan._h, 0, *a, None) == api.EINVAL
     x = [torch.zeros(1, 1, k, 128, device="cuda") for k in (40, 8, 8)]
     no(I, pa.cache_append, ctx, c, 0, x[0][..., :64], x[1], x[2], t, n)
     no(I, pa.cache_append, ctx, c, 0, x[0][:, :, :39], x[1], x[2], t, n)
