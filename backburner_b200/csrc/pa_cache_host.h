@@ -22,19 +22,27 @@ struct DeviceScope {
 // A launch that may start its prologue while the stream's previous kernel ends (every kernel launched so waits for it with
 // pdl_wait before it reads or writes global memory)
 template <class... A>
-cudaError_t launch_pdl(void (*kernel)(A...), dim3 grid, uint32_t threads, size_t smem, cudaStream_t st, const A &...args) {
+cudaError_t launch_pdl_cluster(uint32_t cluster, void (*kernel)(A...), dim3 grid, uint32_t threads, size_t smem, cudaStream_t st,
+                               const A &...args) {
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = grid;
     cfg.blockDim = dim3(threads);
     cfg.dynamicSmemBytes = smem;
     cfg.stream = st;
-    cudaLaunchAttribute attr[1];
+    cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = cluster;
+    attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
     cfg.attrs = attr;
-    cfg.numAttrs = 1;
+    cfg.numAttrs = cluster > 1 ? 2 : 1;
     const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, args...);
     return e != cudaSuccess ? e : cudaGetLastError();
+}
+template <class... A>
+cudaError_t launch_pdl(void (*kernel)(A...), dim3 grid, uint32_t threads, size_t smem, cudaStream_t st, const A &...args) {
+    return launch_pdl_cluster(1, kernel, grid, threads, smem, st, args...);
 }
 
 constexpr uint64_t kCacheMaxKeys = 1ull << 30;   // keys a page table reaches: key indexes and sums of them stay in 32 bits
@@ -78,8 +86,8 @@ struct pa_cuda_cache_plan {
     pa_cuda_mask mask{};
     uint32_t n_sets = 0, max_pages = 0;
     pa_cuda_plan d;                  // launch shape of the split-K kernel
-    bool tc = false;                 // the tcgen05 kernel
-    int nt = 1;                      // ... with nt tiles of 128 rows per CTA, n_rt groups of them per head
+    bool tc = false, pair = false;   // a tcgen05 kernel; on CTA pairs
+    int nt = 1;                      // ... with nt tiles of 128 rows per CTA
     uint32_t n_rt = 1, unit_rows = 1;   // units of a set (row tiles; the split-K kernel: one) and their rows
     uint32_t n_parts = 1;            // CTAs along the keys = slots of partials (pa_mask.cuh)
     CUtensorMap *d_maps = nullptr;   // K and V rows of the whole cache
@@ -101,6 +109,12 @@ cudaError_t launch_prefill_paged(const pa_cuda_cache_plan *p, const CUtensorMap 
     constexpr int smem = pa::pre::Smem<Q, NT, D>::TOTAL + 1024;
     return launch_pdl(pa::pre::prefill_kernel<Q, NT, D, true>, dim3(p->n_parts * p->sh.nkv), 32 * pa::pre::cta_warps(NT), smem,
                       st, tq, prm);
+}
+template <int Q, int NT, int D>
+cudaError_t launch_pair_paged(const pa_cuda_cache_plan *p, const CUtensorMap &tq, const pa::pre::PagedParams &prm, cudaStream_t st) {
+    constexpr int smem = pa::pre::PairSmem<Q, NT, D>::TOTAL + 1024;
+    return launch_pdl_cluster(2, pa::pre::prefill_pair_kernel<Q, NT, D, true>, dim3(2 * p->n_parts * p->sh.nkv),
+                              32 * (4 + 4 * NT + pa::pre::pair_dq_warps(D)), smem, st, tq, prm);
 }
 // f(kernel instance's constants) for the plan's kernel; f is a generic lambda
 template <int HD, int W, class F>
@@ -172,7 +186,7 @@ int cache_attn(pa_cuda_cache_plan *p, uint32_t layer, const uint16_t *Qs, const 
     pg.n_parts = p->n_parts;
     pg.rows = sh.rows;
     pg.tile_rows = p->unit_rows;
-    pg.half_rows = p->tc && p->nt == 2 ? (uint32_t) pa::pre::BM : 0u;
+    pg.half_rows = p->tc && !p->pair && p->nt == 2 ? (uint32_t) pa::pre::BM : 0u;
     pg.n_rt = p->n_rt;
     pg.crange = p->d_crange;
     cudaError_t e;
@@ -194,7 +208,9 @@ int cache_attn(pa_cuda_cache_plan *p, uint32_t layer, const uint16_t *Qs, const 
         prm.n_rt = 1;
         prm.timeout_ns = ctx->timeout_ns;
         prm.stall = ctx->stall_test;
-        e = with_prefill(p, [&](auto q, auto nt, auto d) { return launch_prefill_paged<q.value, nt.value, d.value>(p, tq, prm, st); });
+        e = with_prefill(p, [&](auto q, auto nt, auto d) {
+            return p->pair ? launch_pair_paged<q.value, nt.value, d.value>(p, tq, prm, st) : launch_prefill_paged<q.value, nt.value, d.value>(p, tq, prm, st);
+        });
     } else {
         pa::dec::PagedParams prm{};
         prm.pg = pg;
@@ -250,9 +266,9 @@ int shape_cache_plan(pa_cuda_cache_plan *p) {
     int rc = plan_decode_shape(ctx, &p->d);
     if (rc) return rc;
     const bool tc_ok = sh.quant != PA_CUDA_F16 && encode_fn() != nullptr;
-    if (ctx->kernel_choice > 2 || (ctx->kernel_choice == 2 && !tc_ok))
-        return fail(ctx, PA_CUDA_EUNSUPPORTED, "the paged cache takes the split-K kernel or, over quantised rows, the single-CTA tcgen05 kernel");
-    p->tc = tc_ok && (ctx->kernel_choice == 2 || (ctx->kernel_choice == 0 && sh.rows >= (sh.hd == 128 ? kPrefillMinRows128 : kPrefillMinRows256)));
+    if (ctx->kernel_choice >= 2 && !tc_ok) return fail(ctx, PA_CUDA_EUNSUPPORTED, "tcgen05 kernels need quantised (Q8_0 / Q4_0) rows");
+    p->tc = tc_ok && (ctx->kernel_choice >= 2 || (ctx->kernel_choice == 0 && sh.rows >= (sh.hd == 128 ? kPrefillMinRows128 : kPrefillMinRows256)));
+    p->pair = p->tc && (ctx->kernel_choice == 3 || (ctx->kernel_choice == 0 && sh.rows >= (sh.hd == 256 ? kSingle256MaxRows + 1 : kPairMinRows)));
     // groups of keys that one set can have to read
     const uint32_t G = p->tc ? 64 : 16;
     const uint64_t cap = (uint64_t) p->max_pages * p->cache.page_keys;
@@ -261,25 +277,29 @@ int shape_cache_plan(pa_cuda_cache_plan *p) {
         groups = std::min(groups, ((uint64_t) p->mask.window + p->mask.n_tok + G - 1) / G + 1 + std::min<uint64_t>((p->mask.sinks + (uint64_t) G - 1) / G, groups));
     uint64_t parts, units;
     if (p->tc) {
-        p->nt = sh.hd == 128 && sh.rows > (uint32_t) pa::pre::BM ? 2 : 1;
-        p->unit_rows = (uint32_t) (pa::pre::BM * p->nt);
+        const uint32_t tile = (uint32_t) pa::pre::BM * (p->pair ? 2u : 1u), ctas = p->pair ? 2 : 1;
+        p->nt = sh.hd == 128 && sh.rows > tile ? 2 : 1;
+        p->unit_rows = tile * p->nt;
         p->n_rt = (sh.rows + p->unit_rows - 1) / p->unit_rows;
         units = (uint64_t) p->n_sets * p->n_rt;
-        p->kernel = p->nt == 2 ? "pa::pre::prefill_kernel<2 tiles, paged>" : "pa::pre::prefill_kernel<1 tile, paged>";
+        static const char *names[2][2] = {{"pa::pre::prefill_kernel<1 tile, paged>", "pa::pre::prefill_kernel<2 tiles, paged>"},
+                                          {"pa::pre::prefill_pair_kernel<1 tile, paged>", "pa::pre::prefill_pair_kernel<2 tiles, paged>"}};
+        p->kernel = names[p->pair][p->nt - 1];
+        const uint64_t y = (uint64_t) sh.nkv * ctas;   // CTAs of a part
         // the count that minimises waves x (groups of a part + a CTA's overhead), all units as long as they can be; parts
         // that are left over by equal units' remainders are counted out
         const uint64_t spare = units > 1 ? units : 0;
         uint64_t best = ~0ull;
         parts = units;
-        for (uint64_t c = std::max<uint64_t>(1, units); c <= spare + std::max<uint64_t>(1, 8ull * ctx->n_sm / sh.nkv); c++) {
+        for (uint64_t c = std::max<uint64_t>(1, units); c <= spare + std::max<uint64_t>(1, 8ull * ctx->n_sm / y); c++) {
             const uint64_t per = (groups + c / units - 1) / (c / units);
-            const uint64_t cost = ((c / units * units * sh.nkv + ctx->n_sm - 1) / ctx->n_sm) * (per + kGroups64Overhead);
+            const uint64_t cost = ((c / units * units * y + ctx->n_sm - 1) / ctx->n_sm) * (per + kGroups64Overhead);
             if (cost < best) { best = cost; parts = c; }
         }
         // as many as the waves hold anyway (units differ in length)
-        const uint64_t waves = (parts * sh.nkv + ctx->n_sm - 1) / ctx->n_sm;
-        parts = std::max(parts, waves * ctx->n_sm / sh.nkv);
-        if (2 * units * sh.nkv + parts * sh.nkv > 0x7FFFFFFFull) return fail(ctx, PA_CUDA_EUNSUPPORTED, "too many rows and sets in one call");
+        const uint64_t waves = (parts * y + ctx->n_sm - 1) / ctx->n_sm;
+        parts = std::max(parts, waves * ctx->n_sm / y);
+        if ((2 * units + parts) * y > 0x7FFFFFFFull) return fail(ctx, PA_CUDA_EUNSUPPORTED, "too many rows and sets in one call");
     } else {
         if (p->d.grid_y > 65535) return fail(ctx, PA_CUDA_EUNSUPPORTED, "too many head/row groups");
         p->kernel = "pa::dec::decode_kernel<paged>";
@@ -375,7 +395,8 @@ int pa_cuda_cache_plan_create(pa_cuda_ctx *ctx, const pa_cuda_shape *shape, cons
         const uint32_t rows = cache->n_layers * cache->n_pages * cache->page_keys;
         const uint32_t raw = (uint32_t) pa::pre::raw_row_bytes((int) shape->quant, (int) shape->hd);
         CUtensorMap maps[2];
-        if (!map_rows(&maps[0], cache->k, shape->rs, rows, raw, pa::pre::BN) || !map_rows(&maps[1], cache->v, shape->rs, rows, raw, pa::pre::BN)) {
+        // a CTA of a pair loads half of each block's K rows and all of its V rows
+        if (!map_rows(&maps[0], cache->k, shape->rs, rows, raw, p->pair ? pa::pre::BN / 2 : pa::pre::BN) || !map_rows(&maps[1], cache->v, shape->rs, rows, raw, pa::pre::BN)) {
             pa_cuda_cache_plan_destroy(p);
             return fail(ctx, PA_CUDA_ECUDA, "cuTensorMapEncodeTiled (K/V rows) failed");
         }
@@ -383,6 +404,11 @@ int pa_cuda_cache_plan_create(pa_cuda_ctx *ctx, const pa_cuda_shape *shape, cons
             e = cudaMemcpy(p->d_maps, maps, sizeof maps, cudaMemcpyHostToDevice);
         if (e == cudaSuccess)
             e = with_prefill(p, [&](auto q, auto nt, auto d) {
+                if (p->pair) {
+                    constexpr int smem = pa::pre::PairSmem<q.value, nt.value, d.value>::TOTAL + 1024;
+                    return cudaFuncSetAttribute(pa::pre::prefill_pair_kernel<q.value, nt.value, d.value, true>,
+                                                cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+                }
                 constexpr int smem = pa::pre::Smem<q.value, nt.value, d.value>::TOTAL + 1024;
                 return cudaFuncSetAttribute(pa::pre::prefill_kernel<q.value, nt.value, d.value, true>,
                                             cudaFuncAttributeMaxDynamicSharedMemorySize, smem);

@@ -282,7 +282,7 @@ __global__ void __launch_bounds__(32 * cta_warps(NT), 1) prefill_kernel(const __
     const uint32_t h = PAGED ? cid % p.nkv : (cid / p.n_rt) % p.nkv;
     const uint32_t warp = threadIdx.x / 32, lane = threadIdx.x % 32;
     uint32_t rt = cid % p.n_rt;
-    dec::Job job;
+    dec::Job job{};
     uint32_t nblk = 0;
     __shared__ pg::Part s_part;
     __shared__ pg::Tile s_tile;

@@ -154,9 +154,10 @@ __host__ __device__ __forceinline__ uint32_t dq_chunk(uint32_t ql, uint32_t key,
     return ((4 * (ql % 2) + cc) ^ (key % 8)) * 16;
 }
 
-template <int QUANT, int NT, int D>
+// PAGED: as in pa_prefill.cuh (a block is one group of 64 keys); both CTAs work on the unit part that CTA 0 found.
+template <int QUANT, int NT, int D, bool PAGED = false>
 __global__ void __launch_bounds__(32 * (4 + 4 * NT + pair_dq_warps(D)), 1) prefill_pair_kernel(const __grid_constant__ CUtensorMap tq,
-                                                                            const Params p) {
+                                                                            const typename ParamsOf<PAGED>::type p) {
     using L = PairSmem<QUANT, NT, D>;
     static_assert((D == 128 && (NT == 1 || NT == 2)) || (D == 256 && NT == 1), "TMEM holds NT x (128 + D) columns");
     constexpr int RAWB = L::RAWB, KH = L::KH, KVB = L::KVB, TS = L::TS;
@@ -187,15 +188,34 @@ __global__ void __launch_bounds__(32 * (4 + 4 * NT + pair_dq_warps(D)), 1) prefi
     const uint32_t cr = cluster_rank();
     // cluster order (a 1-D grid of CTA pairs): row-tile group fastest, then KV head, then job, so the clusters that read
     // the same K/V blocks (all row groups and heads of one chunk of keys) run at the same time and share them through L2
+    // (PAGED: KV head, then part)
     const uint32_t cid = blockIdx.x / 2;
-    const uint32_t rt = cid % p.n_rt, h = (cid / p.n_rt) % p.nkv;
-    const dec::Job job = p.jobs[cid / (p.n_rt * p.nkv)];
+    const uint32_t h = PAGED ? cid % p.nkv : (cid / p.n_rt) % p.nkv;
     const uint32_t warp = threadIdx.x / 32, lane = threadIdx.x % 32;
-    const uint32_t nblk = (job.nk + BN - 1) / BN;
+    uint32_t rt = cid % p.n_rt;
+    dec::Job job{};
+    uint32_t nblk = 0;
+    // PAGED: what the pair works on, and the words of each group of keys (see pa_prefill.cuh)
+    constexpr uint32_t NO_GROUP = 0xFFFFFFFFu;
+    __shared__ pg::Part s_part;
+    __shared__ pg::Tile s_tile;
+    __shared__ uint32_t s_group[64], s_grow[64];
+    __shared__ uint64_t s_live[64];
+    __shared__ pg::Row s_row[PAGED ? NT * BM : 1];
+    if constexpr (PAGED) {
+        pdl_trigger();
+        pdl_wait();
+        if (warp == 2 && cr == 0) {
+            const pg::Part f = pg::find_part<64>(p.pg, cid / p.nkv, cid == 0, lane);
+            if (lane == 0) s_part = f;
+        }
+    } else {
+        job = p.jobs[cid / (p.n_rt * p.nkv)];
+        nblk = (job.nk + BN - 1) / BN;
+    }
     const uint32_t hbyte = h * (uint32_t) p.hb;
     const int hx = (int) (hbyte & ~15u);
     const uint32_t hoff = hbyte & 15u;
-    const uint32_t row0 = rt * NT * 2 * BM;       // first query row of this pair (within the head)
     const uint64_t tmo = p.timeout_ns;
     bool ok = true;
     // CTA 0's barrier at the same offset as `b`, as a shared::cluster address (arrivals of both CTAs go there)
@@ -229,8 +249,25 @@ __global__ void __launch_bounds__(32 * (4 + 4 * NT + pair_dq_warps(D)), 1) prefi
     // of a call that already failed (uniform, before TMEM is allocated), and neither exits before both have read it
     cluster_sync();
     const uint32_t skip = ld_cluster_u32(mapa(smem_u32((const void *) abort_flag), 0));
+    if constexpr (PAGED) {   // CTA 1 takes CTA 0's part, so that both take every branch alike
+        static_assert(sizeof(pg::Part) % 4 == 0 && sizeof(pg::Part) <= 128, "one word a lane");
+        if (cr == 1 && threadIdx.x < sizeof(pg::Part) / 4)
+            reinterpret_cast<uint32_t *>(&s_part)[threadIdx.x] = ld_cluster_u32(mapa(smem_u32(&s_part) + 4 * threadIdx.x, 0));
+    }
     cluster_sync();
     if (skip) return;
+    if constexpr (PAGED) {
+        if (__shfl_sync(0xffffffffu, s_part.of, 0) == 0) return;
+        uint32_t first, count;
+        s_part.share((uint32_t) pg::span_of<64>(p.pg.v, s_part.st, s_part.t0, s_part.t1).n, first, count);
+        rt = __shfl_sync(0xffffffffu, s_part.rt, 0);
+        nblk = __shfl_sync(0xffffffffu, count, 0);
+        if (warp == 2) {
+            const pg::Tile tl = pg::tile_of(p.pg.v, s_part.st, s_part.set, s_part.t0, s_part.t1, lane);
+            if (lane == 0) s_tile = tl;
+        }
+    }
+    const uint32_t row0 = rt * NT * 2 * BM;       // first query row of this pair (within the head)
     if (warp == 1) {   // TMEM: per pair tile S 64 + P 2 x 32 + O D columns, the same columns in both CTAs
         asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)),
                      "r"(L::TMEM_COLS)
@@ -269,22 +306,50 @@ __global__ void __launch_bounds__(32 * (4 + 4 * NT + pair_dq_warps(D)), 1) prefi
       if (warp == 0) {
         // ------------------------------------------------ TMA producer (each CTA its own operands)
         if (lane == 0) {
-            const int qrow = (int) (((uint64_t) job.set * p.nkv + h) * p.rows + row0 + cr * BM);
+            const int qrow = (int) (((uint64_t) (PAGED ? s_part.set : job.set) * p.nkv + h) * p.rows + row0 + cr * BM);
             mbar_arrive_expect_tx(q_full, NT * BM * D * 2);
             for (int t = 0; t < NT; t++)
                 for (int c = 0; c < D / 64; c++)
                     tma_2d(smem + L::Q + t * BM * D * 2 + c * BM * 128, &tq, c * 64, qrow + t * 2 * BM, q_full);
-            const CUtensorMap *km = p.kv_maps + 2 * job.seg, *vm = km + 1;
-            uint32_t issued = 0;
-            for (uint32_t j = 0; j < nblk; j++) {
-                const uint32_t st = j % NS;
-                if (j >= NS && !wait(&raw_empty[st], ((j / NS) - 1) & 1)) break;
-                mbar_arrive_expect_tx(&raw_full[st], (KH + BN) * RAWB);
-                uint8_t *dst = smem + L::RAW + st * L::RAW_STAGE;
-                tma_2d(dst, km, hx / 2, (int) (job.key0 + j * BN + cr * KH), &raw_full[st]);
-                tma_2d(dst + L::RAW_V, vm, hx / 2, (int) (job.key0 + j * BN), &raw_full[st]);
-                issued = j + 1;
+        }
+        const CUtensorMap *km = p.kv_maps + (PAGED ? 0 : 2 * job.seg), *vm = km + 1;
+        pg::Span span{};
+        uint32_t pg0 = 0;   // PAGED: this pair's first group of its unit's span
+        if constexpr (PAGED) {
+            uint32_t count;
+            span = pg::span_of<64>(p.pg.v, s_part.st, s_part.t0, s_part.t1);
+            s_part.share((uint32_t) span.n, pg0, count);
+        }
+        uint32_t issued = 0;
+        for (uint32_t j = 0; j < nblk; j++) {
+            const uint32_t st = j % NS;
+            if constexpr (PAGED) {
+                if (j % 32 == 0) {
+                    const uint32_t g = j + lane;
+                    const int k0 = span.group((int) (pg0 + g)) * BN;
+                    const bool some = g < nblk, full = some && s_tile.full(k0, BN);
+                    s_grow[g % 64] = some ? p.pg.row0 + pg::row_at(p.pg.v, s_part.set, (uint32_t) k0) : 0u;
+                    s_group[g % 64] = !some ? NO_GROUP : full ? (uint32_t) k0 : (uint32_t) k0 | 0x80000000u;
+                    if (!full) s_live[g % 64] = some ? pg::vis64(s_tile.any, k0) : 0ull;
+                    __syncwarp();
+                }
             }
+            if (lane == 0) {
+                if (j >= NS) wait(&raw_empty[st], ((j / NS) - 1) & 1);
+                if (ok) {
+                    mbar_arrive_expect_tx(&raw_full[st], (KH + BN) * RAWB);
+                    uint8_t *dst = smem + L::RAW + st * L::RAW_STAGE;
+                    int key;
+                    if constexpr (PAGED) key = (int) s_grow[j % 64];
+                    else key = (int) (job.key0 + j * BN);
+                    tma_2d(dst, km, hx / 2, key + (int) cr * KH, &raw_full[st]);
+                    tma_2d(dst + L::RAW_V, vm, hx / 2, key, &raw_full[st]);
+                    issued = j + 1;
+                }
+            }
+            if (!__shfl_sync(0xffffffffu, ok, 0)) break;
+        }
+        if (lane == 0) {
             if (!ok) {
                 const uint64_t drain = tmo > dec::DRAIN_NS ? tmo : dec::DRAIN_NS;
                 if (!mbar_wait_bounded(q_full, 0, drain, nullptr)) atomicCAS(p.status, ST_OK, ST_TIMEOUT_DRAIN);
@@ -365,6 +430,7 @@ __global__ void __launch_bounds__(32 * (4 + 4 * NT + pair_dq_warps(D)), 1) prefi
         const bool pad = NT == 1 && row0 + t * 2 * BM + cr * BM + wq * 32 >= p.rows;   // (NT = 1: registers, as there)
         float m_used = -INFINITY, l = 0.f;
         float m_row = -INFINITY;   // the row's exact maximum (log2 units); O and l are reported against it
+        if constexpr (PAGED) s_row[t * BM + r] = pg::row_of(p.pg.v, s_part.st, s_part.set, (row0 + t * 2 * BM + cr * BM + r) % p.pg.v.n_tok);
         for (uint32_t j = 0; j < nblk; j++) {
             const uint32_t b = j & 1;
             if (!wait(&s_full[t], j & 1)) break;
@@ -386,11 +452,24 @@ __global__ void __launch_bounds__(32 * (4 + 4 * NT + pair_dq_warps(D)), 1) prefi
             tc_fence_before();
             __syncwarp();
             if (lane == 0) mbar_arrive_cl(lead(&s_empty[t]));
+            if constexpr (PAGED) {
+                const uint32_t group = *(volatile uint32_t *) &s_group[j % 64];
+                if ((int) group < 0) {
+                    const uint64_t see = pg::vis64(s_row[t * BM + r], (int) (group & 0x7FFFFFFFu));
+                    const uint32_t lo = (uint32_t) see, hi = (uint32_t) (see >> 32);
+#pragma unroll
+                    for (int i = 0; i < 32; i++) {
+                        if (!(lo >> i & 1u)) s[i] = -INFINITY;
+                        if (!(hi >> i & 1u)) s[32 + i] = -INFINITY;
+                    }
+                }
+            } else {
             const int nvalid = (int) (job.nk - j * BN);
             if (nvalid < BN) {
 #pragma unroll
                 for (int i = 0; i < BN; i++)
                     if (i >= nvalid) s[i] = -INFINITY;
+            }
             }
             float mx = s[0];
 #pragma unroll
@@ -400,7 +479,7 @@ __global__ void __launch_bounds__(32 * (4 + 4 * NT + pair_dq_warps(D)), 1) prefi
             m_row = fmaxf(m_row, mx);
             float alpha = 1.f;
             bool rescale = false;
-            if (j == 0) m_used = mx;
+            if (j == 0) m_used = PAGED ? fmaxf(mx, M_EMPTY) : mx;   // PAGED: the row may see nothing of the block
             else if (mx > m_used + 8.f) {
                 alpha = ex2(m_used - mx);
                 m_used = mx;
@@ -413,9 +492,10 @@ __global__ void __launch_bounds__(32 * (4 + 4 * NT + pair_dq_warps(D)), 1) prefi
             for (int i = 0; i < 32; i++) {
                 float t0, t1;
                 unpack_f2(fma_f2(pack_f2(s[2 * i], s[2 * i + 1]), l2e2, nm2), t0, t1);
-                // every 4th pair on the FMA pipe, the rest on MUFU (measured: +3-5% over MUFU alone; every 2nd: -2%)
+                // every 4th pair on the FMA pipe, the rest on MUFU (measured: +3-5% over MUFU alone; every 2nd: -2%). PAGED:
+                // MUFU, since a row's lse is a result there and the polynomial is off by up to 7.5e-5
                 float p0, p1;
-                if (i % 4 == 3) ex2_pair_fma(t0, t1, p0, p1);
+                if (!PAGED && i % 4 == 3) ex2_pair_fma(t0, t1, p0, p1);
                 else { p0 = ex2(t0); p1 = ex2(t1); }
                 const uint64_t pp = pack_f2(p0, p1);
                 acc = add_f2(acc, pp);
@@ -452,7 +532,12 @@ __global__ void __launch_bounds__(32 * (4 + 4 * NT + pair_dq_warps(D)), 1) prefi
         if (ok && !pad && nblk > 0 && wait(&o_ready[t], 0)) {
             tc_fence_after();
             const uint32_t row = row0 + t * 2 * BM + cr * BM + r;
-            const uint64_t orow = ((uint64_t) job.slot * p.nkv + h) * p.rows + row;
+            // PAGED: a slot holds one unit's rows
+            const uint64_t orow = PAGED ? ((uint64_t) (cid / p.nkv) * p.nkv + h) * (NT * 2 * BM) + (row - row0)
+                                        : ((uint64_t) job.slot * p.nkv + h) * p.rows + row;
+            if constexpr (PAGED) {   // a padding token's row is empty, whatever its scores were
+                if (pg::is_padding(p.pg.v, s_part.set, row % p.pg.v.n_tok)) l = 0.f;
+            }
             const float fix = m_row > -INFINITY ? ex2(m_used - m_row) : 1.f;
 #pragma unroll
             for (int q = 0; q < D / 32; q++) {
@@ -549,6 +634,19 @@ __global__ void __launch_bounds__(32 * (4 + 4 * NT + pair_dq_warps(D)), 1) prefi
                     sts128(kbase + (((c0 + 3) ^ (key % 8)) * 16), hi[4], hi[5], hi[6], hi[7]);
                 }
               }
+                if constexpr (PAGED) {
+                    if (kv == 1 && (int) *(volatile uint32_t *) &s_group[j % 64] < 0) {   // V rows that no row sees: cleared
+#pragma unroll 1
+                        for (int ps = 0; ps < NPASS; ps++) {
+                            uint32_t ql, qb, key;
+                            dq_item<D, NDQ>(1, ps, dw, lane, cr, ql, qb, key);
+                            if (s_live[j % 64] >> key & 1ull) continue;
+                            const uint32_t kb = sbase + L::V + b * L::V_BUF + dq_row(1, ql, key);
+#pragma unroll 1
+                            for (uint32_t cc = 0; cc < 4; cc++) sts128(kb + dq_chunk(ql, key, cc), 0u, 0u, 0u, 0u);
+                        }
+                    }
+                }
                 fence_proxy_async();
                 __syncwarp();
                 if (lane == 0) mbar_arrive_cl(lead(kv == 0 ? &k_full[b] : &v_full[b]));

@@ -282,7 +282,7 @@ typedef struct pa_cuda_cache_plan pa_cuda_cache_plan;
 /* A plan fixes the geometry (shape->rows = GQA group x n_tok rows per KV head, row g * n_tok + t) and owns the workspace
  * of its calls: calls of one plan must not overlap (two streams, two captured graphs replayed at once: two plans). The
  * cache's memory outlives the plan.
- * Reads pa_cuda_set_kernel (0, 1 or 2) as pa_cuda_plan_create does; the int8-domain QK is refused. */
+ * Reads pa_cuda_set_kernel as pa_cuda_plan_create does; the int8-domain QK is refused. */
 int pa_cuda_cache_plan_create(pa_cuda_ctx *ctx, const pa_cuda_shape *shape, const pa_cuda_cache *cache, uint32_t n_sets,
                               uint32_t max_pages, const pa_cuda_mask *mask, pa_cuda_cache_plan **out);
 /* name of the plan's attention kernel (static storage) */

@@ -170,7 +170,7 @@ def _run(ctx, sq, tok, gqa, kernel, window=0, sinks=0, q_pos=None, bits=None):
     plan.close()
 
 
-KERNELS = [0, 1, 2]
+KERNELS = [0, 1, 2, 3]
 LENS = [0, 1, 15, 16, 17, 63, 64, 65, 127, 129, 500, 1031]
 
 
@@ -179,7 +179,7 @@ LENS = [0, 1, 15, 16, 17, 63, 64, 65, 127, 129, 500, 1031]
 @pytest.mark.parametrize("hd,nkv,gqa,tok", [(128, 8, 5, 1), (256, 4, 6, 1), (128, 4, 3, 5), (256, 8, 4, 12), (128, 2, 7, 40)])
 @pytest.mark.parametrize("window,sinks", [(0, 0), (1, 0), (64, 4), (100, 65), (700, 17)])
 def test_window(ctx, kernel, quant, hd, nkv, gqa, tok, window, sinks):
-    if kernel == 2 and quant == pa.F16:
+    if kernel >= 2 and quant == pa.F16:
         pytest.skip("f16 rows run on the split-K kernel")
     sq = Seqs(11 * tok + window, LENS, hd, nkv, quant, 64 if hd == 128 else 128)
     _run(ctx, sq, tok, gqa, kernel, window, sinks)
@@ -190,7 +190,7 @@ def test_window(ctx, kernel, quant, hd, nkv, gqa, tok, window, sinks):
 @pytest.mark.parametrize("hd,nkv,gqa,tok", [(128, 8, 5, 1), (256, 4, 6, 7), (128, 2, 8, 33), (128, 4, 1, 64), (256, 8, 1, 3)])
 @pytest.mark.parametrize("window,sinks", [(0, 0), (64, 70)])
 def test_tree(ctx, kernel, quant, hd, nkv, gqa, tok, window, sinks):
-    if kernel == 2 and quant == pa.F16:
+    if kernel >= 2 and quant == pa.F16:
         pytest.skip("f16 rows run on the split-K kernel")
     sq = Seqs(13 * tok + hd, LENS, hd, nkv, quant, 64 if hd == 128 else 192)
     _run(ctx, sq, tok, gqa, kernel, window, sinks, bits=_tree(np.random.default_rng(tok), len(LENS), tok, 0.2))
@@ -207,7 +207,7 @@ def test_positions_of_the_queries(ctx, kernel, bits, window, sinks):
     _run(ctx, sq, tok, 5, kernel, window, sinks, q_pos, _tree(np.random.default_rng(1), 9, tok, 0.1) if bits else None)
 
 
-@pytest.mark.parametrize("kernel,quant", [(0, pa.Q8_0), (1, pa.Q4_0), (2, pa.Q8_0)])
+@pytest.mark.parametrize("kernel,quant", [(0, pa.Q8_0), (1, pa.Q4_0), (2, pa.Q8_0), (3, pa.Q8_0)])
 def test_many_ragged_sequences(ctx, kernel, quant):
     """more units than a warp has lanes: their parts are found in rounds, and every length keeps its own"""
     rng = np.random.default_rng(5)
@@ -216,11 +216,12 @@ def test_many_ragged_sequences(ctx, kernel, quant):
     _run(ctx, sq, 30, 9, kernel, 50, 5)
 
 
-@pytest.mark.parametrize("kernel,quant", [(0, pa.Q8_0), (1, pa.Q4_0), (2, pa.Q4_0), (0, pa.F16)])
+@pytest.mark.parametrize("kernel,quant", [(0, pa.Q8_0), (1, pa.Q4_0), (2, pa.Q4_0), (3, pa.Q4_0), (0, pa.F16)])
 def test_many_rows_and_a_long_cache(ctx, kernel, quant):
     """several row tiles, several parts of a sequence, wide pages, rows with padding bytes"""
     sq = Seqs(3, [4097, 130, 2500], 128, 8, quant, 1024, pad_row=16)
     _run(ctx, sq, 75, 5, kernel, 333, 21)
+    _run(ctx, sq, 110, 5, kernel, 333, 21)
     _run(ctx, sq, 60, 5, kernel, bits=_tree(np.random.default_rng(2), 3, 60))
 
 
@@ -310,7 +311,7 @@ def test_two_plans_on_two_streams(ctx):
         plans[i].close()
 
 
-@pytest.mark.parametrize("kernel", [1, 2])
+@pytest.mark.parametrize("kernel", [1, 2, 3])
 def test_a_wait_that_runs_out_is_reported_and_the_next_call_is_right(ctx, kernel):
     sq = Seqs(43, [300, 80], page=64)
     ctx.set_kernel(kernel)
@@ -333,7 +334,7 @@ def test_a_wait_that_runs_out_is_reported_and_the_next_call_is_right(ctx, kernel
     plan.close()
 
 
-@pytest.mark.parametrize("kernel", [1, 2])
+@pytest.mark.parametrize("kernel", [1, 2, 3])
 def test_pages_past_four_gigabytes(ctx, kernel):
     """row offsets that pass 32 bits: every call on the last pages of a layer of 4.6 GB"""
     import torch
@@ -606,11 +607,10 @@ def test_refusals(ctx):
     no(U, P, ctx, c, 1, 65, 5, 4, tree=True)
     no(U, P, ctx, c, 1, 9, 5, 4, 8, tree=True)
     no(U, P, ctx, c, 65536, 1, 5, 4)
-    ctx.set_kernel(3)
-    no(U, P, ctx, c, 1, 1, 5, 4)
-    ctx.set_kernel(2)
-    no(U, P, ctx, pa.Cache(128, 8, pa.F16, 1, 4, 64), 1, 1, 5, 4)
-    ctx.set_kernel(0)
+    for k in (2, 3):
+        ctx.set_kernel(k)
+        no(U, P, ctx, pa.Cache(128, 8, pa.F16, 1, 4, 64), 1, 1, 5, 4)
+        ctx.set_kernel(0)
     no(U, P, ctx, c, 65535, 1 << 14, 1, 4)
     no(U, P, ctx, pa.Cache(128, 8, pa.Q8_0, 1, 4, 96), 1, 1, 5, 4)
     no(U, P, ctx, pa.Cache(64, 8, pa.Q8_0, 1, 4, 64), 1, 1, 5, 4)
