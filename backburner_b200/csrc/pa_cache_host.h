@@ -268,13 +268,22 @@ int shape_cache_plan(pa_cuda_cache_plan *p) {
     const bool tc_ok = sh.quant != PA_CUDA_F16 && encode_fn() != nullptr;
     if (ctx->kernel_choice >= 2 && !tc_ok) return fail(ctx, PA_CUDA_EUNSUPPORTED, "tcgen05 kernels need quantised (Q8_0 / Q4_0) rows");
     p->tc = tc_ok && (ctx->kernel_choice >= 2 || (ctx->kernel_choice == 0 && sh.rows >= (sh.hd == 128 ? kPrefillMinRows128 : kPrefillMinRows256)));
-    p->pair = p->tc && (ctx->kernel_choice == 3 || (ctx->kernel_choice == 0 && sh.rows >= (sh.hd == 256 ? kSingle256MaxRows + 1 : kPairMinRows)));
     // groups of keys that one set can have to read
     const uint32_t G = p->tc ? 64 : 16;
     const uint64_t cap = (uint64_t) p->max_pages * p->cache.page_keys;
     uint64_t groups = cap / G;
     if (p->mask.window)
         groups = std::min(groups, ((uint64_t) p->mask.window + p->mask.n_tok + G - 1) / G + 1 + std::min<uint64_t>((p->mask.sinks + (uint64_t) G - 1) / G, groups));
+    if (p->tc) {
+        // CTA pairs (512 rows a unit at hd 128) run a row of a group in 7/8 of the single-CTA kernel's time, if their rows are
+        // real and the keys long: us single vs pair, 8 KV heads, 65,536 Q8_0 keys: 305 rows 159 vs 147, 640 rows 225 vs 308, 2,560
+        // rows 884 vs 849; 2,560 rows over a window of 1,024 keys 51 vs 56, of 4,096 102 vs 98 (Q4_0 91 vs 96). hd 256, where
+        // the single-CTA kernel has one tile: 240 rows x 4,096 keys 26.7 vs 24.6, 768 x 16,384 76 vs 67
+        const uint64_t in_pairs = ((uint64_t) sh.rows + 511) / 512 * 512, left = sh.rows % 256;
+        const uint64_t single = (uint64_t) sh.rows / 256 * 256 + (left == 0 ? 0 : left <= 128 ? 224 : 256);
+        const bool better = sh.hd == 256 ? sh.rows > kSingle256MaxRows : sh.rows >= kPairMinRows && groups >= 128 && 7 * in_pairs <= 8 * single;
+        p->pair = ctx->kernel_choice == 3 || (ctx->kernel_choice == 0 && better);
+    }
     uint64_t parts, units;
     if (p->tc) {
         const uint32_t tile = (uint32_t) pa::pre::BM * (p->pair ? 2u : 1u), ctas = p->pair ? 2 : 1;

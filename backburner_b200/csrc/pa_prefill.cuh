@@ -252,6 +252,10 @@ __global__ void __launch_bounds__(32 * cta_warps(NT), 1) prefill_kernel(const __
     static_assert(NSB == 1 && NPB == 2 && T_O + D <= (NT == 1 ? T_Q : 256u) && T_Q + (QT ? D / 2 : 0) <= TCOLS,
                   "tensor memory layout");
     static_assert(!QT || NT == 1, "Q in tensor memory with one tile only");
+    // dequant items loaded ahead and maxima in four chains: measured with and without, us a call over a plan's segments (Q4_0 80
+    // rows x 4 x 196,608 keys 509 vs 537; Q8_0 200 rows x 4 x 65,536 303 vs 298; hd 256 48 rows x 8 x 32,768 177 vs 173) and over
+    // the paged cache (512 tokens x 4 heads, window 4,096: 91 vs 93; hd 256, 24 trees of 8 tokens: 75 vs 73)
+    constexpr bool AHEAD = D == 128 && (NT == 1 || PAGED);
     // column of P buffer i (relative to the tile)
     auto p_col = [](uint32_t i) -> uint32_t { return T_P + i * (B / 2); };
 
@@ -385,8 +389,8 @@ __global__ void __launch_bounds__(32 * cta_warps(NT), 1) prefill_kernel(const __
       // 16 warps launched with 128 registers each at NT = 1 and 2; each warpgroup resizes its share (NT = 1, 64-key
       // blocks: control 160, softmax 168, two dequant warpgroups 88; 128-key blocks: control 128, softmax 200 (the 128
       // scores of a row), dequant 88: 128 x (160 + 168 + 88 + 88) or 128 x (128 + 200 + 88 + 88) = 64,512 <= 65,536)
-      // (PAGED: the dequantisers hold the live masks too: control 96, dequant 112 (NT = 2) or 104; hd 256: control 128, dequant
-      // 104. 128 x (96 + 152 + 152 + 112), 128 x (96 + 200 + 104 + 104), 128 x (128 + 168 + 104 + 104) <= 65,536)
+      // (PAGED: more for the dequantisers' items loaded ahead, less for control, which must not drop below the TMA warp's mask
+      // words: control 96, dequant 112 (NT = 2) or 104; hd 256: control 128, dequant 104. 128 x (96 + 152 + 152 + 112), 128 x (96 + 200 + 104 + 104), 128 x (128 + 168 + 104 + 104) <= 65,536)
       if constexpr (PAGED && !(NT == 1 && B == 64)) asm volatile("setmaxnreg.dec.sync.aligned.u32 96;");
       else if constexpr (!PAGED && NT == 1 && B == 64) asm volatile("setmaxnreg.inc.sync.aligned.u32 160;");
       if (warp == 0) {
@@ -401,16 +405,28 @@ __global__ void __launch_bounds__(32 * cta_warps(NT), 1) prefill_kernel(const __
             }
         }
         const CUtensorMap *km = p.kv_maps + (PAGED ? 0 : 2 * job.seg), *vm = km + 1;
-        pg::Span span{};
-        uint32_t pg0 = 0, pgn = 0;   // PAGED: this CTA's groups [pg0, pg0 + pgn) of its unit's span
-        if constexpr (PAGED) {
-            span = pg::span_of<64>(p.pg.v, s_part.st, s_part.t0, s_part.t1);
-            s_part.share((uint32_t) span.n, pg0, pgn);
-        }
         uint32_t issued = 0;
-        for (uint32_t j = 0; j < nblk; j++) {
-            const uint32_t st = j % NRS;
-            if constexpr (PAGED) {
+        if constexpr (!PAGED) {
+            if (lane == 0)
+                for (uint32_t j = 0; j < nblk; j++) {
+                    const uint32_t st = j % NRS;
+                    if (j >= NRS && !wait(&raw_empty[st], ((j / NRS) - 1) & 1)) break;
+                    mbar_arrive_expect_tx(&raw_full[st], 2 * B * RAWB);
+                    uint8_t *dst = smem + L::RAW + st * L::RAW_STAGE;
+#pragma unroll
+                    for (int c = 0; c < B / BN; c++) {   // the tensor maps' boxes hold 64 keys
+                        const int key = (int) (job.key0 + j * B) + c * BN;
+                        tma_2d(dst + c * BN * RAWB, km, hx / 2, key, &raw_full[st]);
+                        tma_2d(dst + (B + c * BN) * RAWB, vm, hx / 2, key, &raw_full[st]);
+                    }
+                    issued = j + 1;
+                }
+        } else {
+            const pg::Span span = pg::span_of<64>(p.pg.v, s_part.st, s_part.t0, s_part.t1);
+            uint32_t pg0, pgn;   // this CTA's groups [pg0, pg0 + pgn) of its unit's span
+            s_part.share((uint32_t) span.n, pg0, pgn);
+            for (uint32_t j = 0; j < nblk; j++) {
+                const uint32_t st = j % NRS;
                 if (j % (32 / (B / BN)) == 0) {
                     const uint32_t g = j * (B / BN) + lane;
                     const int k0 = span.group((int) (pg0 + g)) * BN;
@@ -420,30 +436,24 @@ __global__ void __launch_bounds__(32 * cta_warps(NT), 1) prefill_kernel(const __
                     if (!full) s_live[g % 64] = some ? pg::vis64(s_tile.any, k0) : 0ull;
                     __syncwarp();
                 }
-            }
-            if (lane == 0) {
-                if (j >= NRS) wait(&raw_empty[st], ((j / NRS) - 1) & 1);
-                if (ok) {
-                    // PAGED: the last block may hold one group fewer
-                    const uint32_t copies = PAGED ? min((uint32_t) (B / BN), pgn - j * (B / BN)) : (uint32_t) (B / BN);
-                    mbar_arrive_expect_tx(&raw_full[st], 2 * copies * BN * RAWB);
-                    uint8_t *dst = smem + L::RAW + st * L::RAW_STAGE;
+                if (lane == 0) {
+                    if (j >= NRS) wait(&raw_empty[st], ((j / NRS) - 1) & 1);
+                    if (ok) {
+                        const uint32_t copies = min((uint32_t) (B / BN), pgn - j * (B / BN));   // the last block may hold one fewer
+                        mbar_arrive_expect_tx(&raw_full[st], 2 * copies * BN * RAWB);
+                        uint8_t *dst = smem + L::RAW + st * L::RAW_STAGE;
 #pragma unroll
-                    for (int c = 0; c < B / BN; c++) {   // the tensor maps' boxes hold 64 keys
-                        int key;
-                        if constexpr (PAGED) {
+                        for (int c = 0; c < B / BN; c++) {
                             if (c >= (int) copies) break;
-                            key = (int) s_grow[(j * (B / BN) + c) % 64];
-                        } else {
-                            key = (int) (job.key0 + j * B) + c * BN;
+                            const int key = (int) s_grow[(j * (B / BN) + c) % 64];
+                            tma_2d(dst + c * BN * RAWB, km, hx / 2, key, &raw_full[st]);
+                            tma_2d(dst + (B + c * BN) * RAWB, vm, hx / 2, key, &raw_full[st]);
                         }
-                        tma_2d(dst + c * BN * RAWB, km, hx / 2, key, &raw_full[st]);
-                        tma_2d(dst + (B + c * BN) * RAWB, vm, hx / 2, key, &raw_full[st]);
+                        issued = j + 1;
                     }
-                    issued = j + 1;
                 }
+                if (!__shfl_sync(0xffffffffu, ok, 0)) break;
             }
-            if (!__shfl_sync(0xffffffffu, ok, 0)) break;
         }
         if (lane == 0) {
             // on an abort, every issued copy lands before the CTA exits
@@ -610,15 +620,16 @@ __global__ void __launch_bounds__(32 * cta_warps(NT), 1) prefill_kernel(const __
                     if (i >= nvalid) s[i] = -INFINITY;
             }
             }
-            float mx4[4];   // four chains: one would be B / 2 dependent steps long
+            constexpr int CH = AHEAD ? 4 : 1;   // independent chains of maxima
+            float mxc[CH];
 #pragma unroll
-            for (int q = 0; q < 4; q++) {
-                mx4[q] = s[q * (B / 4)];
+            for (int q = 0; q < CH; q++) {
+                mxc[q] = s[q * (B / CH)];
 #pragma unroll
-                for (int i = 1; i + 1 < B / 4; i += 2) mx4[q] = max3(mx4[q], s[q * (B / 4) + i], s[q * (B / 4) + i + 1]);
-                mx4[q] = fmaxf(mx4[q], s[q * (B / 4) + B / 4 - 1]);
+                for (int i = 1; i + 1 < B / CH; i += 2) mxc[q] = max3(mxc[q], s[q * (B / CH) + i], s[q * (B / CH) + i + 1]);
+                mxc[q] = fmaxf(mxc[q], s[q * (B / CH) + B / CH - 1]);
             }
-            float mx = fmaxf(max3(mx4[0], mx4[1], mx4[2]), mx4[3]);
+            float mx = CH == 1 ? mxc[0] : fmaxf(max3(mxc[0], mxc[1 % CH], mxc[2 % CH]), mxc[3 % CH]);
             mx *= LOG2E;
             m_row = fmaxf(m_row, mx);
             float alpha = 1.f;
@@ -719,9 +730,8 @@ __global__ void __launch_bounds__(32 * cta_warps(NT), 1) prefill_kernel(const __
                 for (int c = 0; c < B / 64; c++) edge |= (int) *(volatile uint32_t *) &s_group[(j * (B / 64) + c) % 64] < 0;
             }
             // Items of the block for this warp: 64-key chunk kc, key half (8 warps) or pass (4 warps), quant block of the
-            // warp; K's, then V's. An item's words are loaded while the one before it is converted (the loads and stores are
-            // ordered among themselves, so without this every item waits out its own shared-memory latency: 64-key blocks of a
-            // 305-row tree over 131,072 Q8_0 keys took 2,500 cycles, 2,100 of them in these warps).
+            // warp; K's, then V's. AHEAD: an item's words are loaded while the one before it is converted (the loads and
+            // stores are ordered among themselves, so without this every item waits out its own shared-memory latency).
             constexpr int NI = (B / 64) * (8 / NDQ) * (D / 128);
             uint32_t W[2][12], S2[2];
             auto qblk_of = [&](int it) -> uint32_t { return dw % 4 + 4 * (uint32_t) (it / ((8 / NDQ) * (B / 64))); };
@@ -740,12 +750,14 @@ __global__ void __launch_bounds__(32 * cta_warps(NT), 1) prefill_kernel(const __
                 for (int i = 0; i < (QUANT == 1 ? 3 : 2); i++) lds128(rb + w16 + 16 * i, w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
                 if (QUANT != 1) w[8] = w[9] = w[10] = w[11] = 0u;
             };
-            load(0, W[0], S2[0]);
+            if constexpr (AHEAD) load(0, W[0], S2[0]);
 #pragma unroll
             for (int x = 0; x < 2 * NI; x++) {
                 const int kv = x / NI, it = x % NI;
                 if (it == 0 && j >= KVB && !wait(kv == 0 ? &k_free[b] : &v_free[b], ((j / KVB) - 1) & 1)) break;
-                if (x + 1 < 2 * NI) {
+                if (!AHEAD) {
+                    load(x, W[x & 1], S2[x & 1]);
+                } else if (x + 1 < 2 * NI) {
                     load(x + 1, W[(x + 1) & 1], S2[(x + 1) & 1]);
                 } else {   // the raw stage is read
                     __syncwarp();
@@ -823,6 +835,10 @@ __global__ void __launch_bounds__(32 * cta_warps(NT), 1) prefill_kernel(const __
                 }
             }
             if (!ok) break;
+            if constexpr (!AHEAD) {
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&raw_empty[st]);
+            }
         }
     }
 

@@ -313,17 +313,24 @@ __global__ void __launch_bounds__(32 * (4 + 4 * NT + pair_dq_warps(D)), 1) prefi
                     tma_2d(smem + L::Q + t * BM * D * 2 + c * BM * 128, &tq, c * 64, qrow + t * 2 * BM, q_full);
         }
         const CUtensorMap *km = p.kv_maps + (PAGED ? 0 : 2 * job.seg), *vm = km + 1;
-        pg::Span span{};
-        uint32_t pg0 = 0;   // PAGED: this pair's first group of its unit's span
-        if constexpr (PAGED) {
-            uint32_t count;
-            span = pg::span_of<64>(p.pg.v, s_part.st, s_part.t0, s_part.t1);
-            s_part.share((uint32_t) span.n, pg0, count);
-        }
         uint32_t issued = 0;
-        for (uint32_t j = 0; j < nblk; j++) {
-            const uint32_t st = j % NS;
-            if constexpr (PAGED) {
+        if constexpr (!PAGED) {
+            if (lane == 0)
+                for (uint32_t j = 0; j < nblk; j++) {
+                    const uint32_t st = j % NS;
+                    if (j >= NS && !wait(&raw_empty[st], ((j / NS) - 1) & 1)) break;
+                    mbar_arrive_expect_tx(&raw_full[st], (KH + BN) * RAWB);
+                    uint8_t *dst = smem + L::RAW + st * L::RAW_STAGE;
+                    tma_2d(dst, km, hx / 2, (int) (job.key0 + j * BN + cr * KH), &raw_full[st]);
+                    tma_2d(dst + L::RAW_V, vm, hx / 2, (int) (job.key0 + j * BN), &raw_full[st]);
+                    issued = j + 1;
+                }
+        } else {
+            const pg::Span span = pg::span_of<64>(p.pg.v, s_part.st, s_part.t0, s_part.t1);
+            uint32_t pg0, count;   // this pair's groups of its unit's span
+            s_part.share((uint32_t) span.n, pg0, count);
+            for (uint32_t j = 0; j < nblk; j++) {
+                const uint32_t st = j % NS;
                 if (j % 32 == 0) {
                     const uint32_t g = j + lane;
                     const int k0 = span.group((int) (pg0 + g)) * BN;
@@ -333,21 +340,19 @@ __global__ void __launch_bounds__(32 * (4 + 4 * NT + pair_dq_warps(D)), 1) prefi
                     if (!full) s_live[g % 64] = some ? pg::vis64(s_tile.any, k0) : 0ull;
                     __syncwarp();
                 }
-            }
-            if (lane == 0) {
-                if (j >= NS) wait(&raw_empty[st], ((j / NS) - 1) & 1);
-                if (ok) {
-                    mbar_arrive_expect_tx(&raw_full[st], (KH + BN) * RAWB);
-                    uint8_t *dst = smem + L::RAW + st * L::RAW_STAGE;
-                    int key;
-                    if constexpr (PAGED) key = (int) s_grow[j % 64];
-                    else key = (int) (job.key0 + j * BN);
-                    tma_2d(dst, km, hx / 2, key + (int) cr * KH, &raw_full[st]);
-                    tma_2d(dst + L::RAW_V, vm, hx / 2, key, &raw_full[st]);
-                    issued = j + 1;
+                if (lane == 0) {
+                    if (j >= NS) wait(&raw_empty[st], ((j / NS) - 1) & 1);
+                    if (ok) {
+                        mbar_arrive_expect_tx(&raw_full[st], (KH + BN) * RAWB);
+                        uint8_t *dst = smem + L::RAW + st * L::RAW_STAGE;
+                        const int key = (int) s_grow[j % 64];
+                        tma_2d(dst, km, hx / 2, key + (int) cr * KH, &raw_full[st]);
+                        tma_2d(dst + L::RAW_V, vm, hx / 2, key, &raw_full[st]);
+                        issued = j + 1;
+                    }
                 }
+                if (!__shfl_sync(0xffffffffu, ok, 0)) break;
             }
-            if (!__shfl_sync(0xffffffffu, ok, 0)) break;
         }
         if (lane == 0) {
             if (!ok) {
