@@ -14,6 +14,74 @@
 namespace pa {
 namespace pg {
 
+// ---------------------------------------------------------------- many units dealt out
+// The same dealing as a CTA's own in find_part, for more units than a warp has lanes: one block, a unit to a thread (and every
+// 1,024th after it), whose costs stay in crange until the parts' ends replace them. The bisection stops within 1/32 of the
+// least cost. Bound: latency (a round is two barriers and the loads of the thread's own costs).
+constexpr uint32_t DEAL_THREADS = 1024;
+template <int G>
+__global__ void __launch_bounds__(DEAL_THREADS) deal_kernel(const Paged p) {
+    constexpr uint32_t W = DEAL_THREADS / 32;
+    __shared__ uint64_t sums[W];
+    __shared__ uint32_t tops[W], needs[2][W], ends[W];
+    const uint32_t units = p.v.n_sets * p.n_rt, tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
+    pdl_trigger();
+    pdl_wait();
+    uint64_t total = 0;
+    uint32_t top = 0;
+    for (uint32_t u = tid; u < units; u += DEAL_THREADS) {
+        Part r{};
+        const uint32_t cost = unit_of<G>(p, u, r);
+        p.crange[u + 1] = cost;
+        total += cost;
+        top = max(top, cost);
+    }
+#pragma unroll
+    for (int x = 16; x > 0; x >>= 1) total += __shfl_xor_sync(0xffffffffu, total, x);
+    top = __reduce_max_sync(0xffffffffu, top);
+    if (lane == 0) {
+        sums[warp] = total;
+        tops[warp] = top;
+    }
+    __syncthreads();
+    total = sums[lane];
+#pragma unroll
+    for (int x = 16; x > 0; x >>= 1) total += __shfl_xor_sync(0xffffffffu, total, x);
+    top = __reduce_max_sync(0xffffffffu, tops[lane]);
+    uint32_t lo, hi;
+    part_bounds(p, units, total, lo, hi);
+    hi = max(lo, min(hi, top));   // (one part a unit fits too)
+    for (uint32_t round = 0; hi - lo > lo / 32; round++) {   // the same in all threads
+        const uint32_t mid = lo + (hi - lo) / 2;
+        uint32_t need = 0;
+        for (uint32_t u = tid; u < units; u += DEAL_THREADS) need += (p.crange[u + 1] + mid - 1) / mid;
+        need = __reduce_add_sync(0xffffffffu, need);
+        if (lane == 0) needs[round % 2][warp] = need;
+        __syncthreads();
+        need = __reduce_add_sync(0xffffffffu, needs[round % 2][lane]);
+        if (need <= p.n_parts) hi = mid;
+        else lo = mid + 1;
+    }
+    if (tid == 0) p.crange[0] = 0;
+    uint32_t base = 0;
+    for (uint32_t u0 = 0; u0 < units; u0 += DEAL_THREADS) {
+        const uint32_t u = u0 + tid;
+        uint32_t end = u < units ? (p.crange[u + 1] + hi - 1) / hi : 0;
+#pragma unroll
+        for (int x = 1; x < 32; x <<= 1) {
+            const uint32_t y = __shfl_up_sync(0xffffffffu, end, x);
+            if (lane >= (uint32_t) x) end += y;
+        }
+        __syncthreads();   // the last round's ends are read
+        if (lane == 31) ends[warp] = end;
+        __syncthreads();
+        const uint32_t all = ends[lane];
+        end += base + __reduce_add_sync(0xffffffffu, lane < warp ? all : 0);
+        base += __reduce_add_sync(0xffffffffu, all);
+        if (u < units) p.crange[u + 1] = end;
+    }
+}
+
 // ---------------------------------------------------------------- merge of the paged attention's partials
 // The log-sum-exp merge of a unit's parts (pa_merge.cuh's, over this cache's slots), giving O, m, l or f16(O / l) and lse. A
 // call's merge is a chain of dependent loads (the parts' range, their l and m, their O) behind the attention kernel, so the
@@ -301,9 +369,11 @@ __global__ void __launch_bounds__(32 * APPEND_WARPS, 6) append_kernel(const Appe
     }
     for (uint32_t i = threadIdx.x; i < half; i += 32 * APPEND_WARPS) {
         const double turn = (double) pos * p.freqs[i] * 0.15915494309189535;   // / (2 pi)
+        const double x = 2. * (turn - rint(turn));   // half turns
+        const float hi = (float) x, lo = 3.14159265f * (float) (x - hi);   // the angle's rounding, up to 2^-25 half turns
         float sn, c;
-        sincospif(2.f * (float) (turn - rint(turn)), &sn, &c);
-        cs[i] = make_float2(c, sn);
+        sincospif(hi, &sn, &c);
+        cs[i] = make_float2(fmaf(-lo, sn, c), fmaf(lo, c, sn));
     }
     __syncthreads();
     const int64_t at = s_at;
@@ -336,7 +406,9 @@ __global__ void __launch_bounds__(32 * APPEND_WARPS, 6) append_kernel(const Appe
             ss += s1;
 #pragma unroll
             for (int d = LPH / 2; d > 0; d >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, d);
-            f *= rsqrtf(ss * (1.f / HD) + p.eps);
+            // (the approximation's 2 units in the last place, after a Newton step less than one)
+            const float a = fmaf(ss, 1.f / HD, p.eps), r = rsqrtf(a);
+            f *= fmaf(0.5f * r, fmaf(-a * r, r, 1.f), r);
             const ulonglong2 w0 = reinterpret_cast<const ulonglong2 *>(w8)[0], w1 = reinterpret_cast<const ulonglong2 *>(w8)[1];
             x[0] = mul_f2(x[0], w0.x);
             x[1] = mul_f2(x[1], w0.y);

@@ -73,6 +73,10 @@ bool aligned(uintptr_t n, std::initializer_list<const void *> ptrs) {
     for (const void *p : ptrs) x |= (uintptr_t) p;
     return x % n == 0;
 }
+// whether two device arrays of n and k int32 share a byte
+bool overlap(const int32_t *a, uint64_t n, const int32_t *b, uint64_t k) {
+    return a && b && (uintptr_t) a < (uintptr_t) b + 4 * k && (uintptr_t) b < (uintptr_t) a + 4 * n;
+}
 uint64_t page_mul(uint32_t page_keys) { return ((1ull << 40) + page_keys / 64 - 1) / (page_keys / 64); }
 uint64_t layer_bytes(const pa_cuda_shape &sh, const pa_cuda_cache &c) { return (uint64_t) c.n_pages * c.page_keys * sh.rs; }
 
@@ -189,7 +193,13 @@ int cache_attn(pa_cuda_cache_plan *p, uint32_t layer, const uint16_t *Qs, const 
     pg.half_rows = p->tc && !p->pair && p->nt == 2 ? (uint32_t) pa::pre::BM : 0u;
     pg.n_rt = p->n_rt;
     pg.crange = p->d_crange;
-    cudaError_t e;
+    cudaError_t e = cudaSuccess;
+    if ((uint64_t) p->n_sets * p->n_rt > pa::pg::UNITS_IN_WARP) {
+        e = p->tc ? launch_pdl(pa::pg::deal_kernel<64>, dim3(1), pa::pg::DEAL_THREADS, 0, st, pg)
+                  : launch_pdl(pa::pg::deal_kernel<16>, dim3(1), pa::pg::DEAL_THREADS, 0, st, pg);
+        if (e != cudaSuccess) return cuda_fail(ctx, e, "cache deal launch");
+        ctx->launches++;
+    }
     if (p->tc) {
         CUtensorMap tq;
         if (!map_q(&tq, Qs, p->n_sets * rows_all, sh.hd)) return fail(ctx, PA_CUDA_ECUDA, "cuTensorMapEncodeTiled (Q) failed");
@@ -602,6 +612,10 @@ int pa_cuda_cache_compact(pa_cuda_ctx *ctx, const pa_cuda_shape *shape, const pa
     if (n_tok == 0 || n_tok > pa::pg::COMPACT_MAX) return fail(ctx, PA_CUDA_EUNSUPPORTED, "a path has 1 to 1,024 tokens");
     if (!table || !start || !path || !count) return fail(ctx, PA_CUDA_EINVAL, "null argument");
     if (!aligned(4, {table, start, path, count, n_keys_out})) return fail(ctx, PA_CUDA_EINVAL, "misaligned pointer");
+    // (every block of a set reads them, one writes n_keys_out)
+    if (overlap(n_keys_out, n_sets, start, n_sets) || overlap(n_keys_out, n_sets, count, n_sets) ||
+        overlap(n_keys_out, n_sets, path, (uint64_t) n_sets * n_tok) || overlap(n_keys_out, n_sets, table, (uint64_t) n_sets * max_pages))
+        return fail(ctx, PA_CUDA_EINVAL, "n_keys_out overlaps an input");
     DeviceScope dev(ctx->device);
     if (!dev.ok) return fail(ctx, PA_CUDA_ECUDA, "cudaSetDevice");
     pa::pg::CompactParams a{};

@@ -158,77 +158,79 @@ PA_HD void tokens_of(const Paged &p, uint32_t rt, uint32_t &t0, uint32_t &t1) {
     t0 = a + n > T ? 0u : a;
     t1 = a + n > T ? T - 1 : a + n - 1;
 }
-// warp-collective; every lane gets the result. G keys a group; a group of a unit with one row tile costs 7/8 of one with two.
+// unit u, and the cost of its groups of G keys (a group of a unit with one row tile costs 7/8 of one with two)
+template <int G>
+__device__ __forceinline__ uint32_t unit_of(const Paged &p, uint32_t u, Part &r) {
+    r.set = p.n_rt == 1 ? u : u / p.n_rt;
+    r.rt = u - r.set * p.n_rt;
+    tokens_of(p, r.rt, r.t0, r.t1);
+    r.st = set_of(p.v, r.set);
+    return (uint32_t) span_of<G>(p.v, r.st, r.t0, r.t1).n * (p.rows - r.rt * p.tile_rows <= p.half_rows ? 7u : 8u);
+}
+// the bounds of a part's cost: the least that a part may take, and one with which all units fit n_parts
+__device__ __forceinline__ void part_bounds(const Paged &p, uint32_t units, uint64_t total, uint32_t &lo, uint32_t &hi) {
+    const uint32_t least = max(1u, (uint32_t) sqrtf((float) total / (float) (8ull * units)) / 4) * 8;
+    lo = hi = max(least, (uint32_t) ((total + p.n_parts - 1) / p.n_parts));
+    // sum of ceil(cost / per) < total / per + units <= n_parts at hi (n_parts > units, by the plan); 2^30 is past any
+    // unit's cost
+    if (units > 1) hi = max(lo, (uint32_t) min((uint64_t) 1 << 30, (total + (p.n_parts - units) - 1) / (p.n_parts - units)));
+}
+constexpr uint32_t UNITS_IN_WARP = 32;   // up to so many units every CTA deals them out itself, one to a lane
+// Part c. Warp-collective; every lane gets the result. With more units a kernel of its own has dealt them out (deal_kernel;
+// every CTA going over all of them took 12 times as long at 1,024 sets of 8 tokens) and the CTA looks its part up in crange.
 template <int G>
 __device__ __forceinline__ Part find_part(const Paged &p, uint32_t c, bool write, uint32_t lane) {
-    const View &v = p.v;
-    const uint32_t units = v.n_sets * p.n_rt;
-    // unit u, and the cost of its groups
-    auto unit = [&](uint32_t u, Part &r) -> uint32_t {
-        r.set = p.n_rt == 1 ? u : u / p.n_rt;
-        r.rt = u - r.set * p.n_rt;
-        tokens_of(p, r.rt, r.t0, r.t1);
-        r.st = set_of(v, r.set);
-        return (uint32_t) span_of<G>(v, r.st, r.t0, r.t1).n * (p.rows - r.rt * p.tile_rows <= p.half_rows ? 7u : 8u);
-    };
-    Part mine{};                       // the lane's unit of the last round (the only one with up to 32 units)
-    uint32_t cost = 0;
-    uint64_t total = 0;
-    for (uint32_t u = lane; u < units; u += 32) total += cost = unit(u, mine);
+    const uint32_t units = p.v.n_sets * p.n_rt;
+    Part mine{};
+    if (units > UNITS_IN_WARP) {
+        const volatile uint32_t *ends = p.crange;
+        if (c >= ends[units]) return mine;
+        uint32_t lo = 0, hi = units;   // ends[lo] <= c < ends[hi]
+        while (hi - lo > 1) {
+            const uint32_t step = (hi - lo + 31) / 32, at = lo + lane * step;
+            const uint32_t below = __ballot_sync(0xffffffffu, at < hi && ends[at] <= c);   // rising: a run of lanes from lane 0
+            lo += (uint32_t) (__popc(below) - 1) * step;
+            hi = min(hi, lo + step);
+        }
+        unit_of<G>(p, lo, mine);
+        mine.index = c - ends[lo];
+        mine.of = ends[lo + 1] - ends[lo];
+        return mine;
+    }
+    const uint32_t cost = lane < units ? unit_of<G>(p, lane, mine) : 0;   // a lane's unit
+    uint64_t total = cost;
 #pragma unroll
     for (int x = 16; x > 0; x >>= 1) total += __shfl_xor_sync(0xffffffffu, total, x);
-    const uint32_t least = max(1u, (uint32_t) sqrtf((float) total / (float) (8 * units)) / 4) * 8;
     uint32_t lo, hi;
-    if (units == 1) {   // (below 2^30)
-        lo = hi = max(least, ((uint32_t) total + p.n_parts - 1) / p.n_parts);
-    } else {
-        lo = hi = max(least, (uint32_t) ((total + p.n_parts - 1) / p.n_parts));
-        // sum of ceil(cost / per) < total / per + units <= n_parts at hi (n_parts > units, by the plan); 2^30 is past any
-        // unit's cost
-        hi = max(lo, (uint32_t) min((uint64_t) 1 << 30, (total + (p.n_parts - units) - 1) / (p.n_parts - units)));
-        while (lo < hi) {
-            const uint32_t mid = lo + (hi - lo) / 2;
-            uint32_t need = 0;
-            if (units <= 32) {
-                need = (cost + mid - 1) / mid;
-            } else {
-                Part r;
-                for (uint32_t u = lane; u < units; u += 32) need += (unit(u, r) + mid - 1) / mid;
-            }
-            need = __reduce_add_sync(0xffffffffu, need);
-            if (need <= p.n_parts) hi = mid;
-            else lo = mid + 1;
-        }
+    part_bounds(p, units, total, lo, hi);
+    while (lo < hi) {
+        const uint32_t mid = lo + (hi - lo) / 2, need = __reduce_add_sync(0xffffffffu, (cost + mid - 1) / mid);
+        if (need <= p.n_parts) hi = mid;
+        else lo = mid + 1;
+    }
+    const uint32_t cnt = (cost + hi - 1) / hi;
+    uint32_t end = cnt;
+#pragma unroll
+    for (int x = 1; x < 32; x <<= 1) {
+        const uint32_t y = __shfl_up_sync(0xffffffffu, end, x);
+        if (lane >= (uint32_t) x) end += y;
+    }
+    if (write) {
+        if (lane == 0) p.crange[0] = 0;
+        if (lane < units) p.crange[lane + 1] = end;
     }
     Part r{};
-    uint32_t base = 0;
-    if (write && lane == 0) p.crange[0] = 0;
-    for (uint32_t u0 = 0; u0 < units; u0 += 32) {
-        const uint32_t u = u0 + lane;
-        if (units > 32) cost = u < units ? unit(u, mine) : 0;
-        const uint32_t cnt = u < units ? (cost + hi - 1) / hi : 0;
-        uint32_t end = cnt;
-#pragma unroll
-        for (int x = 1; x < 32; x <<= 1) {
-            const uint32_t y = __shfl_up_sync(0xffffffffu, end, x);
-            if (lane >= (uint32_t) x) end += y;
-        }
-        end += base;
-        if (write && u < units) p.crange[u + 1] = end;
-        const uint32_t hit = __ballot_sync(0xffffffffu, c < end && c >= end - cnt);
-        if (hit) {
-            const int src = __ffs((int) hit) - 1;
-            r.set = __shfl_sync(0xffffffffu, mine.set, src);
-            r.rt = __shfl_sync(0xffffffffu, mine.rt, src);
-            r.t0 = __shfl_sync(0xffffffffu, mine.t0, src);
-            r.t1 = __shfl_sync(0xffffffffu, mine.t1, src);
-            r.of = __shfl_sync(0xffffffffu, cnt, src);
-            r.index = c - (__shfl_sync(0xffffffffu, end, src) - r.of);
-            r.st.nk = __shfl_sync(0xffffffffu, mine.st.nk, src);
-            r.st.q0 = __shfl_sync(0xffffffffu, mine.st.q0, src);
-            if (!write) return r;
-        }
-        base = __shfl_sync(0xffffffffu, end, 31);
+    const uint32_t hit = __ballot_sync(0xffffffffu, c < end && c >= end - cnt);
+    if (hit) {
+        const int src = __ffs((int) hit) - 1;
+        r.set = __shfl_sync(0xffffffffu, mine.set, src);
+        r.rt = __shfl_sync(0xffffffffu, mine.rt, src);
+        r.t0 = __shfl_sync(0xffffffffu, mine.t0, src);
+        r.t1 = __shfl_sync(0xffffffffu, mine.t1, src);
+        r.of = __shfl_sync(0xffffffffu, cnt, src);
+        r.index = c - (__shfl_sync(0xffffffffu, end, src) - r.of);
+        r.st.nk = __shfl_sync(0xffffffffu, mine.st.nk, src);
+        r.st.q0 = __shfl_sync(0xffffffffu, mine.st.q0, src);
     }
     return r;
 }

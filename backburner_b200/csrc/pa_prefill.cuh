@@ -254,7 +254,7 @@ __global__ void __launch_bounds__(32 * cta_warps(NT), 1) prefill_kernel(const __
     static_assert(!QT || NT == 1, "Q in tensor memory with one tile only");
     // dequant items loaded ahead and maxima in four chains: measured with and without, us a call over a plan's segments (Q4_0 80
     // rows x 4 x 196,608 keys 509 vs 537; Q8_0 200 rows x 4 x 65,536 303 vs 298; hd 256 48 rows x 8 x 32,768 177 vs 173) and over
-    // the paged cache (512 tokens x 4 heads, window 4,096: 91 vs 93; hd 256, 24 trees of 8 tokens: 75 vs 73)
+    // the paged cache (Q4_0: 512 tokens x 5 heads, window 4,096: 91 vs 93; hd 256, 8 trees of 16 tokens x 6 heads, 16,301 keys: 75 vs 73)
     constexpr bool AHEAD = D == 128 && (NT == 1 || PAGED);
     // column of P buffer i (relative to the tile)
     auto p_col = [](uint32_t i) -> uint32_t { return T_P + i * (B / 2); };

@@ -259,6 +259,7 @@ uint64_t pa_cuda_graph_calls(const pa_cuda_ctx *ctx);
  * Sequences ("sets") number their keys 0, 1, ...: key j of set s lies in page table[s][j / page_keys] (int32, device,
  * [n_sets][max_pages]; entries no key needs are not read and may hold anything). Rows past a sequence's keys, and rows no
  * token of the call sees, may hold anything, NaN included; a row that some tokens of a call see has to be finite.
+ * Outputs share no memory with inputs, but for the cache's own rows.
  * Arguments that only the device can check (a page id outside the pool, a length past the table's reach, a bad path) do
  * no harm: the rest of the call runs, what they touch is undefined, and pa_cuda_status reports PA_CUDA_EINVAL. */
 typedef struct pa_cuda_cache {

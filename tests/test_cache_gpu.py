@@ -651,6 +651,19 @@ def test_refusals(ctx):
     plan.close()
 
 
+def test_compact_does_not_write_the_lengths_over_an_input(ctx):
+    """n_keys_out over start, count, path or table: blocks of a set read what another has written"""
+    import torch
+    c = pa.Cache(128, 8, pa.Q8_0, 1, 4, 64)
+    buf = torch.zeros(16, dtype=torch.int32, device="cuda")
+    start, count, path, table, out = buf[:2], buf[2:4], buf[4:10].view(2, 3), buf[10:14].view(2, 2), buf[14:]
+    for bad in (start, count, buf[1:3], path.view(-1)[1:3], buf[9:11], buf[13:15]):
+        with pytest.raises(pa.PaCudaError) as e:
+            pa.cache_compact(ctx, c, table, start, path, count, out=bad)
+        assert e.value.code == api.EINVAL
+    assert pa.cache_compact(ctx, c, table, start, path, count, out=out).tolist() == [0, 0]
+
+
 # ------------------------------------------------------------------------------------------------- together
 @pytest.mark.parametrize("quant", QUANTS)
 def test_a_generation_with_drafts(ctx, quant):
