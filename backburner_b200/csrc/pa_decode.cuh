@@ -314,8 +314,10 @@ __global__ void __launch_bounds__(32 * W, min_ctas(HD, W)) decode_kernel(const t
     };
     if (warp == 0) {   // the first NSTAGE stream stages
         uint32_t jn = blockIdx.x, it = 0, n = stages_of(jn);
+        uint32_t rows = 0;   // PAGED: a lane looks up a stage's row
+        if constexpr (PAGED) rows = lane < NSTAGE && lane < n ? row_of_stage(lane) : 0u;
         for (uint32_t g = 0; g < NSTAGE && n > 0; g++) {
-            issue(jn, it, g, row_of_stage(it));
+            issue(jn, it, g, PAGED ? __shfl_sync(0xffffffffu, rows, (int) g) : 0u);
             if (++it == n) {
                 if constexpr (PAGED) break;
                 it = 0;
@@ -380,6 +382,31 @@ __global__ void __launch_bounds__(32 * W, min_ctas(HD, W)) decode_kernel(const t
             qi[b][1] = wv[1];
             dq[b][0] = __shfl_sync(0xffffffffu, df, 8 * t);       // row 2t lives in quad 2t
             dq[b][1] = __shfl_sync(0xffffffffu, df, 8 * t + 4);   // row 2t+1
+        }
+    } else if constexpr (PAGED && QS != 0) {
+        // the lane's quant blocks, 16 bytes at a time, put in dK's order in registers (with 2-byte loads of the single values
+        // the same call takes 2.3 us more)
+        const uint32_t row = rg * 8 + g;
+        const bool odd = t % 2;
+        const uint16_t *q = p.Qs + (((uint64_t) job.set * p.nkv + h) * p.rows + (row < p.rows ? row : 0)) * HD + 32 * t;
+#pragma unroll
+        for (int rep = 0; rep < HD / 128; rep++) {
+            uint32_t w[16];   // pairs of values
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                const uint4 x = row < p.rows ? reinterpret_cast<const uint4 *>(q + 128 * rep)[i] : make_uint4(0u, 0u, 0u, 0u);
+                w[4 * i] = x.x; w[4 * i + 1] = x.y; w[4 * i + 2] = x.z; w[4 * i + 3] = x.w;
+            }
+            // an even block's groups of 4 values start with its first and last pair, an odd one's are in order
+            constexpr int PAIRS = QS == 1 ? 16 : 8;   // pairs of a run (Q4_0: the low, then the high nibbles' values)
+#pragma unroll
+            for (int ss = 0; ss < 8; ss++) {
+                const int gr = QS == 1 ? ss : ss / 2, run = QS == 1 ? 0 : 8 * (ss % 2);
+                const uint32_t a = odd ? w[run + 2 * gr] : w[run + (gr == 0 ? 0 : 2 * gr - 1)];
+                const uint32_t b = odd ? w[run + 2 * gr + 1] : w[run + (gr == 0 ? PAIRS - 1 : 2 * gr)];
+                qf[8 * rep + ss][0] = QS == 1 ? a : prmt(a, b, 0x5410u);
+                qf[8 * rep + ss][1] = QS == 1 ? b : prmt(a, b, 0x7632u);
+            }
         }
     } else {
         const uint32_t row = rg * 8 + g;
@@ -724,16 +751,29 @@ __global__ void __launch_bounds__(32 * W, min_ctas(HD, W)) decode_kernel(const t
     // ---- write the job's slot partial
     const uint64_t rbase = ((uint64_t) job.slot * p.nkv + h) * p.rows;
     const uint32_t r0 = rg * 8 + 2 * t, r1 = r0 + 1;
+    if constexpr (PAGED && QS != 0) {
+        // a lane's dims come in runs of 8 and more, 4 in every other m-tile and its neighbour: 16-byte stores (single floats
+        // are eight stores to every sector: 32 sets x 4,100 keys x 4 heads x 6 rows at hd 256 84.8 us a call, and 75.4 so)
+        constexpr int NEXT = QS == 1 ? 1 : 2;
 #pragma unroll
-    for (int mt = 0; mt < NMT; mt++) {
-        const int d0 = dV(QS, HD, mt, (int) g, 0), d1 = dV(QS, HD, mt, (int) g, 1);
-        if (r0 < p.rows) {
-            p.Op[(rbase + r0) * HD + d0] = o[mt][0];
-            p.Op[(rbase + r0) * HD + d1] = o[mt][2];
+        for (int mt = 0; mt < NMT; mt++) {
+            if (mt / NEXT % 2) continue;
+            const int d = dV(QS, HD, mt, (int) g, 0), nx = (mt + NEXT) % NMT;
+            if (r0 < p.rows) *reinterpret_cast<float4 *>(p.Op + (rbase + r0) * HD + d) = make_float4(o[mt][0], o[mt][2], o[nx][0], o[nx][2]);
+            if (r1 < p.rows) *reinterpret_cast<float4 *>(p.Op + (rbase + r1) * HD + d) = make_float4(o[mt][1], o[mt][3], o[nx][1], o[nx][3]);
         }
-        if (r1 < p.rows) {
-            p.Op[(rbase + r1) * HD + d0] = o[mt][1];
-            p.Op[(rbase + r1) * HD + d1] = o[mt][3];
+    } else {
+#pragma unroll
+        for (int mt = 0; mt < NMT; mt++) {
+            const int d0 = dV(QS, HD, mt, (int) g, 0), d1 = dV(QS, HD, mt, (int) g, 1);
+            if (r0 < p.rows) {
+                p.Op[(rbase + r0) * HD + d0] = o[mt][0];
+                p.Op[(rbase + r0) * HD + d1] = o[mt][2];
+            }
+            if (r1 < p.rows) {
+                p.Op[(rbase + r1) * HD + d0] = o[mt][1];
+                p.Op[(rbase + r1) * HD + d1] = o[mt][3];
+            }
         }
     }
     if (g == 0) {
