@@ -26,6 +26,10 @@
 //   * P is taken against a lazily raised reference max (one warp vote per tile; the cross-lane max and the O rescale
 //     run only when a score passes the reference by 2^8), and the exact row max is restored once per job; a tile's V
 //     words are loaded before its softmax so their shared-memory latency overlaps the softmax.
+//   * PAGED: the same over a paged cache (pa_mask.cuh). A CTA walks its part's 16-key groups, each in one page, whose row
+//     the warps look up two stages ahead; only the groups at the edge of what the rows see are masked, and there V rows
+//     that no row sees get a zero scale. The work is short there (a window), so that its ends count: see the loads of Q
+//     and the stores of O.
 //   * QUANT 3: Q8_0 rows with the int8-domain QK of scripts/sme/sme_attn.c:465-508 (sme_qk_i8blk + i8_combine): Q is
 //     quantised per 32-block by the Q8_0 rule (d = f16(max|x| / 127), q = rint(x / d)) when a job starts, one
 //     mma.m16n8k32 s8 per quant block gives the block's exact int32 dot products T for 16 keys x 8 rows, and
@@ -82,7 +86,7 @@ struct Params {
     uint64_t timeout_ns;
     int stall;            // test hook: consumers first wait on a barrier that nothing completes (bounded)
 };
-// the paged kernel's: jobs, n_jobs unused
+// the paged kernel's (a CTA's job is its part, found on the device): jobs unused, n_jobs the parts
 struct PagedParams : Params {
     pg::Paged pg;
 };
