@@ -216,6 +216,15 @@ def test_many_ragged_sequences(ctx, kernel, quant):
     _run(ctx, sq, 30, 9, kernel, 50, 5)
 
 
+@pytest.mark.parametrize("kernel", [1, 2])
+def test_more_sequences_than_a_block_has_threads(ctx, kernel):
+    """over 1,024 units: dealt out in several rounds, empty sequences and one long one among them"""
+    rng = np.random.default_rng(8)
+    lens = [int(x) for x in rng.integers(0, 90, 1040)]
+    lens[700], lens[:3], lens[-1] = 3000, [0, 0, 0], 0
+    _run(ctx, Seqs(8, lens, 128, 2, pa.Q8_0, 64, layers=1), 1, 1, kernel)
+
+
 @pytest.mark.parametrize("kernel,quant", [(0, pa.Q8_0), (1, pa.Q4_0), (2, pa.Q4_0), (3, pa.Q4_0), (0, pa.F16)])
 def test_many_rows_and_a_long_cache(ctx, kernel, quant):
     """several row tiles, several parts of a sequence, wide pages, rows with padding bytes"""
