@@ -149,6 +149,13 @@ __device__ __forceinline__ uint64_t mul_f2(uint64_t a, uint64_t b) {
     return r;
 }
 
+// 8 floats to global memory, 32-byte aligned: a whole sector a lane
+__device__ __forceinline__ void stg_f8(float *p, const float (&x)[8]) {
+    asm volatile("st.global.v8.f32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "f"(x[0]), "f"(x[1]), "f"(x[2]), "f"(x[3]),
+                 "f"(x[4]), "f"(x[5]), "f"(x[6]), "f"(x[7])
+                 : "memory");
+}
+
 // transpose of an 8x8 b16 matrix held in mma fragment order (one .b32 per lane)
 __device__ __forceinline__ uint32_t movtrans(uint32_t x) {
     uint32_t d;

@@ -177,7 +177,7 @@ __device__ __forceinline__ void part_bounds(const Paged &p, uint32_t units, uint
 }
 constexpr uint32_t UNITS_IN_WARP = 32;   // up to so many units every CTA deals them out itself, one to a lane
 // Part c. Warp-collective; every lane gets the result. With more units a kernel of its own has dealt them out (deal_kernel;
-// every CTA going over all of them took 12 times as long at 1,024 sets of 8 tokens) and the CTA looks its part up in crange.
+// every CTA going over all of them took 6 times as long at 1,024 sets of 8 tokens) and the CTA looks its part up in crange.
 template <int G>
 __device__ __forceinline__ Part find_part(const Paged &p, uint32_t c, bool write, uint32_t lane) {
     const uint32_t units = p.v.n_sets * p.n_rt;

@@ -551,7 +551,17 @@ __global__ void __launch_bounds__(32 * (4 + 4 * NT + pair_dq_warps(D)), 1) prefi
                 float o[32];
                 tmem_ld32(tl + 128 + q * 32, o);
                 tmem_wait_ld();
-                if (row < p.rows) {
+                if constexpr (PAGED) {   // a sector a lane, since the lanes' rows lie far apart
+                    if (row < p.rows) {
+#pragma unroll
+                        for (int i = 0; i < 4; i++) {
+                            float y[8];
+#pragma unroll
+                            for (int e = 0; e < 8; e++) y[e] = o[8 * i + e] * fix;
+                            stg_f8(p.Op + orow * D + q * 32 + 8 * i, y);
+                        }
+                    }
+                } else if (row < p.rows) {
                     float4 *dst = reinterpret_cast<float4 *>(p.Op + orow * D + q * 32);
 #pragma unroll
                     for (int i = 0; i < 8; i++)
