@@ -280,9 +280,16 @@ __device__ __forceinline__ void store_head(uint8_t *head, uint32_t l, bool write
     const float df = __half2float(dh), id = df != 0.f ? __frcp_rn(df) : 0.f;
     uint8_t *blk = head + (l / 4) * dec::q_group_bytes(QUANT);
     const uint32_t in = l % 4;
+    // x / d rounded once (Markstein's correction: a quotient off by at most a unit in the last place, its exact remainder and the
+    // rounded reciprocal), so that a tie is a tie; d = 0 and d = inf give 0
+    const float dd = id != 0.f ? df : 0.f;
     uint32_t q[8];
 #pragma unroll
-    for (int e = 0; e < 8; e++) q[e] = (uint32_t) __float2int_rn(fmaxf(-TOP, fminf(TOP, __fmul_rn(x[e], id))));
+    for (int e = 0; e < 8; e++) {
+        float y = __fmul_rn(x[e], id);
+        y = fmaf(fmaf(-y, dd, x[e]), id, y);
+        q[e] = (uint32_t) __float2int_rn(fmaxf(-TOP, fminf(TOP, y)));
+    }
     if (write && in == 0) *reinterpret_cast<__half *>(blk) = dh;
     uint16_t *dst = reinterpret_cast<uint16_t *>(blk + 2 + 8 * in);   // blocks start at even bytes: 16-bit stores
     if (QUANT == 1) {

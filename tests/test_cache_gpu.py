@@ -24,6 +24,22 @@ def _quantise(torch, x, quant):
     return (pa.quantize_q8_0 if quant == pa.Q8_0 else pa.quantize_q4_0)(x)
 
 
+def _stored(torch, x, quant):
+    """The bytes of float32 x [..., hd] on the CPU by the format's formula, each quotient rounded once (the package's quantisers
+    multiply by the rounded 1 / d, which turns some ties the other way)."""
+    if quant == pa.F16:
+        return _quantise(torch, x, quant)
+    top = 127 if quant == pa.Q8_0 else 7
+    b = x.unflatten(-1, (-1, 32))
+    d = (b.abs().amax(-1, keepdim=True) / top).to(torch.float16)
+    q = torch.where(d == 0, 0.0, torch.round(b / d.float())).clamp(-top, top)
+    data = q.to(torch.int8).view(torch.uint8)
+    if quant == pa.Q4_0:
+        n = (q + 8).to(torch.uint8)
+        data = n[..., :16] | n[..., 16:] << 4
+    return torch.cat([d.view(torch.uint8), data], -1).flatten(-2)
+
+
 def _value(torch, rows, quant, hd):
     """uint8 [..., head bytes] -> the f16 values as float64"""
     if quant == pa.F16:
@@ -444,7 +460,7 @@ def test_append(ctx, dtype, quant, hd, nkv, gqa, tok, rot, inter, view):
             am = x.unflatten(-1, (hd // 32, 32)).abs().amax(-1, keepdim=True).expand(-1, -1, -1, 32).flatten(-2)
             t = am / top * (0.5 + top * 2.0 ** -11 + 2.0 ** -10) + 2.0 ** -11 * (x.abs() + am / top) + size
         assert bool(((g - x).abs() <= t + 2.0 ** -24).all())
-    # V takes no arithmetic: its rows are the package's quantiser's bytes (on the CPU: on the GPU torch divides by a
+    # V takes no arithmetic: its rows are the formula's bytes (on the CPU: on the GPU torch divides by a
     # number as it multiplies by its rounded reciprocal, and max|x| * (1/7) is not always max|x| / 7); nothing else changed
     flat = [p[sq.layer].view(-1, sq.cache.rs) for p in (sq.cache.K, sq.cache.V)]
     touched = torch.zeros(flat[0].shape[0], dtype=torch.bool, device="cuda")
@@ -452,7 +468,7 @@ def test_append(ctx, dtype, quant, hd, nkv, gqa, tok, rot, inter, view):
         js = np.arange(start[s], start[s] + tok)[real[s].cpu().numpy()]
         at = sq.rows(s, js)
         touched[at] = True
-        rows = _quantise(torch, v[s][real[s]].float().cpu(), quant).reshape(len(js), nkv * sq.hb).cuda()
+        rows = _stored(torch, v[s][real[s]].float().cpu(), quant).reshape(len(js), nkv * sq.hb).cuda()
         assert torch.equal(flat[1][at, :nkv * sq.hb], rows)
         assert bool((flat[1][at, nkv * sq.hb:] == 0xFF).all()) and bool((flat[0][at, nkv * sq.hb:] == 0xFF).all())
     for i, p in enumerate((sq.cache.K, sq.cache.V)):
