@@ -320,6 +320,10 @@ int shape_cache_plan(pa_cuda_cache_plan *p) {
         parts = std::max(parts, waves * ctx->n_sm / y);
         if ((2 * units + parts) * y > 0x7FFFFFFFull) return fail(ctx, PA_CUDA_EUNSUPPORTED, "too many rows and sets in one call");
     } else {
+        // f16 rows have this kernel for every row count: with many, a CTA's warps share fewer heads' keys between more
+        // rows (us with as many heads as fit and so: 8 sets x 8,192 keys, 8 heads x 16 rows 95 vs 72, 32 rows 197 vs 129; hd 256,
+        // 2 sets x 4,096 keys, 512 tokens x 4 heads x 6 2,378 vs 1,279)
+        if (sh.quant == PA_CUDA_F16 && p->d.n_rg > 1 && (rc = plan_decode_shape(ctx, &p->d, std::max(1u, p->d.w / p->d.n_rg)))) return rc;
         if (p->d.grid_y > 65535) return fail(ctx, PA_CUDA_EUNSUPPORTED, "too many head/row groups");
         p->kernel = "pa::dec::decode_kernel<paged>";
         int per_sm = 1;
@@ -332,6 +336,10 @@ int shape_cache_plan(pa_cuda_cache_plan *p) {
         parts = std::max<uint64_t>(1, (uint64_t) ctx->n_sm * std::max(1, per_sm) / p->d.grid_y);
         units = p->n_sets;
         p->unit_rows = sh.rows;
+        // (or, where there are about as many sets, that many four times, since few sets can be cut then and the longest one
+        // would be what the call takes: us without and with, 1 token, 256 sets of 512 to 4,096 keys 449 vs 317, 1,024 of up to
+        // 2,048 704 vs 684; 64 sets, which are cut anyway, 95 vs 106)
+        if (2 * units > parts) parts *= 4;
     }
     parts = std::min(parts, units * std::max<uint64_t>(1, groups));
     p->n_parts = (uint32_t) (units > 1 ? std::max(parts, units + 1) : parts);   // find_part: one more than the units

@@ -176,8 +176,8 @@ int check_shape(pa_cuda_ctx *ctx, const pa_cuda_shape *sh) {
     return PA_CUDA_OK;
 }
 
-// launch shape of the decode kernel for a geometry
-int plan_decode_shape(pa_cuda_ctx *ctx, pa_cuda_plan *p) {
+// launch shape of the decode kernel for a geometry (of at most max_hg heads a CTA)
+int plan_decode_shape(pa_cuda_ctx *ctx, pa_cuda_plan *p, uint32_t max_hg = ~0u) {
     const pa_cuda_shape &sh = p->sh;
     // warps per CTA (the kernel instance): 8, except 4 at hd 256 when 8 KV heads cannot share a CTA
     p->w = (sh.hd == 256 && sh.nkv % 8) ? 4 : 8;
@@ -193,7 +193,7 @@ int plan_decode_shape(pa_cuda_ctx *ctx, pa_cuda_plan *p) {
     // the largest head group that divides nkv, gives 16-byte aligned rows and fits shared memory
     uint32_t hg = 0;
     bool aligned = false;
-    for (uint32_t c = std::min(sh.nkv, maxw); c >= 1; c--) {
+    for (uint32_t c = std::min(std::min(sh.nkv, maxw), max_hg); c >= 1; c--) {
         if (sh.nkv % c) continue;
         if ((c * sh.hb) % 16) continue;
         aligned = true;
