@@ -280,8 +280,8 @@ __device__ __forceinline__ void store_head(uint8_t *head, uint32_t l, bool write
     const float df = __half2float(dh), id = df != 0.f ? __frcp_rn(df) : 0.f;
     uint8_t *blk = head + (l / 4) * dec::q_group_bytes(QUANT);
     const uint32_t in = l % 4;
-    // x / d rounded once (Markstein's correction: a quotient off by at most a unit in the last place, its exact remainder and the
-    // rounded reciprocal), so that a tie is a tie; d = 0 and d = inf give 0
+    // x / d (Markstein's correction: a quotient off by a unit or so in the last place, its exact remainder and the rounded
+    // reciprocal; a quotient that fp32 holds, as every tie of rint, comes out exactly); d = 0 and d = inf give 0
     const float dd = id != 0.f ? df : 0.f;
     uint32_t q[8];
 #pragma unroll
