@@ -327,11 +327,16 @@ int shape_cache_plan(pa_cuda_cache_plan *p) {
         if (p->d.grid_y > 65535) return fail(ctx, PA_CUDA_EUNSUPPORTED, "too many head/row groups");
         p->kernel = "pa::dec::decode_kernel<paged>";
         int per_sm = 1;
-        with_decode(p, [&](auto hd, auto q, auto w) {
+        const cudaError_t e = with_decode(p, [&](auto hd, auto q, auto w) {
             auto *k = pa::dec::decode_kernel<hd.value, q.value, w.value, true>;
-            cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, (int) p->d.smem);
-            return cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, k, 32 * (int) p->d.n_consumers, p->d.smem);
+            // the limit is the function's, shared by every plan of the instance: all that a block can have
+            cudaFuncAttributes a{};
+            cudaError_t r = cudaFuncGetAttributes(&a, k);
+            if (r == cudaSuccess) r = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxSmem - (int) a.sharedSizeBytes);
+            if (r == cudaSuccess) r = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, k, 32 * (int) p->d.n_consumers, p->d.smem);
+            return r;
         });
+        if (e != cudaSuccess) return cuda_fail(ctx, e, "cache plan: split-K kernel attributes");
         // as many CTAs as run at once
         parts = std::max<uint64_t>(1, (uint64_t) ctx->n_sm * std::max(1, per_sm) / p->d.grid_y);
         units = p->n_sets;
