@@ -369,7 +369,7 @@ __global__ void __launch_bounds__(32 * APPEND_WARPS, 6) append_kernel(const Appe
         const int64_t key = (int64_t) start + t;
         int64_t at = -1;
         const int32_t pg = key >= 0 && key < capacity(p.view)
-                               ? __ldg(p.view.table + (uint64_t) s * p.view.max_pages + (uint32_t) key / p.view.page_keys) : -1;
+                               ? p.view.table[(uint64_t) s * p.view.max_pages + (uint32_t) key / p.view.page_keys] : -1;
         if ((uint32_t) pg < p.view.n_pages) at = ((int64_t) pg * p.view.page_keys + (uint32_t) key % p.view.page_keys) * (int64_t) p.rs;
         else atomicCAS(p.view.status, ST_OK, ST_BAD_ARGS);
         s_at = at;
@@ -511,7 +511,7 @@ __global__ void __launch_bounds__(256) rows_kernel(const RowsParams p) {
     if (i >= p.n) return;
     const uint32_t s = i / p.v.n_tok, t = i % p.v.n_tok, pieces = p.nkv * (HD / 8);
     const int64_t key = (int64_t) p.first[s] + t;
-    const int32_t pg = key >= 0 && key < capacity(p.v) ? __ldg(p.v.table + (uint64_t) s * p.v.max_pages + (uint32_t) key / p.v.page_keys) : -1;
+    const int32_t pg = key >= 0 && key < capacity(p.v) ? p.v.table[(uint64_t) s * p.v.max_pages + (uint32_t) key / p.v.page_keys] : -1;
     const bool ok = (uint32_t) pg < p.v.n_pages;
     if (!ok && lane == 0) atomicCAS(p.v.status, ST_OK, ST_BAD_ARGS);
     const uint64_t at = ok ? ((uint64_t) pg * p.v.page_keys + (uint32_t) key % p.v.page_keys) * p.rs : 0;

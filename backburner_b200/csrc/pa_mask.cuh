@@ -107,9 +107,11 @@ PA_HD Span span_of(const View &v, Set st, uint32_t t0, uint32_t t1) {
     return p;
 }
 
-// page `index` of a set (a page id outside the pool is reported and replaced by page 0)
+// page `index` of a set (a page id outside the pool is reported and replaced by page 0). An ordinary load, as all loads of a
+// paged call's inputs: its kernels start while the stream's earlier ones run, so the inputs may be written in a kernel's
+// lifetime, before its pdl_wait, and non-coherent loads (__ldg) are for data that nobody writes in it.
 __device__ __forceinline__ uint32_t page_of(const View &v, uint32_t s, uint32_t index) {
-    const int32_t p = __ldg(v.table + (uint64_t) s * v.max_pages + index);
+    const int32_t p = v.table[(uint64_t) s * v.max_pages + index];
     if ((uint32_t) p < v.n_pages) return (uint32_t) p;
     atomicCAS(v.status, ST_OK, ST_BAD_ARGS);
     return 0;

@@ -563,7 +563,9 @@ __global__ void __launch_bounds__(32 * cta_warps(NT), 1) prefill_kernel(const __
                     uint32_t qv[32];
 #pragma unroll
                     for (int i = 0; i < 8; i++) {
-                        const uint4 v = row < p.rows ? __ldg(src + 8 * c + i) : make_uint4(0u, 0u, 0u, 0u);
+                        // (PAGED: ordinary loads, since the kernel may be running while its Q is written, before pdl_wait)
+                        uint4 v = make_uint4(0u, 0u, 0u, 0u);
+                        if (row < p.rows) v = PAGED ? src[8 * c + i] : __ldg(src + 8 * c + i);
                         qv[4 * i] = v.x; qv[4 * i + 1] = v.y; qv[4 * i + 2] = v.z; qv[4 * i + 3] = v.w;
                     }
                     tmem_st32u(tl + T_Q + 32 * c, qv);

@@ -27,3 +27,64 @@ def test_plans_of_one_kernel_keep_their_shared_memory(ctx, quant, first, second)
         _check(sq, Qs, out, tok, 1)
     for _, _, plan in made:
         plan.close()
+
+
+@pytest.mark.parametrize("kernel,tok", [(1, 1), (1, 7), (2, 7), (2, 60), (3, 60)])
+@pytest.mark.parametrize("captured", [False, True])
+def test_steps_that_reuse_their_buffers(ctx, kernel, tok, captured):
+    """append, then attention on the queries it has just written, over a table written just before: one set of buffers for
+    every step, the steps back to back, each as if it were alone"""
+    import torch
+    S, hd, nkv, gqa, steps = 3, 128, 8, 5, 6
+    g = torch.Generator(device="cuda")
+    g.manual_seed(kernel + tok)
+    c = pa.Cache(hd, nkv, pa.Q8_0, 1, 64, 64)
+    tables = [torch.randperm(64, generator=g, device="cuda")[:S * 8].view(S, 8).int() for _ in range(steps)]
+    xs = [[torch.randn(S, tok, n, hd, generator=g, device="cuda") for n in (nkv * gqa, nkv, nkv)] for _ in range(steps)]
+    for p in (c.K, c.V):   # every row of the pool is finite
+        p.copy_(pa.quantize_q8_0(torch.randn(64 * 64, nkv, hd, generator=g, device="cuda")).reshape(p.shape))
+    pool = [p.clone() for p in (c.K, c.V)]
+    start = torch.tensor([300, 0, 129], dtype=torch.int32, device="cuda")
+    n = start + tok
+    ctx.set_kernel(kernel)
+    plan = pa.CachePlan(ctx, c, S, tok, gqa, 8)
+    ctx.set_kernel(0)
+    x, table = [t.clone() for t in xs[0]], tables[0].clone()
+    Qs = torch.empty(S, nkv, gqa * tok, hd, dtype=torch.float16, device="cuda")
+    out = torch.empty_like(Qs), torch.empty(S, nkv, gqa * tok, device="cuda")
+    want = []
+    for i in range(steps):   # each step alone
+        for p, was in zip((c.K, c.V), pool):
+            p.copy_(was)
+        q = pa.cache_append(ctx, c, 0, *xs[i], tables[i], start, scale=hd ** -0.5)
+        torch.cuda.synchronize()
+        o = plan.reply(0, q, tables[i], n)
+        torch.cuda.synchronize()
+        want.append([t.clone() for t in (q, *o)])
+
+    def step():
+        pa.cache_append(ctx, c, 0, *x, table, start, scale=hd ** -0.5, out=Qs)
+        plan.reply(0, Qs, table, n, out=out)
+
+    run = step
+    if captured:
+        graph = torch.cuda.CUDAGraph()
+        step()
+        torch.cuda.synchronize()
+        with torch.cuda.graph(graph):
+            step()
+        run = graph.replay
+    got = []
+    for i in range(steps):
+        for p, was in zip((c.K, c.V), pool):
+            p.copy_(was)
+        for a, b in zip(x, xs[i]):
+            a.copy_(b)
+        table.copy_(tables[i])
+        run()
+        got.append([t.clone() for t in (Qs, *out)])
+    torch.cuda.synchronize()
+    ctx.status()
+    for a, b in zip(got, want):
+        assert all(torch.equal(u, v) for u, v in zip(a, b))
+    plan.close()
