@@ -271,24 +271,25 @@ __device__ __forceinline__ void store_head(uint8_t *head, uint32_t l, bool write
         return;
     }
     constexpr float TOP = QUANT == 1 ? 127.f : 7.f;
-    float am = 0.f;
+    float am = 0.f;   // NaN if a value is: then d is, and with it every value of the block
 #pragma unroll
-    for (int e = 0; e < 8; e++) am = fmaxf(am, fabsf(x[e]));
-    am = fmaxf(am, __shfl_xor_sync(0xffffffffu, am, 1));
-    am = fmaxf(am, __shfl_xor_sync(0xffffffffu, am, 2));
+    for (int e = 0; e < 8; e++) am = max_nan(am, fabsf(x[e]));
+    am = max_nan(am, __shfl_xor_sync(0xffffffffu, am, 1));
+    am = max_nan(am, __shfl_xor_sync(0xffffffffu, am, 2));
     const __half dh = __float2half_rn(__fdiv_rn(am, TOP));
     const float df = __half2float(dh), id = df != 0.f ? __frcp_rn(df) : 0.f;
     uint8_t *blk = head + (l / 4) * dec::q_group_bytes(QUANT);
     const uint32_t in = l % 4;
     // x / d (Markstein's correction: a quotient off by a unit or so in the last place, its exact remainder and the rounded
-    // reciprocal; a quotient that fp32 holds, as every tie of rint, comes out exactly); d = 0 and d = inf give 0
+    // reciprocal; a quotient that fp32 holds, as every tie of rint, comes out exactly). d = 0 gives 0; so do d = inf and d = NaN,
+    // the quotients without a value among them (the conversion turns NaN into 0), so that the block reads as NaN
     const float dd = id != 0.f ? df : 0.f;
     uint32_t q[8];
 #pragma unroll
     for (int e = 0; e < 8; e++) {
         float y = __fmul_rn(x[e], id);
         y = fmaf(fmaf(-y, dd, x[e]), id, y);
-        q[e] = (uint32_t) __float2int_rn(fmaxf(-TOP, fminf(TOP, y)));
+        q[e] = (uint32_t) max(-(int) TOP, min((int) TOP, __float2int_rn(y)));
     }
     if (write && in == 0) *reinterpret_cast<__half *>(blk) = dh;
     uint16_t *dst = reinterpret_cast<uint16_t *>(blk + 2 + 8 * in);   // blocks start at even bytes: 16-bit stores

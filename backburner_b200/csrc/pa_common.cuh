@@ -156,6 +156,13 @@ __device__ __forceinline__ void stg_f8(float *p, const float (&x)[8]) {
                  : "memory");
 }
 
+// the larger one, NaN where either is (fmaxf drops it)
+__device__ __forceinline__ float max_nan(float a, float b) {
+    float r;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+    return r;
+}
+
 // transpose of an 8x8 b16 matrix held in mma fragment order (one .b32 per lane)
 __device__ __forceinline__ uint32_t movtrans(uint32_t x) {
     uint32_t d;

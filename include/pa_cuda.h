@@ -319,7 +319,9 @@ typedef struct pa_cuda_append {
 /* For every token: y = x * rsqrt(mean(x^2) + eps) * w for its query and key heads, the first rot dims of y turned by
  * pos * freqs; Qs [n_sets][nkv][gqa * n_tok][hd] = f16(y * scale) (rows g * n_tok + t, what the attention calls take), the
  * key heads and the value heads as they are stored as the cache row of key start[s] + t, quantised as the format says
- * (d = f16(max|x| / 127 or 7), q = rint(x / d), the quotients as fp32 rounds them). fp32 arithmetic, angles in fp64.
+ * (d = f16(max|x| / 127 or 7), q = rint(x / d), the quotients as fp32 rounds them). fp32 arithmetic, angles in fp64. A block
+ * with a NaN gets d = NaN, one with an infinity (or past f16's range: max|x| / 127 or 7 above 65,504) d = inf and q = 0: all
+ * its values read as NaN. f16 rows keep NaN and infinities where they are.
  * Padding: Qs = 0, nothing stored. shape->rows = gqa * n_tok. Bytes of a row past nkv * hb are left as they are. */
 int pa_cuda_cache_append(pa_cuda_ctx *ctx, const pa_cuda_shape *shape, const pa_cuda_cache *cache, uint32_t layer,
                          const pa_cuda_append *in, uint32_t n_sets, uint32_t n_tok, const int32_t *table, uint32_t max_pages,

@@ -88,3 +88,38 @@ def test_steps_that_reuse_their_buffers(ctx, kernel, tok, captured):
     for a, b in zip(got, want):
         assert all(torch.equal(u, v) for u, v in zip(a, b))
     plan.close()
+
+
+@pytest.mark.parametrize("quant", [pa.F16, pa.Q8_0, pa.Q4_0])
+@pytest.mark.parametrize("dtype", ["float32", "float16"])
+def test_append_keeps_what_is_not_a_number(ctx, quant, dtype):
+    """a NaN, an infinity of either sign and (fp32) a value whose block's d passes f16's range: the block reads as NaN, every
+    other block as if it were not there; f16 rows keep each element. With a norm a NaN takes its head with it."""
+    import torch
+    nkv, hd, tok = 8, 128, 6
+    bad = [float("nan"), float("inf"), -float("inf")] + ([1e7, -1e30] if dtype == "float32" else [])
+    sq = Seqs(1, [0], hd, nkv, quant, 64, extra=tok)
+    x = [torch.randn(1, tok, n, hd, generator=sq.g, device="cuda").to(getattr(torch, dtype)) for n in (nkv, nkv, nkv)]
+    st = torch.tensor([0], dtype=torch.int32, device="cuda")
+    pa.cache_append(ctx, sq.cache, 0, *x, sq.table, st)
+    clean = [t.clone() for t in pa.cache_rows(ctx, sq.cache, 0, sq.table, st, tok)]
+    y = [t.clone() for t in x]
+    want = [t.clone() for t in clean]
+    for i, b in enumerate(bad):
+        for kv in range(2):
+            h, d = (3 * i + kv) % nkv, (37 * i + 5 * kv) % hd   # (lanes, halves of a nibble pair and blocks of every kind)
+            y[1 + kv][0, i, h, d] = b
+            if quant == pa.F16:
+                want[kv][0, i, h, d] = b   # 1e7 and -1e30 are infinities in f16
+            else:
+                want[kv][0, i, h, d // 32 * 32:d // 32 * 32 + 32] = float("nan")
+    pa.cache_append(ctx, sq.cache, 0, *y, sq.table, st)
+    got = pa.cache_rows(ctx, sq.cache, 0, sq.table, st, tok)
+    ctx.status()
+    for g, w in zip(got, want):
+        assert torch.equal(torch.isnan(g), torch.isnan(w)) and torch.equal(torch.nan_to_num(g), torch.nan_to_num(w))
+    w = torch.ones(hd, device="cuda")
+    Qs = pa.cache_append(ctx, sq.cache, 0, *y, sq.table, st, wq=w, wk=w)
+    K, _ = pa.cache_rows(ctx, sq.cache, 0, sq.table, st, tok)
+    ctx.status()
+    assert bool(torch.isnan(K[0, 0, 0]).all()) and not torch.isnan(K[0, 0, 1:]).any() and not torch.isnan(Qs).any()
