@@ -339,7 +339,8 @@ __global__ void __launch_bounds__(32 * APPEND_WARPS, 6) append_kernel(const Appe
     pdl_wait();
     const int start = p.start[s];
     const int pos = p.pos ? p.pos[(uint64_t) s * T + t] : clampi((int64_t) start + t, -1, INT32_MAX);
-    if (pos < 0) {   // padding: its query rows are zero
+    if (pos < 0) {   // padding, or without positions a key before the first one: its query rows are zero
+        if (!p.pos && blockIdx.z == 0 && threadIdx.x == 0) atomicCAS(p.view.status, ST_OK, ST_BAD_ARGS);
 #pragma unroll 1
         for (uint32_t h = hw0 + sub; h < hw0 + HPB * STEPS && h < nq; h += HPB)
             *reinterpret_cast<uint4 *>(p.Qs + (((uint64_t) s * nq + h) * T + t) * HD + 8 * l) = make_uint4(0u, 0u, 0u, 0u);

@@ -123,3 +123,24 @@ def test_append_keeps_what_is_not_a_number(ctx, quant, dtype):
     K, _ = pa.cache_rows(ctx, sq.cache, 0, sq.table, st, tok)
     ctx.status()
     assert bool(torch.isnan(K[0, 0, 0]).all()) and not torch.isnan(K[0, 0, 1:]).any() and not torch.isnan(Qs).any()
+
+
+@pytest.mark.parametrize("start,bad", [(-1, True), (-2 ** 31, True), (0, False), (64 * 5 - 3, False), (64 * 5 - 2, True), (2 ** 31 - 1, True)])
+def test_append_without_positions_reports_keys_out_of_reach(ctx, start, bad):
+    """a start before key 0, or one whose tokens pass the table, is reported whether the call gives positions or not"""
+    import torch
+    sq = Seqs(3, [0, 0], 128, 8, pa.Q8_0, 64, extra=64 * 4)   # (the table has an entry more, outside the pool)
+    table = torch.arange(10, dtype=torch.int32, device="cuda").view(2, 5)
+    x = [torch.randn(2, 3, n, 128, generator=sq.g, device="cuda") for n in (40, 8, 8)]
+    st = torch.tensor([5, start], dtype=torch.int32, device="cuda")
+    pos = torch.zeros(2, 3, dtype=torch.int32, device="cuda")
+    for kw in ({}, dict(pos=pos)):
+        pa.cache_append(ctx, sq.cache, 0, *x, table, st, **kw)
+        if bad:
+            with pytest.raises(pa.PaCudaError) as e:
+                ctx.status()
+            assert e.value.code == api.EINVAL
+        ctx.status()
+    # padding is none of this, wherever its sequence starts
+    pa.cache_append(ctx, sq.cache, 0, *x, table, st, pos=torch.tensor([[0, 0, 0], [-1, -1, -1]], dtype=torch.int32, device="cuda"))
+    ctx.status()
