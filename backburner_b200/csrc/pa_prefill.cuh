@@ -225,6 +225,58 @@ struct Smem {
     static constexpr int TOTAL = BAR + N_BAR * 8 + 32;
 };
 
+// The words of a quant block (from 16-byte aligned shared memory, the block's data at word w0 and `shift` bits into it; sc2: its
+// d twice) as f16 into the operand buffer: atom row kbase of `key`, columns of qblk. w0 and qblk are uniform across the warp.
+template <int QUANT>
+__device__ __forceinline__ void convert_block(const uint32_t (&w)[12], uint32_t sc2, uint32_t w0, uint32_t shift, uint32_t kbase,
+                                              uint32_t qblk, uint32_t key) {
+    if (QUANT == 1) {
+        uint32_t A[8];
+        switch (w0) {   // uniform across the warp
+#define PA_ALIGN8(W0)                                                                        \
+    case W0:                                                                                 \
+        _Pragma("unroll") for (int i = 0; i < 8; i++) A[i] = __funnelshift_r(w[W0 + i], w[(W0 + i + 1 < 12) ? W0 + i + 1 : 11], shift); \
+        break;
+            PA_ALIGN8(0) PA_ALIGN8(1) PA_ALIGN8(2) PA_ALIGN8(3) default: PA_ALIGN8(4)
+#undef PA_ALIGN8
+        }
+#pragma unroll
+        for (int cc = 0; cc < 4; cc++) {
+            uint32_t h0, h1, h2, h3;
+            dec::q8_word(A[2 * cc], sc2, h0, h1);
+            dec::q8_word(A[2 * cc + 1], sc2, h2, h3);
+            const uint32_t c = 4 * (qblk % 2) + cc;
+            sts128(kbase + ((c ^ (key % 8)) * 16), h0, h1, h2, h3);
+        }
+    } else {
+        uint32_t AW[4];
+        switch (w0) {
+#define PA_ALIGN4(W0)                                                                        \
+    case W0:                                                                                 \
+        _Pragma("unroll") for (int i = 0; i < 4; i++) AW[i] = __funnelshift_r(w[W0 + i], w[W0 + i + 1], shift); \
+        break;
+            PA_ALIGN4(0) PA_ALIGN4(1) PA_ALIGN4(2) PA_ALIGN4(3) default: PA_ALIGN4(4)
+#undef PA_ALIGN4
+        }
+        // byte i: element i (low nibble), element i + 16 (high nibble)
+        uint32_t lo[8], hi[8];   // f16x2 of elements (2i, 2i+1) and (16+2i, 17+2i)
+        const uint32_t m = 0x000F000Fu, magic = 0x64006400u, off8 = 0x64086408u;
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const uint32_t y = prmt(AW[i], AW[i], 0x3120u);   // bytes (x0, x2, x1, x3)
+            lo[2 * i] = hmul2(hsub2(and_or(y, m, magic), off8), sc2);
+            lo[2 * i + 1] = hmul2(hsub2(and_or(y >> 8, m, magic), off8), sc2);
+            hi[2 * i] = hmul2(hsub2(and_or(y >> 4, m, magic), off8), sc2);
+            hi[2 * i + 1] = hmul2(hsub2(and_or(y >> 12, m, magic), off8), sc2);
+        }
+        const uint32_t c0 = 4 * (qblk % 2);
+        sts128(kbase + (((c0 + 0) ^ (key % 8)) * 16), lo[0], lo[1], lo[2], lo[3]);
+        sts128(kbase + (((c0 + 1) ^ (key % 8)) * 16), lo[4], lo[5], lo[6], lo[7]);
+        sts128(kbase + (((c0 + 2) ^ (key % 8)) * 16), hi[0], hi[1], hi[2], hi[3]);
+        sts128(kbase + (((c0 + 3) ^ (key % 8)) * 16), hi[4], hi[5], hi[6], hi[7]);
+    }
+}
+
 // PAGED: the keys come from a paged cache and the rows see them through a mask (pa_mask.cuh). A block is B / 64 groups of 64
 // keys, each copied from its own page; the CTA walks its share of the groups its own row tile sees. Only groups at the edge of
 // what the tile's rows see are masked (a thread has its row's 64-bit word for the group); keys no row of the tile sees get a
@@ -395,7 +447,7 @@ __global__ void __launch_bounds__(32 * cta_warps(NT), 1) prefill_kernel(const __
       else if constexpr (!PAGED && NT == 1 && B == 64) asm volatile("setmaxnreg.inc.sync.aligned.u32 160;");
       if (warp == 0) {
         // ------------------------------------------------ TMA producer
-        if (lane == 0) {
+        auto load_q = [&]() {
             if constexpr (!QT) {
                 const int qrow = (int) (((uint64_t) (PAGED ? s_part.set : job.set) * p.nkv + h) * p.rows + row0);
                 mbar_arrive_expect_tx(q_full, nt * BM * D * 2);
@@ -403,11 +455,23 @@ __global__ void __launch_bounds__(32 * cta_warps(NT), 1) prefill_kernel(const __
                     for (int c = 0; c < D / 64; c++)
                         tma_2d(smem + L::Q + t * BM * D * 2 + c * BM * 128, &tq, c * 64, qrow + t * BM, q_full);
             }
-        }
-        const CUtensorMap *km = p.kv_maps + (PAGED ? 0 : 2 * job.seg), *vm = km + 1;
-        uint32_t issued = 0;
-        if constexpr (!PAGED) {
-            if (lane == 0)
+        };
+        // on an abort, every issued copy lands before the CTA exits
+        auto drain = [&](uint32_t issued) {
+            if (!ok) {
+                const uint64_t limit = tmo > dec::DRAIN_NS ? tmo : dec::DRAIN_NS;
+                if (!QT && !mbar_wait_bounded(q_full, 0, limit, nullptr)) atomicCAS(p.status, ST_OK, ST_TIMEOUT_DRAIN);
+                const uint32_t first = issued > NRS ? issued - NRS : 0;
+                for (uint32_t j = first; j < issued; j++)
+                    if (!mbar_wait_bounded(&raw_full[j % NRS], (j / NRS) & 1, limit, nullptr))
+                        atomicCAS(p.status, ST_OK, ST_TIMEOUT_DRAIN);
+            }
+        };
+        if constexpr (!PAGED) {   // (all in one lane's block: three blocks cost two-tile calls 1 %)
+            if (lane == 0) {
+                load_q();
+                const CUtensorMap *km = p.kv_maps + 2 * job.seg, *vm = km + 1;
+                uint32_t issued = 0;
                 for (uint32_t j = 0; j < nblk; j++) {
                     const uint32_t st = j % NRS;
                     if (j >= NRS && !wait(&raw_empty[st], ((j / NRS) - 1) & 1)) break;
@@ -421,7 +485,12 @@ __global__ void __launch_bounds__(32 * cta_warps(NT), 1) prefill_kernel(const __
                     }
                     issued = j + 1;
                 }
+                drain(issued);
+            }
         } else {
+            if (lane == 0) load_q();
+            const CUtensorMap *km = p.kv_maps, *vm = km + 1;
+            uint32_t issued = 0;
             const pg::Span span = pg::span_of<64>(p.pg.v, s_part.st, s_part.t0, s_part.t1);
             uint32_t pg0, pgn;   // this CTA's groups [pg0, pg0 + pgn) of its unit's span
             s_part.share((uint32_t) span.n, pg0, pgn);
@@ -454,17 +523,7 @@ __global__ void __launch_bounds__(32 * cta_warps(NT), 1) prefill_kernel(const __
                 }
                 if (!__shfl_sync(0xffffffffu, ok, 0)) break;
             }
-        }
-        if (lane == 0) {
-            // on an abort, every issued copy lands before the CTA exits
-            if (!ok) {
-                const uint64_t drain = tmo > dec::DRAIN_NS ? tmo : dec::DRAIN_NS;
-                if (!QT && !mbar_wait_bounded(q_full, 0, drain, nullptr)) atomicCAS(p.status, ST_OK, ST_TIMEOUT_DRAIN);
-                const uint32_t first = issued > NRS ? issued - NRS : 0;
-                for (uint32_t j = first; j < issued; j++)
-                    if (!mbar_wait_bounded(&raw_full[j % NRS], (j / NRS) & 1, drain, nullptr))
-                        atomicCAS(p.status, ST_OK, ST_TIMEOUT_DRAIN);
-            }
+            if (lane == 0) drain(issued);
         }
       } else if (warp == 1 || warp == 2) {
         // ------------------------------------------------ MMA issuers: warp 1 the S = Q K^T MMAs, warp 2 the P.V ones.
@@ -742,108 +801,91 @@ __global__ void __launch_bounds__(32 * cta_warps(NT), 1) prefill_kernel(const __
                 for (int c = 0; c < B / 64; c++) edge |= (int) *(volatile uint32_t *) &s_group[(j * (B / 64) + c) % 64] < 0;
             }
             // Items of the block for this warp: 64-key chunk kc, key half (8 warps) or pass (4 warps), quant block of the
-            // warp; K's, then V's. AHEAD: an item's words are loaded while the one before it is converted (the loads and
-            // stores are ordered among themselves, so without this every item waits out its own shared-memory latency).
+            // warp; K's, then V's
             constexpr int NI = (B / 64) * (8 / NDQ) * (D / 128);
-            uint32_t W[2][12], S2[2];
             auto qblk_of = [&](int it) -> uint32_t { return dw % 4 + 4 * (uint32_t) (it / ((8 / NDQ) * (B / 64))); };
             auto key_of = [&](int it) -> uint32_t {
                 return 64 * (uint32_t) (it / (8 / NDQ) % (B / 64)) + (NDQ == 8 ? dw / 4 : (uint32_t) (it % (8 / NDQ))) * 32 + lane;
             };
-            auto load = [&](int x, uint32_t (&w)[12], uint32_t &sc2) {
-                const int kv = x / NI, it = x % NI;
-                const uint32_t bo = hoff + GB * qblk_of(it);   // block start inside the raw window row
-                const uint32_t w16 = bo & ~15u;                // 16-byte aligned start of the words covering it
-                const uint32_t rb = raw + kv * B * RAWB + key_of(it) * RAWB;
-                const uint32_t s2 = lds16(rb + bo);
-                sc2 = s2 | (s2 << 16);
-                // q8_0: the block's 34 bytes lie within 3 aligned 16-byte chunks; q4_0: 18 bytes within 2
-#pragma unroll
-                for (int i = 0; i < (QUANT == 1 ? 3 : 2); i++) lds128(rb + w16 + 16 * i, w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
-                if (QUANT != 1) w[8] = w[9] = w[10] = w[11] = 0u;
-            };
-            if constexpr (AHEAD) load(0, W[0], S2[0]);
-#pragma unroll
-            for (int x = 0; x < 2 * NI; x++) {
-                const int kv = x / NI, it = x % NI;
-                if (it == 0 && j >= KVB && !wait(kv == 0 ? &k_free[b] : &v_free[b], ((j / KVB) - 1) & 1)) break;
-                if (!AHEAD) {
-                    load(x, W[x & 1], S2[x & 1]);
-                } else if (x + 1 < 2 * NI) {
-                    load(x + 1, W[(x + 1) & 1], S2[(x + 1) & 1]);
-                } else {   // the raw stage is read
-                    __syncwarp();
-                    if (lane == 0) mbar_arrive(&raw_empty[st]);
-                }
-                const uint32_t (&w)[12] = W[x & 1];
-                const uint32_t sc2 = S2[x & 1], qblk = qblk_of(it), key = key_of(it);
-                const uint32_t bo = hoff + GB * qblk, ds = bo + 2;                       // first data byte
-                const uint32_t w0 = (ds - (bo & ~15u)) / 4, shift = 8 * (ds % 4);
-                // atom column of this block's d's
-                const uint32_t dst = sbase + (kv == 0 ? L::K : L::V) + b * B * D * 2 + (qblk / 2) * B * 128;
-                const uint32_t kbase = dst + (key / 8) * 1024 + (key % 8) * 128;
-                if (QUANT == 1) {
-                    uint32_t A[8];
-                    switch (w0) {   // uniform across the warp
-#define PA_ALIGN8(W0)                                                                        \
-    case W0:                                                                                 \
-        _Pragma("unroll") for (int i = 0; i < 8; i++) A[i] = __funnelshift_r(w[W0 + i], w[(W0 + i + 1 < 12) ? W0 + i + 1 : 11], shift); \
-        break;
-                        PA_ALIGN8(0) PA_ALIGN8(1) PA_ALIGN8(2) PA_ALIGN8(3) default: PA_ALIGN8(4)
-#undef PA_ALIGN8
-                    }
-#pragma unroll
-                    for (int cc = 0; cc < 4; cc++) {
-                        uint32_t h0, h1, h2, h3;
-                        dec::q8_word(A[2 * cc], sc2, h0, h1);
-                        dec::q8_word(A[2 * cc + 1], sc2, h2, h3);
-                        const uint32_t c = 4 * (qblk % 2) + cc;
-                        sts128(kbase + ((c ^ (key % 8)) * 16), h0, h1, h2, h3);
-                    }
-                } else {
-                    uint32_t AW[4];
-                    switch (w0) {
-#define PA_ALIGN4(W0)                                                                        \
-    case W0:                                                                                 \
-        _Pragma("unroll") for (int i = 0; i < 4; i++) AW[i] = __funnelshift_r(w[W0 + i], w[W0 + i + 1], shift); \
-        break;
-                        PA_ALIGN4(0) PA_ALIGN4(1) PA_ALIGN4(2) PA_ALIGN4(3) default: PA_ALIGN4(4)
-#undef PA_ALIGN4
-                    }
-                    // byte i: element i (low nibble), element i + 16 (high nibble)
-                    uint32_t lo[8], hi[8];   // f16x2 of elements (2i, 2i+1) and (16+2i, 17+2i)
-                    const uint32_t m = 0x000F000Fu, magic = 0x64006400u, off8 = 0x64086408u;
-#pragma unroll
-                    for (int i = 0; i < 4; i++) {
-                        const uint32_t y = prmt(AW[i], AW[i], 0x3120u);   // bytes (x0, x2, x1, x3)
-                        lo[2 * i] = hmul2(hsub2(and_or(y, m, magic), off8), sc2);
-                        lo[2 * i + 1] = hmul2(hsub2(and_or(y >> 8, m, magic), off8), sc2);
-                        hi[2 * i] = hmul2(hsub2(and_or(y >> 4, m, magic), off8), sc2);
-                        hi[2 * i + 1] = hmul2(hsub2(and_or(y >> 12, m, magic), off8), sc2);
-                    }
-                    const uint32_t c0 = 4 * (qblk % 2);
-                    sts128(kbase + (((c0 + 0) ^ (key % 8)) * 16), lo[0], lo[1], lo[2], lo[3]);
-                    sts128(kbase + (((c0 + 1) ^ (key % 8)) * 16), lo[4], lo[5], lo[6], lo[7]);
-                    sts128(kbase + (((c0 + 2) ^ (key % 8)) * 16), hi[0], hi[1], hi[2], hi[3]);
-                    sts128(kbase + (((c0 + 3) ^ (key % 8)) * 16), hi[4], hi[5], hi[6], hi[7]);
-                }
-                if (it + 1 == NI) {
-                    if constexpr (PAGED) {
-                        if (kv == 1 && edge) {   // V rows that no row sees may hold anything (NaN): cleared (rolled: rare)
+            auto done = [&](int kv) {   // K or V of the block is converted
+                if constexpr (PAGED) {
+                    if (kv == 1 && edge) {   // V rows that no row sees may hold anything (NaN): cleared (rolled: rare)
 #pragma unroll 1
-                            for (int z = 0; z < NI; z++) {
-                                const uint32_t k = key_of(z), qb = qblk_of(z);
-                                const uint32_t g = (j * (B / 64) + k / 64) % 64;
-                                if ((int) *(volatile uint32_t *) &s_group[g] >= 0 || (s_live[g] >> (k % 64) & 1ull)) continue;
-                                const uint32_t kb = sbase + L::V + b * B * D * 2 + (qb / 2) * B * 128 + (k / 8) * 1024 + (k % 8) * 128;
+                        for (int z = 0; z < NI; z++) {
+                            const uint32_t k = key_of(z), qb = qblk_of(z);
+                            const uint32_t g = (j * (B / 64) + k / 64) % 64;
+                            if ((int) *(volatile uint32_t *) &s_group[g] >= 0 || (s_live[g] >> (k % 64) & 1ull)) continue;
+                            const uint32_t kb = sbase + L::V + b * B * D * 2 + (qb / 2) * B * 128 + (k / 8) * 1024 + (k % 8) * 128;
 #pragma unroll 1
-                                for (uint32_t c = 4 * (qb % 2); c < 4 * (qb % 2) + 4; c++) sts128(kb + ((c ^ (k % 8)) * 16), 0u, 0u, 0u, 0u);
-                            }
+                            for (uint32_t c = 4 * (qb % 2); c < 4 * (qb % 2) + 4; c++) sts128(kb + ((c ^ (k % 8)) * 16), 0u, 0u, 0u, 0u);
                         }
                     }
-                    fence_proxy_async();
-                    __syncwarp();
-                    if (lane == 0) mbar_arrive(kv == 0 ? &k_full[b] : &v_full[b]);
+                }
+                fence_proxy_async();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(kv == 0 ? &k_full[b] : &v_full[b]);
+            };
+            if constexpr (AHEAD) {
+                // An item's words are loaded while the one before it is converted (the loads and stores are ordered among
+                // themselves, so without this every item waits out its own shared-memory latency). The instances without it
+                // keep a loop of their own: run through this one's, Q8_0 with two tiles spills (200 rows: 1 % more)
+                uint32_t W[2][12], S2[2];
+                auto load = [&](int x, uint32_t (&w)[12], uint32_t &sc2) {
+                    const int kv = x / NI, it = x % NI;
+                    const uint32_t bo = hoff + GB * qblk_of(it);   // block start inside the raw window row
+                    const uint32_t w16 = bo & ~15u;                // 16-byte aligned start of the words covering it
+                    const uint32_t rb = raw + kv * B * RAWB + key_of(it) * RAWB;
+                    const uint32_t s2 = lds16(rb + bo);
+                    sc2 = s2 | (s2 << 16);
+                    // q8_0: the block's 34 bytes lie within 3 aligned 16-byte chunks; q4_0: 18 bytes within 2
+#pragma unroll
+                    for (int i = 0; i < (QUANT == 1 ? 3 : 2); i++) lds128(rb + w16 + 16 * i, w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
+                    if (QUANT != 1) w[8] = w[9] = w[10] = w[11] = 0u;
+                };
+                load(0, W[0], S2[0]);
+#pragma unroll
+                for (int x = 0; x < 2 * NI; x++) {
+                    const int kv = x / NI, it = x % NI;
+                    if (it == 0 && j >= KVB && !wait(kv == 0 ? &k_free[b] : &v_free[b], ((j / KVB) - 1) & 1)) break;
+                    if (x + 1 < 2 * NI) {
+                        load(x + 1, W[(x + 1) & 1], S2[(x + 1) & 1]);
+                    } else {   // the raw stage is read
+                        __syncwarp();
+                        if (lane == 0) mbar_arrive(&raw_empty[st]);
+                    }
+                    const uint32_t qblk = qblk_of(it), key = key_of(it);
+                    const uint32_t bo = hoff + GB * qblk, ds = bo + 2;                       // first data byte
+                    // atom column of this block's d's
+                    const uint32_t dst = sbase + (kv == 0 ? L::K : L::V) + b * B * D * 2 + (qblk / 2) * B * 128;
+                    convert_block<QUANT>(W[x & 1], S2[x & 1], (ds - (bo & ~15u)) / 4, 8 * (ds % 4), dst + (key / 8) * 1024 + (key % 8) * 128, qblk, key);
+                    if (it + 1 == NI) done(kv);
+                }
+            } else {
+#pragma unroll
+                for (int kv = 0; kv < 2; kv++) {
+                    if (j >= KVB && !wait(kv == 0 ? &k_free[b] : &v_free[b], ((j / KVB) - 1) & 1)) break;
+                    const uint32_t src = raw + kv * B * RAWB;
+#pragma unroll
+                    for (int it = 0; it < NI; it++) {
+                        const uint32_t qblk = qblk_of(it);
+                        const uint32_t bo = hoff + GB * qblk;               // block start inside the raw window row
+                        const uint32_t w16 = bo & ~15u;                     // 16-byte aligned start of the words covering it
+                        const uint32_t ds = bo + 2;                         // first data byte
+                        const uint32_t w0 = (ds - w16) / 4, shift = 8 * (ds % 4);
+                        // atom column of this block's d's
+                        const uint32_t dst = sbase + (kv == 0 ? L::K : L::V) + b * B * D * 2 + (qblk / 2) * B * 128;
+                        const uint32_t key = key_of(it);
+                        const uint32_t rb = src + key * RAWB;
+                        const uint32_t s2 = lds16(rb + bo);
+                        const uint32_t sc2 = s2 | (s2 << 16);
+                        uint32_t W[12];
+#pragma unroll
+                        for (int i = 0; i < (QUANT == 1 ? 3 : 2); i++)
+                            lds128(rb + w16 + 16 * i, W[4 * i], W[4 * i + 1], W[4 * i + 2], W[4 * i + 3]);
+                        if (QUANT != 1) W[8] = W[9] = W[10] = W[11] = 0u;
+                        convert_block<QUANT>(W, sc2, w0, shift, dst + (key / 8) * 1024 + (key % 8) * 128, qblk, key);
+                    }
+                    done(kv);
                 }
             }
             if (!ok) break;
