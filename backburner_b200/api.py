@@ -550,17 +550,48 @@ def _want(ctx: Context, t, name: str, dtype, shape):
     return t.data_ptr()
 
 
-def _stream_on(ctx: Context, stream) -> int:
-    """_stream_ptr for the context's device, whatever the current one is."""
+def _stream_on(ctx: Context, stream):
+    """_stream_ptr for the context's device, whatever the current one is; and the torch stream where it is another than the
+    device's current one (else None)."""
+    import torch
+    here = torch._C._cuda_getCurrentRawStream(ctx.device) or 1   # (current_stream's handle, without its Stream object)
     if stream is None:
-        import torch
-        return torch._C._cuda_getCurrentRawStream(ctx.device) or 1   # (current_stream's handle, without its Stream object)
-    return _stream_ptr(stream)
+        return here, None
+    if isinstance(stream, torch.cuda.Stream) and stream.device_index != ctx.device:
+        raise PaCudaError(EINVAL, f"the stream is on cuda:{stream.device_index}, the context on cuda:{ctx.device}")
+    h = int(getattr(stream, "cuda_stream", stream)) or 1     # (1: cudaStreamLegacy, torch's default stream)
+    if h == here:
+        return h, None
+    if not isinstance(stream, torch.cuda.Stream):
+        stream = torch.cuda.default_stream(ctx.device) if h == 1 else torch.cuda.ExternalStream(h, device=ctx.device)
+    return h, stream
+
+
+def _there(side, like, *kinds):
+    """Outputs (shape, type) on like's device, for a call on a stream of its own: allocated on that stream, since memory of the
+    current one may still be read by work that is queued on it, and held for the current stream's use too."""
+    import torch
+    with torch.cuda.stream(side):
+        out = tuple(like.new_empty(shape, dtype=dtype) for shape, dtype in kinds)
+    for t in out:
+        t.record_stream(torch.cuda.current_stream(t.device))
+    return out
+
+
+def _keep(side, *tensors):
+    """What a call on a stream of its own reads and writes is not given out again before that stream is done with it."""
+    for t in tensors:
+        if t is not None:
+            t.record_stream(side)
 
 
 class Cache:
     """A paged device cache (pa_cuda_cache): K and V uint8 [n_layers][n_pages][page_keys][row bytes] on one device, rows of
-    nkv heads in the F16, Q8_0 or Q4_0 format. Tables, lengths and positions stay with the caller."""
+    nkv heads in the F16, Q8_0 or Q4_0 format. Tables, lengths and positions stay with the caller.
+
+    The calls on a cache run on torch's current stream or on `stream` (a torch stream, or a handle that outlives the call's
+    tensors). There the caller orders the streams as for any torch call; the tensors may be dropped as soon as a call
+    returns."""
 
     def __init__(self, hd: int, nkv: int, quant: int = Q8_0, n_layers: int = 1, n_pages: int = 1, page_keys: int = 256,
                  device: int = 0, rs: int | None = None):
@@ -637,15 +668,19 @@ class CachePlan:
         import torch
         ctx, f32 = self.ctx, torch.float32
         args = self._args(layer, Qs, table, n_keys, q_pos, tree)
-        if out is None:
+        st, side = _stream_on(ctx, stream)
+        if out is None and side is None:
             m = Qs.new_empty(self._rows, dtype=f32)
             out = Qs.new_empty(self._full, dtype=f32), m, torch.empty_like(m)
+        elif out is None:
+            out = _there(side, Qs, (self._full, f32), (self._rows, f32), (self._rows, f32))
         else:
             for t, name, shape in zip(out, ("O", "m", "l"), (self._full, self._rows, self._rows)):
                 _want(ctx, t, name, f32, shape)
         O, m, l = out
-        ctx.check(lib().pa_cuda_cache_attn(*args, O.data_ptr(), m.data_ptr(), l.data_ptr(), _stream_on(ctx, stream)),
-                  "cache_attn")
+        ctx.check(lib().pa_cuda_cache_attn(*args, O.data_ptr(), m.data_ptr(), l.data_ptr(), st), "cache_attn")
+        if side is not None:
+            _keep(side, Qs, table, n_keys, q_pos, tree, *out, self.cache.K, self.cache.V)
         return O, m, l
 
     def reply(self, layer: int, Qs, table, n_keys, q_pos=None, tree=None, out=None, stream=None):
@@ -653,14 +688,18 @@ class CachePlan:
         import torch
         ctx = self.ctx
         args = self._args(layer, Qs, table, n_keys, q_pos, tree)
-        if out is None:
+        st, side = _stream_on(ctx, stream)
+        if out is None and side is None:
             out = torch.empty_like(Qs), Qs.new_empty(self._rows, dtype=torch.float32)
+        elif out is None:
+            out = _there(side, Qs, (self._full, torch.float16), (self._rows, torch.float32))
         else:
             _want(ctx, out[0], "Oh", torch.float16, self._full)
             _want(ctx, out[1], "lse", torch.float32, self._rows)
         Oh, lse = out
-        ctx.check(lib().pa_cuda_cache_attn_reply(*args, Oh.data_ptr(), lse.data_ptr(), _stream_on(ctx, stream)),
-                  "cache_attn_reply")
+        ctx.check(lib().pa_cuda_cache_attn_reply(*args, Oh.data_ptr(), lse.data_ptr(), st), "cache_attn_reply")
+        if side is not None:
+            _keep(side, Qs, table, n_keys, q_pos, tree, *out, self.cache.K, self.cache.V)
         return Oh, lse
 
     def close(self):
@@ -718,15 +757,18 @@ def cache_append(ctx: Context, cache: Cache, layer: int, q, k, v, table, start, 
                 kinds[dt], w_dtype, rot, 1 if interleaved else 0, eps, scale)
     n_rows = nq // cache.nkv * T
     rows = (S, cache.nkv, n_rows, hd)
+    st, side = _stream_on(ctx, stream)
     if out is None:
-        out = q.new_empty(rows, dtype=torch.float16)
+        out = q.new_empty(rows, dtype=torch.float16) if side is None else _there(side, q, (rows, torch.float16))[0]
     else:
         _want(ctx, out, "out", torch.float16, rows)
     pages = table.shape[-1]
     ctx.check(lib().pa_cuda_cache_append(ctx.handle, cache.shape(n_rows or 1), cache.on(ctx), layer, ctypes.byref(a), S, T,
                                          _want(ctx, table, "table", torch.int32, (S, pages)), pages,
                                          _want(ctx, start, "start", torch.int32, (S,)),
-                                         out.data_ptr(), _stream_on(ctx, stream)), "cache_append")
+                                         out.data_ptr(), st), "cache_append")
+    if side is not None:
+        _keep(side, q, k, v, table, start, pos, wq, wk, freqs, out, cache.K, cache.V)
     return out
 
 
@@ -736,16 +778,21 @@ def cache_rows(ctx: Context, cache: Cache, layer: int, table, first, n: int, out
     import torch
     S = table.shape[0]
     shape = (S, n, cache.nkv, cache.hd)
-    if out is None:
+    st, side = _stream_on(ctx, stream)
+    if out is None and side is None:
         K = table.new_empty(shape, dtype=torch.float16)
         out = (K, torch.empty_like(K))
+    elif out is None:
+        out = _there(side, table, (shape, torch.float16), (shape, torch.float16))
     else:
         _want(ctx, out[0], "K", torch.float16, shape)
         _want(ctx, out[1], "V", torch.float16, shape)
     ctx.check(lib().pa_cuda_cache_rows(ctx.handle, cache.shape(1), cache.on(ctx), layer, S, n,
                                        _want(ctx, table, "table", torch.int32, (S, table.shape[1])), table.shape[1],
                                        _want(ctx, first, "first", torch.int32, (S,)),
-                                       out[0].data_ptr(), out[1].data_ptr(), _stream_on(ctx, stream)), "cache_rows")
+                                       out[0].data_ptr(), out[1].data_ptr(), st), "cache_rows")
+    if side is not None:
+        _keep(side, table, first, *out, cache.K, cache.V)
     return out
 
 
@@ -754,10 +801,13 @@ def cache_copy_pages(ctx: Context, cache: Cache, src, dst, stream=None):
     prefix copies the page it will write to. No page is both read and written in one call."""
     import torch
     n = src.numel()
+    st, side = _stream_on(ctx, stream)
     ctx.check(lib().pa_cuda_cache_copy_pages(ctx.handle, cache.shape(1), cache.on(ctx),
                                              _want(ctx, src, "src", torch.int32, (n,)),
-                                             _want(ctx, dst, "dst", torch.int32, (n,)), n, _stream_on(ctx, stream)),
+                                             _want(ctx, dst, "dst", torch.int32, (n,)), n, st),
               "cache_copy_pages")
+    if side is not None:
+        _keep(side, src, dst, cache.K, cache.V)
 
 
 def cache_compact(ctx: Context, cache: Cache, table, start, path, count, out=None, stream=None):
@@ -766,13 +816,16 @@ def cache_compact(ctx: Context, cache: Cache, table, start, path, count, out=Non
     start + count."""
     import torch
     S, T = path.shape
+    st, side = _stream_on(ctx, stream)
     if out is None:
-        out = torch.empty_like(start)
+        out = torch.empty_like(start) if side is None else _there(side, start, (start.shape, start.dtype))[0]
     ctx.check(lib().pa_cuda_cache_compact(ctx.handle, cache.shape(1), cache.on(ctx), S, T,
                                           _want(ctx, table, "table", torch.int32, (S, table.shape[1])), table.shape[1],
                                           _want(ctx, start, "start", torch.int32, (S,)),
                                           _want(ctx, path, "path", torch.int32, (S, T)),
                                           _want(ctx, count, "count", torch.int32, (S,)),
-                                          _want(ctx, out, "out", torch.int32, (S,)), _stream_on(ctx, stream)),
+                                          _want(ctx, out, "out", torch.int32, (S,)), st),
               "cache_compact")
+    if side is not None:
+        _keep(side, table, start, path, count, out, cache.K, cache.V)
     return out

@@ -144,3 +144,75 @@ def test_append_without_positions_reports_keys_out_of_reach(ctx, start, bad):
     # padding is none of this, wherever its sequence starts
     pa.cache_append(ctx, sq.cache, 0, *x, table, st, pos=torch.tensor([[0, 0, 0], [-1, -1, -1]], dtype=torch.int32, device="cuda"))
     ctx.status()
+
+
+def _inputs(sq, x, Qs):
+    """inputs of every call on a cache that nothing else holds, in the order of _all_calls"""
+    import torch
+    table, n = sq.table, sq.n_keys
+    i32 = dict(dtype=torch.int32, device="cuda")
+    S = len(sq.lens)
+    return [[Qs.clone(), table.clone(), n + 0], [Qs.clone(), table.clone(), n + 0], [*(t.clone() for t in x), table.clone(), n - 3],
+            [table.clone(), n - 9], [table[0, :1].clone(), table[1, :1].clone()], [table.clone(), n - n],
+            [table.clone(), n - 3, torch.tensor([[0, 2, 0]] * S, **i32), torch.tensor([2] * S, **i32)]]
+
+
+def _all_calls(ctx, sq, plan, inputs, stream):
+    """every call on a cache, on `stream`; a call's inputs are dropped when it returns"""
+    out = [*plan.reply(sq.layer, *inputs.pop(0), stream=stream)]
+    out += plan.run(sq.layer, *inputs.pop(0), stream=stream)
+    out += [pa.cache_append(ctx, sq.cache, 0, *inputs.pop(0), scale=0.5, stream=stream)]
+    out += pa.cache_rows(ctx, sq.cache, sq.layer, *inputs.pop(0), 9, stream=stream)
+    pa.cache_copy_pages(ctx, sq.cache, *inputs.pop(0), stream=stream)
+    out += pa.cache_rows(ctx, sq.cache, sq.layer, *inputs.pop(0), 5, stream=stream)
+    out += [pa.cache_compact(ctx, sq.cache, *inputs.pop(0), stream=stream)]
+    return out
+
+
+@pytest.mark.parametrize("as_handle", [False, True])
+def test_calls_on_another_stream_own_what_they_use(ctx, as_handle):
+    """`stream=` while the current stream is still reading memory that was given back, and inputs dropped as soon as a call
+    returns: outputs come from elsewhere, and the inputs' memory is not given out before the calls have run"""
+    import torch
+    S, tok, gqa = 2, 4, 5
+    sq = Seqs(51, [300, 130], extra=8)
+    plan = pa.CachePlan(ctx, sq.cache, S, tok, gqa, sq.max_pages)
+    Qs = sq.q(tok, gqa)
+    x = [torch.randn(S, 2, n, 128, generator=sq.g, device="cuda") for n in (40, 8, 8)]
+    pool = [p.clone() for p in (sq.cache.K, sq.cache.V)]
+    want = [t.clone() for t in _all_calls(ctx, sq, plan, _inputs(sq, x, Qs), None)]
+    for p, was in zip((sq.cache.K, sq.cache.V), pool):
+        p.copy_(was)
+    side = torch.cuda.Stream()
+    inputs = _inputs(sq, x, Qs)
+    sizes = [t.numel() for i in inputs for t in i if t.dtype == torch.int32]
+    seven = [torch.full_like(t, 7) for t in want]   # a block of every output's size
+    torch.cuda.synchronize()
+    torch.cuda._sleep(200_000_000)                  # (about 0.1 s)
+    late = [t.clone() for t in seven]               # read late by the current stream, and given back at once
+    del seven
+    with torch.cuda.stream(side):
+        torch.cuda._sleep(600_000_000)              # the calls run after everything below is queued
+    got = _all_calls(ctx, sq, plan, inputs, side.cuda_stream if as_handle else side)
+    junk = [torch.full((n,), 2 ** 30, dtype=torch.int32, device="cuda") for n in sizes for _ in range(4)]
+    torch.cuda.synchronize()
+    ctx.status()
+    assert all(bool((t == 7).all()) for t in late)
+    for a, b in zip(got, want):
+        assert torch.equal(a, b)
+    del junk
+    plan.close()
+
+
+def test_a_stream_of_another_device_is_refused(ctx):
+    import torch
+
+    class Other(torch.cuda.Stream):   # (one GPU is enough to ask for it)
+        device_index = 1
+
+    sq = Seqs(52, [30, 10])
+    plan = pa.CachePlan(ctx, sq.cache, 2, 1, 5, sq.max_pages)
+    with pytest.raises(pa.PaCudaError) as e:
+        plan.reply(0, sq.q(1, 5), sq.table, sq.n_keys, stream=Other())
+    assert e.value.code == api.EINVAL
+    plan.close()
