@@ -226,7 +226,8 @@ class Context:
             raise PaCudaError(rc, f"{what}: {msg}" if what else msg)
 
     def status(self, stream=None):
-        """Synchronise the stream and raise if a kernel gave up a bounded wait (pa_cuda_status)."""
+        """Synchronise the stream and raise if a kernel gave up a bounded wait (ETIMEOUT) or a cache call met an argument out
+        of range on the device (EINVAL); after both, the next call raises the second (pa_cuda_status)."""
         self.check(lib().pa_cuda_status(self._h, _stream_ptr(stream)), "status")
 
     def set_timeout_ns(self, ns: int):

@@ -794,14 +794,12 @@ int pa_cuda_status(pa_cuda_ctx *ctx, void *stream) {
     PA_CK(cudaMemcpyAsync(ctx->h_status, ctx->d_status, 2 * sizeof(int), cudaMemcpyDeviceToHost, st), "status read");
     PA_CK(cudaStreamSynchronize(st), "stream synchronize");
     const int h = ctx->h_status[0], args = ctx->h_status[1];
-    if (h != pa::ST_OK || args != pa::ST_OK) {
-        PA_CK(cudaMemsetAsync(ctx->d_status, 0, 2 * sizeof h, st), "status clear");
-        PA_CK(cudaStreamSynchronize(st), "stream synchronize");
-        if (h == pa::ST_OK)
-            return fail(ctx, PA_CUDA_EINVAL, "a cache call met a page id, length or path out of range on the device");
-        return fail(ctx, PA_CUDA_ETIMEOUT, "a kernel gave up a bounded wait (code " + std::to_string(h) + ")");
-    }
-    return PA_CUDA_OK;
+    if (h == pa::ST_OK && args == pa::ST_OK) return PA_CUDA_OK;
+    // the word that is reported is cleared; the other one is the next call's
+    PA_CK(cudaMemsetAsync(ctx->d_status + (h != pa::ST_OK ? 0 : 1), 0, sizeof h, st), "status clear");
+    PA_CK(cudaStreamSynchronize(st), "stream synchronize");
+    if (h != pa::ST_OK) return fail(ctx, PA_CUDA_ETIMEOUT, "a kernel gave up a bounded wait (code " + std::to_string(h) + ")");
+    return fail(ctx, PA_CUDA_EINVAL, "a cache call met a page id, length or path out of range on the device");
 }
 
 int pa_cuda_plan_create(pa_cuda_ctx *ctx, const pa_cuda_shape *shape, uint32_t n_sets, const pa_cuda_seg *segs,

@@ -89,7 +89,7 @@ void pa_cuda_destroy(pa_cuda_ctx *ctx);
 const char *pa_cuda_last_error(const pa_cuda_ctx *ctx);
 /* Synchronise `stream` (a cudaStream_t; NULL = the context's stream), then return and clear the device status word:
  * PA_CUDA_OK, PA_CUDA_ETIMEOUT if a kernel gave up a bounded wait since the last call, or PA_CUDA_EINVAL if a paged-cache
- * kernel met an argument out of range. */
+ * kernel met an argument out of range. After both, the first call returns PA_CUDA_ETIMEOUT and the next PA_CUDA_EINVAL. */
 int pa_cuda_status(pa_cuda_ctx *ctx, void *stream);
 /* Bound on every in-kernel wait (default 2 s). */
 void pa_cuda_set_timeout_ns(pa_cuda_ctx *ctx, uint64_t ns);

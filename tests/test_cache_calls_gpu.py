@@ -216,3 +216,32 @@ def test_a_stream_of_another_device_is_refused(ctx):
         plan.reply(0, sq.q(1, 5), sq.table, sq.n_keys, stream=Other())
     assert e.value.code == api.EINVAL
     plan.close()
+
+
+def test_status_reports_a_wait_and_a_bad_argument(ctx):
+    """a wait that ran out and an argument out of range, both since the last look: one after the other, then neither"""
+    import torch
+    sq = Seqs(61, [300, 80])
+    x = [torch.randn(2, 1, n, 128, generator=sq.g, device="cuda") for n in (40, 8, 8)]
+    ctx.set_kernel(1)
+    plan = pa.CachePlan(ctx, sq.cache, 2, 1, 5, sq.max_pages)
+    ctx.set_kernel(0)
+    Qs = sq.q(1, 5)
+    ctx.set_timeout_ns(20_000_000)
+    ctx.set_stall_test(True)
+    try:
+        plan.reply(sq.layer, Qs, sq.table, sq.n_keys)
+        torch.cuda.synchronize()
+    finally:
+        ctx.set_stall_test(False)
+        ctx.set_timeout_ns(2_000_000_000)
+    pa.cache_append(ctx, sq.cache, 0, *x, sq.table, torch.tensor([-1, 0], dtype=torch.int32, device="cuda"))
+    for code in (api.ETIMEOUT, api.EINVAL):
+        with pytest.raises(pa.PaCudaError) as e:
+            ctx.status()
+        assert e.value.code == code
+    ctx.status()
+    out = plan.reply(sq.layer, Qs, sq.table, sq.n_keys)
+    ctx.status()
+    _check(sq, Qs, out, 1, 5)
+    plan.close()
