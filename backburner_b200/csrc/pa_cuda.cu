@@ -149,6 +149,7 @@ int fail(pa_cuda_ctx *ctx, int code, const std::string &msg) {
     return code;
 }
 int cuda_fail(pa_cuda_ctx *ctx, cudaError_t e, const char *what) {
+    cudaGetLastError();   // reported here, and not left for the thread's next CUDA call, whoever makes it
     return fail(ctx, PA_CUDA_ECUDA, std::string(what) + ": " + cudaGetErrorString(e));
 }
 #define PA_CK(call, what)                                    \

@@ -245,3 +245,32 @@ def test_status_reports_a_wait_and_a_bad_argument(ctx):
     ctx.status()
     _check(sq, Qs, out, 1, 5)
     plan.close()
+
+
+def test_a_failed_launch_leaves_no_error_behind(ctx):
+    """a launch that CUDA refuses (the legacy stream while a blocking stream captures) is the call's error and nobody else's"""
+    import ctypes
+    import torch
+    sq = Seqs(71, [300, 80])
+    plan = pa.CachePlan(ctx, sq.cache, 2, 1, 5, sq.max_pages)
+    Qs = sq.q(1, 5)
+    out = plan.reply(sq.layer, Qs, sq.table, sq.n_keys)
+    torch.cuda.synchronize()
+    with open("/proc/self/maps") as f:
+        rt = ctypes.CDLL(next(line.split()[-1] for line in f if "libcudart" in line))
+    stream, graph = ctypes.c_void_p(), ctypes.c_void_p()
+    assert rt.cudaStreamCreate(ctypes.byref(stream)) == 0
+    assert rt.cudaStreamBeginCapture(stream, 0) == 0
+    try:
+        with pytest.raises(pa.PaCudaError) as e:
+            plan.reply(sq.layer, Qs, sq.table, sq.n_keys, out=out, stream=1)
+        left = rt.cudaPeekAtLastError()
+    finally:
+        rt.cudaStreamEndCapture(stream, ctypes.byref(graph))   # (invalidated by the refused launch)
+        rt.cudaGetLastError()
+        rt.cudaStreamDestroy(stream)
+    assert e.value.code == api.ECUDA and left == 0
+    again = plan.reply(sq.layer, Qs, sq.table, sq.n_keys)
+    ctx.status()
+    assert all(torch.equal(a, b) for a, b in zip(again, out))
+    plan.close()
