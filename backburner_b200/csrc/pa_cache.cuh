@@ -192,18 +192,22 @@ __global__ void __launch_bounds__(256) cache_merge_kernel(const MergeParams p) {
         }
     }
     if (!active) return;
+    // L is 0 where the row sees nothing, and NaN (a part's l is) where its scores are not numbers: no value then
     if constexpr (REPLY) {
-        const float inv = L > 0.f ? 1.f / L : 0.f;
+        const float inv = L == 0.f ? 0.f : 1.f / L;
 #pragma unroll
         for (int q = 0; q < V; q += 2)
             *reinterpret_cast<uint32_t *>(p.Oh + row * HD + lane * V + q) = pack_h2(acc[q] * inv, acc[q + 1] * inv);
-        if (lane == 0) p.lse[row] = L > 0.f ? M + logf(L) : -INFINITY;
+        if (lane == 0) p.lse[row] = L == 0.f ? -INFINITY : M + logf(L);
     } else {
+        if (!(L >= 0.f))
+#pragma unroll
+            for (int q = 0; q < V; q++) acc[q] = L;
 #pragma unroll
         for (int q = 0; q < V / 4; q++)
             reinterpret_cast<float4 *>(p.O + row * HD + lane * V)[q] = make_float4(acc[4 * q], acc[4 * q + 1], acc[4 * q + 2], acc[4 * q + 3]);
         if (lane == 0) {
-            p.M[row] = L > 0.f ? M : -INFINITY;
+            p.M[row] = L > 0.f ? M : L == 0.f ? -INFINITY : L;
             p.L[row] = L;
         }
     }

@@ -274,7 +274,8 @@ typedef struct pa_cuda_cache {
  *   tree = 1: the tokens are drafted and n_tok <= 64; token t sees the keys before q0 (with window > 0 those with
  *     j > q0 + depth - window or j < sinks, depth = the bits set in its mask less one; window >= n_tok) and the drafted
  *     keys q0 + u for which bit u of tree[s][t] is set (its ancestors and itself). A mask of 0 marks padding: it sees nothing.
- * A token that sees nothing has m = -inf, l = 0 (lse = -inf) and O = 0. */
+ * A token that sees nothing has m = -inf, l = 0 (lse = -inf) and O = 0. One with NaN among its scores (its query or a key that
+ * it sees is not finite) has NaN in all of them (pa_cuda_merge and pa_cuda_normalize take such a partial for an empty one). */
 typedef struct pa_cuda_mask {
     uint32_t n_tok, window, sinks, tree;
 } pa_cuda_mask;

@@ -274,3 +274,39 @@ def test_a_failed_launch_leaves_no_error_behind(ctx):
     ctx.status()
     assert all(torch.equal(a, b) for a, b in zip(again, out))
     plan.close()
+
+
+@pytest.mark.parametrize("kernel,quant,hd,nkv", [(1, pa.Q8_0, 128, 8), (1, pa.F16, 256, 4), (2, pa.Q8_0, 128, 8), (2, pa.Q4_0, 256, 4),
+                                                 (3, pa.Q8_0, 128, 8)])
+def test_scores_that_are_not_numbers_give_nan(ctx, kernel, quant, hd, nkv):
+    """a query row with a NaN or an infinity, and a key with NaN that every token sees: NaN, not an empty row's zeros; the
+    other rows and heads as they are, and a key outside the window changes nothing"""
+    import torch
+    tok, gqa, W = 5, 5, 700
+    sq = Seqs(81, [2000, 900], hd, nkv, quant, 64)
+    ctx.set_kernel(kernel)
+    plan = pa.CachePlan(ctx, sq.cache, 2, tok, gqa, sq.max_pages, W, 3)
+    ctx.set_kernel(0)
+    Qs = sq.q(tok, gqa)
+    clean = plan.reply(sq.layer, Qs, sq.table, sq.n_keys)
+    _check(sq, Qs, clean, tok, gqa, W, 3)
+    bad = torch.zeros(2, nkv, gqa * tok, dtype=torch.bool, device="cuda")
+    Qb = Qs.clone()
+    for s, h, r, d, x in ((0, 0, 0, 0, float("nan")), (0, 1, 24, hd - 1, float("nan")), (1, nkv - 1, 7, 5, float("inf"))):
+        Qb[s, h, r, d] = x
+        bad[s, h, r] = True
+    K = sq.cache.K[sq.layer].view(-1, sq.cache.rs)
+    at = sq.rows(0, [1999 - 400])[0]
+    K[at, 2 * sq.hb:2 * sq.hb + 2] = 0x7E   # f16 0x7e7e is NaN: d of head 2's first block, or its first value
+    bad[0, 2] = True
+    K[sq.rows(0, [1000])[0], :2] = 0x7E     # no token's
+    Oh, lse = plan.reply(sq.layer, Qb, sq.table, sq.n_keys)
+    O, m, l = plan.run(sq.layer, Qb, sq.table, sq.n_keys)
+    ctx.status()
+    for t in (lse, l, m):
+        assert torch.equal(torch.isnan(t), bad)
+    for t in (Oh, O):
+        assert torch.equal(torch.isnan(t), bad[..., None].expand_as(t))
+    assert bool(((Oh - clean[0]).abs()[~bad] <= 2.0 ** -10 * clean[0].abs().amax()).all())
+    assert bool(((lse - clean[1]).abs()[~bad] <= 2.0 ** -18 * clean[1].abs().amax()).all())
+    plan.close()
