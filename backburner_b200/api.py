@@ -551,6 +551,12 @@ def _want(ctx: Context, t, name: str, dtype, shape):
     return t.data_ptr()
 
 
+def _layer(cache, layer: int) -> int:
+    if not 0 <= layer < cache.n_layers:   # (ctypes would take it modulo 2^32)
+        raise PaCudaError(EINVAL, f"layer {layer} of a cache of {cache.n_layers}")
+    return layer
+
+
 def _stream_on(ctx: Context, stream):
     """_stream_ptr for the context's device, whatever the current one is; and the torch stream where it is another than the
     device's current one (else None)."""
@@ -642,6 +648,10 @@ class CachePlan:
         self.ctx, self.cache, self.n_sets, self.n_tok, self.gqa = ctx, cache, n_sets, n_tok, gqa
         self.max_pages, self.tree = max_pages, bool(tree)
         self._h = _P()
+        for name, x in dict(n_sets=n_sets, n_tok=n_tok, gqa=gqa, max_pages=max_pages, window=window, sinks=sinks,
+                            rows=gqa * n_tok).items():
+            if not 0 <= x < 1 << 32:   # (ctypes would take it modulo 2^32)
+                raise PaCudaError(EINVAL, f"CachePlan: {name} = {x}")
         mask = _Mask(n_tok, window, sinks, 1 if tree else 0)
         ctx.check(lib().pa_cuda_cache_plan_create(ctx.handle, cache.shape(gqa * n_tok), cache.on(ctx), n_sets, max_pages,
                                                   ctypes.byref(mask), ctypes.byref(self._h)), "cache_plan_create")
@@ -658,7 +668,7 @@ class CachePlan:
         ctx, i32, per = self.ctx, torch.int32, (self.n_sets,)
         if (tree is not None) != self.tree:
             raise PaCudaError(EINVAL, "a tree plan takes the tree's masks, another plan none")
-        return (self._h, layer, _want(ctx, Qs, "Qs", torch.float16, self._full),
+        return (self._h, _layer(self.cache, layer), _want(ctx, Qs, "Qs", torch.float16, self._full),
                 _want(ctx, table, "table", i32, (self.n_sets, self.max_pages)), _want(ctx, n_keys, "n_keys", i32, per),
                 None if q_pos is None else _want(ctx, q_pos, "q_pos", i32, per),
                 None if tree is None else _want(ctx, tree, "tree", torch.int64, (self.n_sets, self.n_tok)))
@@ -764,7 +774,8 @@ def cache_append(ctx: Context, cache: Cache, layer: int, q, k, v, table, start, 
     else:
         _want(ctx, out, "out", torch.float16, rows)
     pages = table.shape[-1]
-    ctx.check(lib().pa_cuda_cache_append(ctx.handle, cache.shape(n_rows or 1), cache.on(ctx), layer, ctypes.byref(a), S, T,
+    ctx.check(lib().pa_cuda_cache_append(ctx.handle, cache.shape(n_rows or 1), cache.on(ctx), _layer(cache, layer),
+                                         ctypes.byref(a), S, T,
                                          _want(ctx, table, "table", torch.int32, (S, pages)), pages,
                                          _want(ctx, start, "start", torch.int32, (S,)),
                                          out.data_ptr(), st), "cache_append")
@@ -788,7 +799,7 @@ def cache_rows(ctx: Context, cache: Cache, layer: int, table, first, n: int, out
     else:
         _want(ctx, out[0], "K", torch.float16, shape)
         _want(ctx, out[1], "V", torch.float16, shape)
-    ctx.check(lib().pa_cuda_cache_rows(ctx.handle, cache.shape(1), cache.on(ctx), layer, S, n,
+    ctx.check(lib().pa_cuda_cache_rows(ctx.handle, cache.shape(1), cache.on(ctx), _layer(cache, layer), S, n,
                                        _want(ctx, table, "table", torch.int32, (S, table.shape[1])), table.shape[1],
                                        _want(ctx, first, "first", torch.int32, (S,)),
                                        out[0].data_ptr(), out[1].data_ptr(), st), "cache_rows")
