@@ -1,6 +1,7 @@
-// pa_cache.cuh - a paged device cache of quantised (or f16) key/value rows: which keys a query token sees (sliding
-// window with sinks, or a tree of drafted tokens), the append of new rows (head norm, rotation, quantisation), reading
-// rows back, copying pages and compacting accepted rows.
+// pa_cache.cuh - a paged device cache of quantised (or f16) key/value rows: the dealing of many units and the merge of the
+// attention's partials, the append of new rows (head norm, rotation, quantisation), reading rows back, copying pages and
+// compacting accepted rows. (Which keys a query token sees: pa_mask.cuh; the attention kernels: pa_decode.cuh, pa_prefill.cuh,
+// pa_prefill_pair.cuh.)
 //
 // The cache: rows of layer i, page p, position j at base + ((i * n_pages + p) * page_keys + j) * rs, K and V alike, each
 // row nkv heads of hb bytes (the row formats of pa_decode.cuh). The keys of sequence s are numbered 0, 1, ...; key j lies in
@@ -318,8 +319,10 @@ constexpr int APPEND_WARPS = 4;
 __host__ __device__ constexpr int append_heads(int hd) { return APPEND_WARPS * 256 / hd; }
 // Block = token x STEPS * append_heads heads. The heads are numbered queries, then keys, then values, each kind rounded up to
 // whole warps, so that a warp's step is of one kind. A warp loads all its heads before it works on the first, and the loads
-// fly while the block computes the token's angles. Bound: for long prompts memory (the loads alone run at 6 TB/s) and issue
-// (60 instructions a query head's warp step, 160 a key's); for single tokens a chain of a few loads.
+// fly while the block computes the token's angles. Bound: for long prompts issue (2 x 8,191 tokens of 40 + 8 + 8 heads, bf16 to
+// Q8_0: 5,040 warp instructions a token, half of them in the heads' steps of 60 for queries and 160 for keys, the rest the
+// token's own angles, weights, row and addresses; issue slots 65 % busy; the loads alone run at 6 TB/s); for single tokens a
+// chain of a few loads.
 // How a head's pairs meet: halves, by a shuffle to the lane half / 8 away (HALVES: half a multiple of 8); within a lane
 // (PAIRS: interleaved); through shared memory, for any rot, order and alignment (ANY). A template, since the compiler runs
 // the paths not taken as predicated instructions.

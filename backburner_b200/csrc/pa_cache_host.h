@@ -288,7 +288,11 @@ int shape_cache_plan(pa_cuda_cache_plan *p) {
         // CTA pairs (512 rows a unit at hd 128) run a row of a group in 7/8 of the single-CTA kernel's time, if their rows are
         // real and the keys long: us single vs pair, 8 KV heads, 65,536 Q8_0 keys: 305 rows 159 vs 147, 640 rows 225 vs 308, 2,560
         // rows 884 vs 849; 2,560 rows over a window of 1,024 keys 51 vs 56, of 4,096 102 vs 98 (Q4_0 91 vs 96). hd 256, where
-        // the single-CTA kernel has one tile: 240 rows x 4,096 keys 26.7 vs 24.6, 768 x 16,384 76 vs 67
+        // the single-CTA kernel has one tile: 240 rows x 4,096 keys 26.7 vs 24.6, 768 x 16,384 76 vs 67. Between those lengths,
+        // 64 / 128 / 256 / 512 groups: 305 rows 25.7 vs 25.0, 33.0 vs 33.3, 51 vs 50, 92 vs 84; 512 rows 26.4 vs 26.4, 35.5 vs 34.7,
+        // 53 vs 51, 95 vs 90; 640 rows 30 vs 36, 43 vs 54, 69 vs 90, 130 vs 171; 2,560 rows 82 vs 86, 131 vs 134, 228 vs 228, 461 vs 461;
+        // hd 256, 128 and 512 groups: 144 rows 27 vs 25, 56 vs 50, 384 rows 36 vs 38, 79 vs 86, 768 rows 47 vs 44, 134 vs 120. The
+        // rule's choice is within 3 % of the better one at most of them, 9 % off at worst (hd 256, 384 rows)
         const uint64_t in_pairs = ((uint64_t) sh.rows + 511) / 512 * 512, left = sh.rows % 256;
         const uint64_t single = (uint64_t) sh.rows / 256 * 256 + (left == 0 ? 0 : left <= 128 ? 224 : 256);
         const bool better = sh.hd == 256 ? sh.rows > kSingle256MaxRows : sh.rows >= kPairMinRows && groups >= 128 && 7 * in_pairs <= 8 * single;

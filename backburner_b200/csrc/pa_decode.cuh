@@ -26,18 +26,15 @@
 //   * P is taken against a lazily raised reference max (one warp vote per tile; the cross-lane max and the O rescale
 //     run only when a score passes the reference by 2^8), and the exact row max is restored once per job; a tile's V
 //     words are loaded before its softmax so their shared-memory latency overlaps the softmax.
-//   * PAGED: the same over a paged cache (pa_mask.cuh). A CTA walks its part's 16-key groups, each in one page, whose row
-//     the warps look up two stages ahead; only the groups at the edge of what the rows see are masked, and there V rows
-//     that no row sees get a zero scale. The work is short there (a window), so that its ends count: see the loads of Q
-//     and the stores of O.
 //   * QUANT 3: Q8_0 rows with the int8-domain QK of scripts/sme/sme_attn.c:465-508 (sme_qk_i8blk + i8_combine): Q is
 //     quantised per 32-block by the Q8_0 rule (d = f16(max|x| / 127), q = rint(x / d)) when a job starts, one
 //     mma.m16n8k32 s8 per quant block gives the block's exact int32 dot products T for 16 keys x 8 rows, and
 //     s = sum_b float(T_b) * (dq_b * dk_b) in block order (fma). Softmax and P.V are those of QUANT 1.
 //   * PAGED: the keys come from a paged cache and the rows see them through a mask (pa_mask.cuh). A CTA finds its part of
-//     its set's visible 16-key groups on the device; pages hold whole stages, so a stage is copied whole. Only stages at the
-//     edge of what the rows see compute the mask (one 64-bit word per row, from its range and its tree bits); keys no row of
-//     the warp sees get a zero V scale, since their rows may hold NaN.
+//     its set's visible 16-key groups on the device; pages hold whole stages, so a stage is copied whole, and its row is
+//     looked up NSTAGE stages ahead. Only stages at the edge of what the rows see compute the mask (one 64-bit word per row,
+//     from its range and its tree bits); keys no row of the warp sees get a zero V scale, since their rows may hold NaN. The
+//     work is short there (a window), so that its ends count: see the loads of Q and the stores of O.
 #pragma once
 #include "pa_common.cuh"
 #include "pa_mask.cuh"

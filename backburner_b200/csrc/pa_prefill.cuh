@@ -279,8 +279,8 @@ __device__ __forceinline__ void convert_block(const uint32_t (&w)[12], uint32_t 
 
 // PAGED: the keys come from a paged cache and the rows see them through a mask (pa_mask.cuh). A block is B / 64 groups of 64
 // keys, each copied from its own page; the CTA walks its share of the groups its own row tile sees. Only groups at the edge of
-// what the tile's rows see are masked (a thread has its row's 64-bit word for the group); keys no row of the tile sees get a
-// zero V scale in the dequantisers, since their rows may hold NaN (a masked K row only reaches its own masked scores).
+// what the tile's rows see are masked (a thread has its row's 64-bit word for the group); the converted V rows of keys that no
+// row of the tile sees are cleared by the dequantisers, since they may hold NaN (a masked K row only reaches its own masked scores).
 template <int QUANT, int NT, int D = 128, bool PAGED = false>
 __global__ void __launch_bounds__(32 * cta_warps(NT), 1) prefill_kernel(const __grid_constant__ CUtensorMap tq,
                                                                        const typename ParamsOf<PAGED>::type p) {
@@ -304,8 +304,8 @@ __global__ void __launch_bounds__(32 * cta_warps(NT), 1) prefill_kernel(const __
     static_assert(NSB == 1 && NPB == 2 && T_O + D <= (NT == 1 ? T_Q : 256u) && T_Q + (QT ? D / 2 : 0) <= TCOLS,
                   "tensor memory layout");
     static_assert(!QT || NT == 1, "Q in tensor memory with one tile only");
-    // dequant items loaded ahead and maxima in four chains: measured with and without, us a call over a plan's segments (Q4_0 80
-    // rows x 4 x 196,608 keys 509 vs 537; Q8_0 200 rows x 4 x 65,536 303 vs 298; hd 256 48 rows x 8 x 32,768 177 vs 173) and over
+    // dequant items loaded ahead and maxima in four chains: us a call with and without, over a plan's segments (Q4_0 80 rows x
+    // 4 x 196,608 keys 509 vs 537; Q8_0 200 rows x 4 x 65,536 303 vs 298; hd 256 48 rows x 8 x 32,768 177 vs 173) and over
     // the paged cache (Q4_0: 512 tokens x 5 heads, window 4,096: 91 vs 93; hd 256, 8 trees of 16 tokens x 6 heads, 16,301 keys: 75 vs 73)
     constexpr bool AHEAD = D == 128 && (NT == 1 || PAGED);
     // column of P buffer i (relative to the tile)

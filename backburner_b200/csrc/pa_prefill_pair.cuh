@@ -26,8 +26,8 @@
 // (CTA-scope) release, as CUTLASS's cluster barriers arrive on a peer: a cluster-scope release arrive measured
 // 500-775 ns under this kernel's load against ~80 ns, and a relay thread issuing those serialised the pipeline. No TMA
 // copy multicasts.
-// PAGED: the same over a paged cache, as in pa_prefill.cuh; each CTA of the pair works out the pair's part and masks for its
-// own rows.
+// PAGED: the same over a paged cache, as in pa_prefill.cuh; CTA 0 finds the pair's part and CTA 1 copies it, and each works out
+// the masks of its own rows.
 // All waits are bounded; both CTAs reach the final cluster barrier on every path, so neither exits while the other
 // can still reach its shared memory, and TMEM is released by both.
 #pragma once

@@ -283,7 +283,7 @@ typedef struct pa_cuda_mask {
 typedef struct pa_cuda_cache_plan pa_cuda_cache_plan;
 /* A plan fixes the geometry (shape->rows = GQA group x n_tok rows per KV head, row g * n_tok + t) and owns the workspace
  * of its calls: calls of one plan must not overlap (two streams, two captured graphs replayed at once: two plans). The
- * cache's memory outlives the plan.
+ * cache's memory outlives the plan. It allocates and copies: not under a capture.
  * Reads pa_cuda_set_kernel as pa_cuda_plan_create does; the int8-domain QK is refused. */
 int pa_cuda_cache_plan_create(pa_cuda_ctx *ctx, const pa_cuda_shape *shape, const pa_cuda_cache *cache, uint32_t n_sets,
                               uint32_t max_pages, const pa_cuda_mask *mask, pa_cuda_cache_plan **out);
@@ -293,7 +293,10 @@ void pa_cuda_cache_plan_destroy(pa_cuda_cache_plan *plan);
 /* Attention of every set over one layer. Qs: f16(q * scale) [n_sets][nkv][rows][hd]; table, n_keys [n_sets], q_pos [n_sets]
  * or NULL, tree [n_sets][n_tok] (tree plans) or NULL: device. Gives the unnormalised partial O [n_sets][nkv][rows][hd],
  * m, l [n_sets][nkv][rows], which pa_cuda_merge folds with other partials of the same queries; the _reply form gives
- * f16(O / l) and lse = m + log l, as pa_cuda_normalize. Asynchronous, capturable. */
+ * f16(O / l) and lse = m + log l, as pa_cuda_normalize. Scores, m, l and the sums are held in fp32; P = exp(s - m) is rounded to
+ * f16 for the product with V, as in the other attention calls, so that an output is off by up to 2^-11 of sum(P |V|) / l beside its
+ * own rounding to f16. The order of the sums follows the plan and the lengths: the same call gives the same bits, another split
+ * of the same keys need not. Asynchronous, capturable. */
 int pa_cuda_cache_attn(pa_cuda_cache_plan *plan, uint32_t layer, const uint16_t *Qs, const int32_t *table, const int32_t *n_keys,
                        const int32_t *q_pos, const uint64_t *tree, float *O, float *m, float *l, void *stream);
 int pa_cuda_cache_attn_reply(pa_cuda_cache_plan *plan, uint32_t layer, const uint16_t *Qs, const int32_t *table,
