@@ -586,19 +586,23 @@ def _there(side, like, *kinds):
 
 
 def _keep(side, *tensors):
-    """What a call on a stream of its own reads and writes is not given out again before that stream is done with it."""
-    for t in tensors:
-        if t is not None:
-            t.record_stream(side)
+    """What a call on a stream of its own reads and writes is not given out again before that stream is done with it. Only for
+    streams that torch owns: the allocator uses the stream when the tensor is freed (a cache's rows perhaps long after), and
+    another's may have been destroyed by then."""
+    import torch
+    if not isinstance(side, torch.cuda.ExternalStream):
+        for t in tensors:
+            if t is not None:
+                t.record_stream(side)
 
 
 class Cache:
     """A paged device cache (pa_cuda_cache): K and V uint8 [n_layers][n_pages][page_keys][row bytes] on one device, rows of
     nkv heads in the F16, Q8_0 or Q4_0 format. Tables, lengths and positions stay with the caller.
 
-    The calls on a cache run on torch's current stream or on `stream` (a torch stream, or a handle that outlives the call's
-    tensors). There the caller orders the streams as for any torch call; the tensors may be dropped as soon as a call
-    returns."""
+    The calls on a cache run on torch's current stream or on `stream`, whose order with other streams is the caller's. With a
+    torch stream the tensors may be dropped as soon as a call returns; with another's stream (a handle, an ExternalStream)
+    the caller keeps them until the call has run."""
 
     def __init__(self, hd: int, nkv: int, quant: int = Q8_0, n_layers: int = 1, n_pages: int = 1, page_keys: int = 256,
                  device: int = 0, rs: int | None = None):

@@ -158,7 +158,7 @@ def _inputs(sq, x, Qs):
 
 
 def _all_calls(ctx, sq, plan, inputs, stream):
-    """every call on a cache, on `stream`; a call's inputs are dropped when it returns"""
+    """every call on a cache, on `stream`; a call's inputs are dropped when it returns, unless the caller holds them"""
     out = [*plan.reply(sq.layer, *inputs.pop(0), stream=stream)]
     out += plan.run(sq.layer, *inputs.pop(0), stream=stream)
     out += [pa.cache_append(ctx, sq.cache, 0, *inputs.pop(0), scale=0.5, stream=stream)]
@@ -171,8 +171,8 @@ def _all_calls(ctx, sq, plan, inputs, stream):
 
 @pytest.mark.parametrize("as_handle", [False, True])
 def test_calls_on_another_stream_own_what_they_use(ctx, as_handle):
-    """`stream=` while the current stream is still reading memory that was given back, and inputs dropped as soon as a call
-    returns: outputs come from elsewhere, and the inputs' memory is not given out before the calls have run"""
+    """`stream=` while the current stream is still reading memory that was given back, and (torch's streams) inputs dropped as
+    soon as a call returns: outputs come from elsewhere, and the inputs' memory is not given out before the calls have run"""
     import torch
     S, tok, gqa = 2, 4, 5
     sq = Seqs(51, [300, 130], extra=8)
@@ -193,6 +193,7 @@ def test_calls_on_another_stream_own_what_they_use(ctx, as_handle):
     del seven
     with torch.cuda.stream(side):
         torch.cuda._sleep(600_000_000)              # the calls run after everything below is queued
+    held = [list(i) for i in inputs] if as_handle else None   # (of another's stream the caller keeps them)
     got = _all_calls(ctx, sq, plan, inputs, side.cuda_stream if as_handle else side)
     junk = [torch.full((n,), 2 ** 30, dtype=torch.int32, device="cuda") for n in sizes for _ in range(4)]
     torch.cuda.synchronize()
@@ -200,7 +201,41 @@ def test_calls_on_another_stream_own_what_they_use(ctx, as_handle):
     assert all(bool((t == 7).all()) for t in late)
     for a, b in zip(got, want):
         assert torch.equal(a, b)
-    del junk
+    del junk, held
+    plan.close()
+
+
+@pytest.mark.parametrize("external", [False, True])
+def test_a_stream_that_torch_does_not_own_may_end_before_the_tensors(ctx, external):
+    """calls on a stream of the caller's, which is destroyed while the cache, the inputs and the outputs live on: freeing them
+    later does not touch it"""
+    import ctypes
+    import torch
+    with open("/proc/self/maps") as f:
+        rt = ctypes.CDLL(next(line.split()[-1] for line in f if "libcudart" in line))
+    sq = Seqs(53, [300, 130], extra=8)
+    plan = pa.CachePlan(ctx, sq.cache, 2, 4, 5, sq.max_pages)
+    Qs = sq.q(4, 5)
+    x = [torch.randn(2, 2, n, 128, generator=sq.g, device="cuda") for n in (40, 8, 8)]
+    inputs = _inputs(sq, x, Qs)
+    held = [list(i) for i in inputs]
+    # (no tensor has the stream on record, so that no free can meet it: looked at before the stream is destroyed)
+    kept = []
+    record, torch.Tensor.record_stream = torch.Tensor.record_stream, lambda t, s: kept.append(s)
+    torch.cuda.synchronize()
+    own = ctypes.c_void_p()
+    assert rt.cudaStreamCreate(ctypes.byref(own)) == 0
+    try:
+        out = _all_calls(ctx, sq, plan, inputs, torch.cuda.ExternalStream(own.value) if external else own.value)
+    finally:
+        torch.Tensor.record_stream = record
+        torch.cuda.synchronize()
+        assert rt.cudaStreamDestroy(own) == 0
+    ctx.status()
+    assert own.value not in [s.cuda_stream for s in kept]
+    want = plan.reply(sq.layer, held[0][0], sq.table, sq.n_keys)
+    assert out[0].shape == want[0].shape
+    del out, held, sq
     plan.close()
 
 
